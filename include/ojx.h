@@ -319,6 +319,122 @@ int ojx_attention(void* out, const void* q, const void* k, const void* v, int32_
 #define OJX_ATTN_FLAG_TWO_QTILE 0x4 /* fused kernel with two 128-query tiles per CTA (ping-pong;
                                        the default) */
 
+/* ── serving: norms and rotations of queries and keys, a quantised paged cache,
+ * attention of new or drafted tokens over it, verification of drafts.  No counterpart
+ * in the reference.  All calls are asynchronous on s.  Index arrays live on the device;
+ * one found out of its range there is skipped and reported by the next
+ * ojx_poll_device_error as OJX_ERR_INVALID.  ────────────────────────────────────── */
+
+/* element formats of a cache: 16-bit floats (the dtype's own code), or 8 bits with one
+ * fp32 step per row (one head of one token): int8 holds round(x / step), e4m3 the
+ * nearest 8-bit float of x / step, step = max|x| / 127 or / 448 */
+enum { OJX_KV_BF16 = OJX_BF16, OJX_KV_F16 = OJX_F16, OJX_KV_INT8 = 3, OJX_KV_FP8 = 4 };
+
+/* Pages of keys and values: [num_pages][kv_heads][page_size][head_dim] each, and for
+ * the 8-bit formats [num_pages][kv_heads][page_size] steps.  Token slot s is row
+ * s % page_size of page s / page_size.  head_dim: a multiple of 16, at most 512; k and v
+ * 16-byte aligned. */
+typedef struct ojx_kv_cache {
+  void* k;
+  void* v;
+  float* k_scale; /* NULL for the 16-bit formats */
+  float* v_scale;
+  int64_t num_pages;
+  int32_t page_size, kv_heads, head_dim, format;
+} ojx_kv_cache;
+
+/* Rows of a [tokens][heads][head_dim] tensor are `head_dim` consecutive elements;
+ * tokens and heads are stride_t and stride_h elements apart. */
+typedef struct ojx_rows {
+  const void* data;
+  int64_t stride_t, stride_h;
+} ojx_rows;
+
+/* y = rotate(weight * x / sqrt(mean(x^2) + eps)) of every query and key head; element
+ * pairs (i, i + rotary_dim/2), or (2i, 2i + 1) when interleaved, turn by the angle whose
+ * cosine and sine are table[position][i] and table[position][rotary_dim/2 + i].
+ * A token whose position lies outside the table gives NaN. */
+typedef struct ojx_qk_desc {
+  int64_t tokens;
+  int32_t q_heads, kv_heads, head_dim, rotary_dim;
+  int32_t interleaved, dtype, dtype_weight, positions_int64;
+  float eps;
+  int32_t reserved;
+  ojx_rows q, k;
+  const void* q_weight; /* [head_dim]; NULL: ones */
+  const void* k_weight;
+  const float* table; /* [table_rows][rotary_dim] */
+  int64_t table_rows;
+  const void* positions; /* [tokens] */
+} ojx_qk_desc;
+
+/* q_out [tokens][q_heads][head_dim] and k_out [tokens][kv_heads][head_dim], dense */
+int ojx_qk_norm_rope(const ojx_qk_desc* d, void* q_out, void* k_out, ojx_stream s);
+/* Gradients for dL/dq_out = gq, dL/dk_out = gk: dq, dk dense like the outputs; dqw, dkw
+ * [head_dim] in the weights' dtype (NULL: not wanted).  Sums run in fp32 in a fixed order. */
+int ojx_qk_norm_rope_backward(const ojx_qk_desc* d, const ojx_rows* gq, const ojx_rows* gk, void* dq,
+                              void* dk, void* dqw, void* dkw, ojx_stream s);
+/* The serving form: q_out as above; the normed and rotated keys and the values v are
+ * written to the cache at `slots` ([tokens], 32- or 64-bit; negative: skip the token). */
+int ojx_qkv_to_cache(const ojx_qk_desc* d, const ojx_rows* v, void* q_out, const ojx_kv_cache* cache,
+                     const void* slots, int32_t slots_int64, ojx_stream s);
+
+/* Keys and values [n][kv_heads][head_dim] into the cache at `slots`. */
+int ojx_kv_append(const ojx_kv_cache* cache, const ojx_rows* k, const ojx_rows* v, int32_t dtype,
+                  int64_t n, const void* slots, int32_t slots_int64, ojx_stream s);
+/* The rows at `slots` as dense [n][kv_heads][head_dim] of `dtype` (zeros where skipped). */
+int ojx_kv_read(const ojx_kv_cache* cache, void* k_out, void* v_out, int32_t dtype, int64_t n,
+                const void* slots, int32_t slots_int64, ojx_stream s);
+/* Keeps the accepted drafts: for every sequence b the rows of nodes path[b][0..count[b]]
+ * (at context_lens[b] + node) move to context_lens[b] + 0, 1, ...; path must ascend. */
+int ojx_kv_keep_path(const ojx_kv_cache* cache, const int32_t* page_table, int32_t table_width,
+                     const int32_t* context_lens, const int32_t* path, const int32_t* count,
+                     int64_t batch, int32_t tokens, ojx_stream s);
+
+/* Attention of the newest `tokens` of each sequence over its pages.  Query i of sequence
+ * b sees keys 0 .. context_lens[b]-1 and the new tokens j < draft_lens[b] (at position
+ * context_lens[b] + j) whose bit j % 64 is set in mask[b][i][j / 64]; without a mask,
+ * j <= i.  Queries i >= draft_lens[b], and queries that see nothing, give zeros.
+ * head_dim 64 or 128; dtype bf16 or fp16 (a 16-bit cache has the same type). */
+typedef struct ojx_tree_attention_desc {
+  ojx_kv_cache cache;
+  const void* q; /* [batch][tokens][q_heads][head_dim], strides below, rows contiguous */
+  void* out;     /* dense */
+  int64_t q_stride_b, q_stride_t, q_stride_h;
+  int32_t dtype, batch, tokens, q_heads;
+  const int32_t* page_table; /* [batch][table_width] */
+  const int32_t* context_lens; /* [batch] */
+  const int32_t* draft_lens;   /* [batch]; NULL: all tokens */
+  const int64_t* mask;         /* [batch][tokens][ceil(tokens / 64)]; NULL: causal */
+  int64_t mask_stride_b;       /* words from one sequence's mask to the next (0: shared) */
+  int32_t table_width;
+  float scale;
+} ojx_tree_attention_desc;
+int ojx_tree_attention(const ojx_tree_attention_desc* d, ojx_stream s);
+
+/* Verification of drafted tokens.  Node 0 is the root; node i carries token_ids[b][i]
+ * drafted after node parents[b][i] < i (negative token: no node).  target[b][n] and
+ * draft[b][n] are the probabilities of the token after node n.  Nodes are tried in index
+ * order, when their parent is the node reached; with r = target row, W = 1:
+ *   accept node i when u_i * (q(x_i) * W) < r(x_i);  else r = max(r - W q, 0), W = sum(r).
+ * draft NULL: q is 1 at x_i (a rejected token's r becomes 0, W falls by it).  The next
+ * token is the first v whose cumulated floor(r * 2^38) passes floor(u_0 * total).
+ * path [batch][tokens]: nodes accepted, from the root, then -1; count [batch]: accepted
+ * drafts; next_token [batch] (-1: the row holds no probability). */
+typedef struct ojx_verify_desc {
+  const void* target;
+  const void* draft;
+  int64_t target_stride_b, target_stride_t, draft_stride_b, draft_stride_t, vocab;
+  const int32_t* token_ids;
+  const int32_t* parents;
+  const float* uniforms; /* [batch][tokens] in [0, 1) */
+  int32_t* path;
+  int32_t* count;
+  int32_t* next_token;
+  int32_t batch, tokens, dtype, reserved;
+} ojx_verify_desc;
+int ojx_verify_drafts(const ojx_verify_desc* d, ojx_stream s);
+
 /* ── graph capture and replay ──────────────────────────────────────────────
  * Replaces torchcl/jit/graph_runner.py: `capture_graph` (:70-86) records the
  * launches made inside a `with` block and `CapturedGraph.replay` (:58-62)

@@ -356,6 +356,9 @@ int ojx_poll_device_error(void) {
   unsigned int w = 0;
   int st = read_and_clear_device_error(&w);
   if (st) return st;
+  unsigned int serving = 0;
+  if ((st = read_and_clear_serving_error(&serving))) return st;
+  w |= serving & 1u;  // (bounds records are kept by the GEMM kernels' unit only)
   if (w & 2u) {  // bit 1: a debug-build bounds check failed (sm100.cuh, OJX_DEVERR_BOUNDS)
     long long info[4] = {0, 0, 0, 0};
     if ((st = read_bounds_info(info))) return st;
@@ -368,6 +371,10 @@ int ojx_poll_device_error(void) {
     return set_error(OJX_ERR_TIMEOUT,
                      "a device-side wait exceeded its budget; the kernel returned early and its "
                      "output is incomplete");
+  if (serving & 4u)  // bit 2: an index read on the device was out of range (qk_cache.cuh)
+    return set_error(OJX_ERR_INVALID,
+                     "a slot, page, position, token or parent index was out of range; its access "
+                     "was skipped");
   return OJX_OK;
 }
 

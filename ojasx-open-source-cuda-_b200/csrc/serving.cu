@@ -1,0 +1,419 @@
+// serving.cu — the serving operators' kernels and their C-ABI (include/ojx.h): argument
+// checks, launch shapes and workspaces.  A translation unit of its own, with its own
+// device error word, so that it compiles beside the GEMM kernels.
+#include <algorithm>
+#include "qk_cache.cuh"
+#include "tree_attention.cuh"
+#include "verify.cuh"
+
+namespace ojx {
+
+static std::atomic<int> g_serving_launched{0};
+
+int read_and_clear_serving_error(unsigned int* word) {
+  *word = 0;
+  if (!g_serving_launched.exchange(0)) return OJX_OK;
+  unsigned int zero = 0;
+  int st = cuda_status(cudaMemcpyFromSymbol(word, g_dev_error, sizeof(unsigned int)), "read serving error word");
+  if (st) return st;
+  if (!*word) return OJX_OK;
+  return cuda_status(cudaMemcpyToSymbol(g_dev_error, &zero, sizeof(unsigned int)), "clear serving error word");
+}
+
+static int launched(const char* what) {
+  g_launches.fetch_add(1);
+  g_serving_launched.store(1);
+  return cuda_status(cudaGetLastError(), what);
+}
+
+static bool known_dtype(int dt) { return dt == OJX_F32 || dt == OJX_BF16 || dt == OJX_F16; }
+static bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
+
+static int check_cache(const char* who, const ojx_kv_cache* c) {
+  if (!c) return set_error(OJX_ERR_INVALID, "%s: cache is NULL", who);
+  if (c->format < OJX_KV_BF16 || c->format > OJX_KV_FP8)
+    return set_error(OJX_ERR_INVALID, "%s: unknown cache format %d", who, c->format);
+  if (c->num_pages < 1 || c->page_size < 1 || c->kv_heads < 1)
+    return set_error(OJX_ERR_INVALID, "%s: a cache has at least one page, row and head", who);
+  if (c->num_pages > INT32_MAX) return set_error(OJX_ERR_INVALID, "%s: too many pages", who);
+  if (c->head_dim < 16 || c->head_dim > 512 || c->head_dim % 16)
+    return set_error(OJX_ERR_INVALID, "%s: head_dim %d is not a multiple of 16 up to 512", who, c->head_dim);
+  if (!c->k || !c->v || !aligned16(c->k) || !aligned16(c->v))
+    return set_error(OJX_ERR_INVALID, "%s: cache pages must be 16-byte aligned", who);
+  if (c->format >= OJX_KV_INT8 && (!c->k_scale || !c->v_scale))
+    return set_error(OJX_ERR_INVALID, "%s: an 8-bit cache needs its steps", who);
+  return OJX_OK;
+}
+
+// Whether rows can be read as 16-byte vectors.
+static bool vector_rows(const ojx_rows& r, int es) {
+  return !r.data || (aligned16(r.data) && (r.stride_t * es) % 16 == 0 && (r.stride_h * es) % 16 == 0);
+}
+// Whether every chunk of eight elements lies wholly inside or outside the turning part,
+// and pairs of chunks cover a row.
+static bool vector_pairs(int D, int rotary, bool inter) {
+  if (D % 16 || D > 512) return false;
+  return inter ? rotary % 16 == 0 : (rotary / 2) % 8 == 0 && (D - rotary) % 16 == 0;
+}
+static int pow2_at_least(int n) {
+  int p = 1;
+  while (p < n) p *= 2;
+  return p;
+}
+
+template <typename F>
+static int for_dtype(int dtype, F f) {
+  if (dtype == OJX_F32) return f(float{});
+  if (dtype == OJX_BF16) return f(__nv_bfloat16{});
+  return f(__half{});
+}
+
+static int launch_rows(QkParams& p, int dtype, bool vec, bool inter, cudaStream_t s) {
+  if (p.tokens == 0) return OJX_OK;
+  const int CH = vec ? 8 : 1;
+  p.npairs = p.D / (2 * CH);
+  p.lanes = std::min(32, pow2_at_least(p.npairs));
+  const int per_warp = 32 / p.lanes, heads = p.hq + p.hk + p.hv;
+  const int groups = (heads + per_warp - 1) / per_warp;
+  // One warp runs all heads of a token, so that the token's cosines are read once, unless
+  // that leaves SMs without work: then its heads are split over more warps.
+  const int64_t want = 16ll * current_props().sm_count;
+  int split = 1;
+  while (split < groups && p.tokens * split < want) split *= 2;
+  split = std::min(split, groups);
+  p.iters = (groups + split - 1) / split;
+  p.blocks_per_token = (groups + p.iters - 1) / p.iters;
+  const int64_t warps = p.tokens * p.blocks_per_token;
+  const int64_t grid = (warps + 7) / 8;
+  if (grid > INT32_MAX) return set_error(OJX_ERR_INVALID, "too many rows for one call");
+  return for_dtype(dtype, [&](auto t) {
+    using T = decltype(t);
+    const unsigned gr = static_cast<unsigned>(grid);
+    if (vec && !inter) qk_rows_kernel<T, 8, 1, false><<<gr, 256, 0, s>>>(p);
+    else if (vec) qk_rows_kernel<T, 8, 1, true><<<gr, 256, 0, s>>>(p);
+    else if (!inter) qk_rows_kernel<T, 1, 8, false><<<gr, 256, 0, s>>>(p);
+    else qk_rows_kernel<T, 1, 8, true><<<gr, 256, 0, s>>>(p);
+    return launched("qk_rows launch");
+  });
+}
+
+static int check_qk(const char* who, const ojx_qk_desc* d) {
+  if (!d) return set_error(OJX_ERR_INVALID, "%s: desc is NULL", who);
+  if (d->tokens < 0 || d->q_heads < 0 || d->kv_heads < 0)
+    return set_error(OJX_ERR_INVALID, "%s: negative size", who);
+  if (!known_dtype(d->dtype) || !known_dtype(d->dtype_weight))
+    return set_error(OJX_ERR_INVALID, "%s: unknown dtype", who);
+  if (d->head_dim < 2 || d->head_dim > 512 || d->head_dim % 2)
+    return set_error(OJX_ERR_INVALID, "%s: head_dim %d is not an even number up to 512", who, d->head_dim);
+  if (d->rotary_dim < 0 || d->rotary_dim > d->head_dim || d->rotary_dim % 2)
+    return set_error(OJX_ERR_INVALID, "%s: rotary_dim %d is not an even number up to head_dim", who, d->rotary_dim);
+  if (!(d->eps >= 0.0f)) return set_error(OJX_ERR_INVALID, "%s: eps must not be negative", who);
+  if (d->table_rows < 0) return set_error(OJX_ERR_INVALID, "%s: negative size", who);
+  if (d->tokens > 0 && ((d->q_heads && !d->q.data) || (d->kv_heads && !d->k.data) || !d->positions || (d->rotary_dim && !d->table)))
+    return set_error(OJX_ERR_INVALID, "%s: NULL pointer", who);
+  return OJX_OK;
+}
+
+static QkParams make_qk(const ojx_qk_desc* d) {
+  QkParams p{};
+  p.tokens = d->tokens;
+  p.D = d->head_dim;
+  p.rotary = d->rotary_dim;
+  p.half = d->rotary_dim / 2;
+  p.norm = 1;
+  p.hq = d->q_heads;
+  p.hk = d->kv_heads;
+  p.dtype_w = d->dtype_weight;
+  p.pos64 = d->positions_int64;
+  p.eps = d->eps;
+  p.q = d->q.data, p.q_st = d->q.stride_t, p.q_sh = d->q.stride_h;
+  p.k = d->k.data, p.k_st = d->k.stride_t, p.k_sh = d->k.stride_h;
+  p.qw = d->q_weight;
+  p.kw = d->k_weight;
+  p.table = d->table;
+  p.table_rows = d->table_rows;
+  p.positions = d->positions;
+  return p;
+}
+
+static bool qk_vector(const ojx_qk_desc* d) {
+  const int es = dtype_size(d->dtype);
+  return vector_pairs(d->head_dim, d->rotary_dim, d->interleaved != 0) && vector_rows(d->q, es) &&
+         vector_rows(d->k, es) && aligned16(d->q_weight) && aligned16(d->k_weight);
+}
+
+template <int FMT, int D, int MT>
+static int launch_tree(TaParams& p, cudaStream_t s) {
+  using L = TaLayout<FMT, D, MT>;
+  auto kern = tree_attention_kernel<FMT, D, MT>;
+  int st = ensure_smem_attr(reinterpret_cast<const void*>(kern), L::SMEM);
+  if (st) return st;
+  const int rows = p.tokens * p.group;
+  p.row_tiles = (rows + L::ROWS - 1) / L::ROWS;
+  const int64_t segments = static_cast<int64_t>(p.batch) * p.cache.kv_heads * p.row_tiles;
+  const int64_t most_keys = static_cast<int64_t>(p.width) * p.cache.page_size;
+  const int64_t steps = (most_keys + L::NW * L::KB - 1) / (L::NW * L::KB);
+  const int sms = current_props().sm_count;
+  int64_t splits = std::max<int64_t>(1, std::min((sms + segments - 1) / segments, steps));
+  p.splits = static_cast<int>(splits);
+  if (segments * splits > INT32_MAX) return set_error(OJX_ERR_INVALID, "ojx_tree_attention: too many rows");
+  if (splits > 1) {
+    const size_t slots = static_cast<size_t>(segments) * splits * L::ROWS;
+    char* ws = static_cast<char*>(stream_workspace(s, slots * (D * 4 + 8), 8, false));
+    if (!ws) return workspace_error();
+    p.part_o = reinterpret_cast<float*>(ws);
+    p.part_ml = reinterpret_cast<float2*>(ws + slots * D * 4);
+  }
+  kern<<<static_cast<unsigned>(segments * splits), L::NW * 32, L::SMEM, s>>>(p);
+  if ((st = launched("tree_attention launch"))) return st;
+  if (splits > 1) {
+    const int64_t all = static_cast<int64_t>(p.batch) * p.cache.kv_heads * rows;
+    tree_attention_join_kernel<D><<<static_cast<unsigned>((all + 3) / 4), 128, 0, s>>>(p, L::ROWS);
+    st = launched("tree_attention join launch");
+  }
+  return st;
+}
+
+template <int FMT>
+static int launch_tree_fmt(TaParams& p, cudaStream_t s) {
+  const bool wide = p.tokens * p.group > 16;  // more than one 16-row tile
+  if (p.cache.head_dim == 64) return wide ? launch_tree<FMT, 64, 2>(p, s) : launch_tree<FMT, 64, 1>(p, s);
+  return wide ? launch_tree<FMT, 128, 2>(p, s) : launch_tree<FMT, 128, 1>(p, s);
+}
+
+}  // namespace ojx
+
+using namespace ojx;
+
+extern "C" {
+
+int ojx_qk_norm_rope(const ojx_qk_desc* d, void* q_out, void* k_out, ojx_stream s) {
+  NvtxRange nvtx("ojx_qk_norm_rope");
+  int st = check_qk("ojx_qk_norm_rope", d);
+  if (st) return st;
+  if (d->tokens == 0 || d->q_heads + d->kv_heads == 0) return OJX_OK;
+  if ((d->q_heads && !q_out) || (d->kv_heads && !k_out))
+    return set_error(OJX_ERR_INVALID, "ojx_qk_norm_rope: NULL output");
+  QkParams p = make_qk(d);
+  p.q_out = q_out;
+  p.k_out = k_out;
+  const bool vec = qk_vector(d) && aligned16(q_out) && aligned16(k_out);
+  return launch_rows(p, d->dtype, vec, d->interleaved != 0, static_cast<cudaStream_t>(s));
+}
+
+int ojx_qkv_to_cache(const ojx_qk_desc* d, const ojx_rows* v, void* q_out, const ojx_kv_cache* cache,
+                     const void* slots, int32_t slots_int64, ojx_stream s) {
+  NvtxRange nvtx("ojx_qkv_to_cache");
+  int st = check_qk("ojx_qkv_to_cache", d);
+  if (st) return st;
+  if ((st = check_cache("ojx_qkv_to_cache", cache))) return st;
+  if (cache->head_dim != d->head_dim || cache->kv_heads != d->kv_heads)
+    return set_error(OJX_ERR_INVALID, "ojx_qkv_to_cache: the cache holds %d heads of %d, the keys have %d of %d",
+                     cache->kv_heads, cache->head_dim, d->kv_heads, d->head_dim);
+  if (d->tokens == 0) return OJX_OK;
+  if (!v || !v->data || !slots || (d->q_heads && !q_out))
+    return set_error(OJX_ERR_INVALID, "ojx_qkv_to_cache: NULL pointer");
+  QkParams p = make_qk(d);
+  p.hv = d->kv_heads;
+  p.v = v->data, p.v_st = v->stride_t, p.v_sh = v->stride_h;
+  p.q_out = q_out;
+  p.k_to_cache = 1;
+  p.cache = *cache;
+  p.slots = slots;
+  p.slot64 = slots_int64;
+  const bool vec = qk_vector(d) && vector_rows(*v, dtype_size(d->dtype)) && aligned16(q_out);
+  return launch_rows(p, d->dtype, vec, d->interleaved != 0, static_cast<cudaStream_t>(s));
+}
+
+int ojx_qk_norm_rope_backward(const ojx_qk_desc* d, const ojx_rows* gq, const ojx_rows* gk, void* dq,
+                              void* dk, void* dqw, void* dkw, ojx_stream stream) {
+  NvtxRange nvtx("ojx_qk_norm_rope_backward");
+  int st = check_qk("ojx_qk_norm_rope_backward", d);
+  if (st) return st;
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  const size_t wbytes = static_cast<size_t>(d->head_dim) * dtype_size(d->dtype_weight);
+  if (d->tokens == 0 || d->q_heads + d->kv_heads == 0) {  // no rows: the weights' sums are empty
+    if (dqw && (st = cuda_status(cudaMemsetAsync(dqw, 0, wbytes, s), "clear dqw"))) return st;
+    if (dkw && (st = cuda_status(cudaMemsetAsync(dkw, 0, wbytes, s), "clear dkw"))) return st;
+    return OJX_OK;
+  }
+  if ((d->q_heads && (!gq || !gq->data || !dq)) || (d->kv_heads && (!gk || !gk->data || !dk)))
+    return set_error(OJX_ERR_INVALID, "ojx_qk_norm_rope_backward: NULL pointer");
+  QkParams p = make_qk(d);
+  const int es = dtype_size(d->dtype);
+  bool vec = qk_vector(d) && aligned16(dq) && aligned16(dk);
+  if (gq) p.gq = gq->data, p.gq_st = gq->stride_t, p.gq_sh = gq->stride_h, vec = vec && vector_rows(*gq, es);
+  if (gk) p.gk = gk->data, p.gk_st = gk->stride_t, p.gk_sh = gk->stride_h, vec = vec && vector_rows(*gk, es);
+  p.dq = dq;
+  p.dk = dk;
+  const bool inter = d->interleaved != 0;
+  p.npairs = p.D / (vec ? 16 : 2);
+  p.lanes = std::min(32, pow2_at_least(p.npairs));
+  // Blocks in proportion to each side's heads, at most one warp per token of it.
+  const int64_t most = 3ll * current_props().sm_count;
+  auto blocks_of = [&](int heads) -> int64_t {
+    if (heads == 0) return 0;
+    const int64_t share = std::max<int64_t>(1, most * heads / (d->q_heads + d->kv_heads));
+    return std::min(share, (d->tokens + 7) / 8);
+  };
+  p.q_blocks = static_cast<int>(blocks_of(d->q_heads));
+  const int blocks = p.q_blocks + static_cast<int>(blocks_of(d->kv_heads));
+  p.partial = static_cast<float*>(stream_workspace(s, static_cast<size_t>(blocks) * p.D * 4, 9, false));
+  if (!p.partial) return workspace_error();
+  const int smem = 8 * p.D * 4;
+  st = for_dtype(d->dtype, [&](auto t) {
+    using T = decltype(t);
+    if (vec && !inter) qk_grad_kernel<T, 8, 1, false><<<blocks, 256, smem, s>>>(p);
+    else if (vec) qk_grad_kernel<T, 8, 1, true><<<blocks, 256, smem, s>>>(p);
+    else if (!inter) qk_grad_kernel<T, 1, 8, false><<<blocks, 256, smem, s>>>(p);
+    else qk_grad_kernel<T, 1, 8, true><<<blocks, 256, smem, s>>>(p);
+    return launched("qk_grad launch");
+  });
+  if (st || (!dqw && !dkw)) return st;
+  qk_grad_weight_kernel<<<dim3((p.D + 31) / 32, 2), dim3(32, 8), 0, s>>>(p.partial, p.q_blocks, blocks, p.D, dqw,
+                                                                        dkw, d->dtype_weight);
+  return launched("qk_grad_weight launch");
+}
+
+int ojx_kv_append(const ojx_kv_cache* cache, const ojx_rows* k, const ojx_rows* v, int32_t dtype,
+                  int64_t n, const void* slots, int32_t slots_int64, ojx_stream s) {
+  NvtxRange nvtx("ojx_kv_append");
+  int st = check_cache("ojx_kv_append", cache);
+  if (st) return st;
+  if (n < 0) return set_error(OJX_ERR_INVALID, "ojx_kv_append: negative size");
+  if (!known_dtype(dtype)) return set_error(OJX_ERR_INVALID, "ojx_kv_append: unknown dtype");
+  if (n == 0) return OJX_OK;
+  if (!k || !v || !k->data || !v->data || !slots) return set_error(OJX_ERR_INVALID, "ojx_kv_append: NULL pointer");
+  QkParams p{};
+  p.tokens = n;
+  p.D = cache->head_dim;
+  p.hk = p.hv = cache->kv_heads;
+  p.k = k->data, p.k_st = k->stride_t, p.k_sh = k->stride_h;
+  p.v = v->data, p.v_st = v->stride_t, p.v_sh = v->stride_h;
+  p.k_to_cache = 1;
+  p.cache = *cache;
+  p.slots = slots;
+  p.slot64 = slots_int64;
+  const int es = dtype_size(dtype);
+  return launch_rows(p, dtype, vector_rows(*k, es) && vector_rows(*v, es), false, static_cast<cudaStream_t>(s));
+}
+
+int ojx_kv_read(const ojx_kv_cache* cache, void* k_out, void* v_out, int32_t dtype, int64_t n,
+                const void* slots, int32_t slots_int64, ojx_stream stream) {
+  NvtxRange nvtx("ojx_kv_read");
+  int st = check_cache("ojx_kv_read", cache);
+  if (st) return st;
+  if (n < 0) return set_error(OJX_ERR_INVALID, "ojx_kv_read: negative size");
+  if (!known_dtype(dtype)) return set_error(OJX_ERR_INVALID, "ojx_kv_read: unknown dtype");
+  if (n == 0) return OJX_OK;
+  if (!k_out || !v_out || !slots) return set_error(OJX_ERR_INVALID, "ojx_kv_read: NULL pointer");
+  if (!aligned16(k_out) || !aligned16(v_out))
+    return set_error(OJX_ERR_INVALID, "ojx_kv_read: outputs must be 16-byte aligned");
+  const int64_t threads = 2 * n * cache->kv_heads * (cache->head_dim / 8);
+  const int64_t grid = (threads + 255) / 256;
+  if (grid > INT32_MAX) return set_error(OJX_ERR_INVALID, "ojx_kv_read: too many rows for one call");
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  return for_dtype(dtype, [&](auto t) {
+    using T = decltype(t);
+    kv_read_kernel<T><<<static_cast<unsigned>(grid), 256, 0, s>>>(*cache, slots, slots_int64, n,
+                                                                  static_cast<T*>(k_out), static_cast<T*>(v_out));
+    return launched("kv_read launch");
+  });
+}
+
+int ojx_kv_keep_path(const ojx_kv_cache* cache, const int32_t* page_table, int32_t table_width,
+                     const int32_t* context_lens, const int32_t* path, const int32_t* count,
+                     int64_t batch, int32_t tokens, ojx_stream s) {
+  NvtxRange nvtx("ojx_kv_keep_path");
+  int st = check_cache("ojx_kv_keep_path", cache);
+  if (st) return st;
+  if (batch < 0 || tokens < 0 || table_width < 0)
+    return set_error(OJX_ERR_INVALID, "ojx_kv_keep_path: negative size");
+  if (batch == 0 || tokens == 0) return OJX_OK;
+  if (!page_table || !context_lens || !path || !count)
+    return set_error(OJX_ERR_INVALID, "ojx_kv_keep_path: NULL pointer");
+  if (batch * cache->kv_heads > INT32_MAX) return set_error(OJX_ERR_INVALID, "ojx_kv_keep_path: too many heads");
+  kv_keep_path_kernel<<<static_cast<unsigned>(batch * cache->kv_heads), 128, 0, static_cast<cudaStream_t>(s)>>>(
+      *cache, page_table, table_width, context_lens, path, count, tokens);
+  return launched("kv_keep_path launch");
+}
+
+int ojx_tree_attention(const ojx_tree_attention_desc* d, ojx_stream stream) {
+  NvtxRange nvtx("ojx_tree_attention");
+  if (!d) return set_error(OJX_ERR_INVALID, "ojx_tree_attention: desc is NULL");
+  int st = check_cache("ojx_tree_attention", &d->cache);
+  if (st) return st;
+  const ojx_kv_cache& c = d->cache;
+  if (c.head_dim != 64 && c.head_dim != 128)
+    return set_error(OJX_ERR_INVALID, "ojx_tree_attention: head_dim %d is not 64 or 128", c.head_dim);
+  if (d->dtype != OJX_BF16 && d->dtype != OJX_F16)
+    return set_error(OJX_ERR_INVALID, "ojx_tree_attention: queries are bf16 or fp16");
+  if (c.format < OJX_KV_INT8 && c.format != d->dtype)
+    return set_error(OJX_ERR_INVALID, "ojx_tree_attention: a 16-bit cache has the queries' dtype");
+  if (d->batch < 0 || d->tokens < 0 || d->q_heads < 0 || d->table_width < 0)
+    return set_error(OJX_ERR_INVALID, "ojx_tree_attention: negative size");
+  if (d->q_heads % c.kv_heads)
+    return set_error(OJX_ERR_INVALID, "ojx_tree_attention: %d query heads do not share %d key heads evenly",
+                     d->q_heads, c.kv_heads);
+  if (!(d->scale > 0.0f)) return set_error(OJX_ERR_INVALID, "ojx_tree_attention: scale must be positive");
+  if (d->batch == 0 || d->tokens == 0 || d->q_heads == 0) return OJX_OK;
+  if (!d->q || !d->out || !d->context_lens || (d->table_width > 0 && !d->page_table))
+    return set_error(OJX_ERR_INVALID, "ojx_tree_attention: NULL pointer");
+  if (static_cast<int64_t>(d->tokens) * d->q_heads > INT32_MAX / 2 ||
+      static_cast<int64_t>(d->table_width) * c.page_size > INT32_MAX / 2)
+    return set_error(OJX_ERR_INVALID, "ojx_tree_attention: too large");
+  TaParams p{};
+  p.cache = c;
+  p.q = d->q;
+  p.out = d->out;
+  p.q_sb = d->q_stride_b, p.q_st = d->q_stride_t, p.q_sh = d->q_stride_h;
+  p.dtype = d->dtype, p.batch = d->batch, p.tokens = d->tokens, p.q_heads = d->q_heads;
+  p.group = d->q_heads / c.kv_heads;
+  p.page_table = d->page_table;
+  p.width = d->table_width;
+  p.contexts = d->context_lens;
+  p.drafts = d->draft_lens;
+  p.mask = d->mask;
+  p.mask_sb = d->mask_stride_b;
+  p.words = (d->tokens + 63) / 64;
+  p.scale_log2 = d->scale * 1.4426950408889634f;
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  if (c.format == OJX_KV_F16) return launch_tree_fmt<TA_F16>(p, s);
+  if (c.format == OJX_KV_BF16) return launch_tree_fmt<TA_BF16>(p, s);
+  if (c.format == OJX_KV_INT8) return launch_tree_fmt<TA_INT8>(p, s);
+  return launch_tree_fmt<TA_FP8>(p, s);
+}
+
+int ojx_verify_drafts(const ojx_verify_desc* d, ojx_stream stream) {
+  NvtxRange nvtx("ojx_verify_drafts");
+  if (!d) return set_error(OJX_ERR_INVALID, "ojx_verify_drafts: desc is NULL");
+  if (d->batch < 0 || d->tokens < 0 || d->vocab < 0)
+    return set_error(OJX_ERR_INVALID, "ojx_verify_drafts: negative size");
+  if (!known_dtype(d->dtype)) return set_error(OJX_ERR_INVALID, "ojx_verify_drafts: unknown dtype");
+  if (d->batch == 0) return OJX_OK;
+  if (d->tokens < 1 || d->tokens > VD_MAX_TOKENS)
+    return set_error(OJX_ERR_INVALID, "ojx_verify_drafts: 1 to %d nodes, not %d", VD_MAX_TOKENS, d->tokens);
+  if (d->vocab < 1 || d->vocab > (1 << 22))
+    return set_error(OJX_ERR_INVALID, "ojx_verify_drafts: a vocabulary has 1 to %d tokens", 1 << 22);
+  if (!d->target || !d->token_ids || !d->parents || !d->uniforms || !d->path || !d->count || !d->next_token)
+    return set_error(OJX_ERR_INVALID, "ojx_verify_drafts: NULL pointer");
+  if (d->batch > INT32_MAX / VD_CLUSTER) return set_error(OJX_ERR_INVALID, "ojx_verify_drafts: too many sequences");
+  VerifyParams p{};
+  p.target = d->target, p.t_sb = d->target_stride_b, p.t_st = d->target_stride_t;
+  p.draft = d->draft, p.d_sb = d->draft_stride_b, p.d_st = d->draft_stride_t;
+  p.tokens = d->token_ids, p.parents = d->parents, p.uniforms = d->uniforms;
+  p.path = d->path, p.count = d->count, p.next = d->next_token;
+  p.T = d->tokens;
+  p.V = d->vocab;
+  const int64_t per_warp = (p.V + VD_CLUSTER * VD_WARPS - 1) / (VD_CLUSTER * VD_WARPS);
+  const int smem = d->draft ? 0 : static_cast<int>((per_warp * VD_WARPS + 31) / 32 * 4);
+  return for_dtype(d->dtype, [&](auto t) {
+    auto kern = verify_drafts_kernel<decltype(t)>;
+    int st = ensure_smem_attr(reinterpret_cast<const void*>(kern), 96 * 1024);
+    if (st) return st;
+    kern<<<d->batch * VD_CLUSTER, VD_THREADS, smem, static_cast<cudaStream_t>(stream)>>>(p);
+    return launched("verify_drafts launch");
+  });
+}
+
+}  // extern "C"

@@ -23,7 +23,7 @@ from torchcl.api import (
     relu, sigmoid, tanh_, gelu, silu,
     matmul, transpose, linear, fused_attention,
 )
-from torchcl import blas  # noqa: E402
+from torchcl import blas, serving  # noqa: E402
 
 __all__ = [
     "get_device_info", "is_available", "synchronize", "init_opencl", "init",
@@ -31,6 +31,6 @@ __all__ = [
     "zeros", "zeros_like", "ones", "ones_like", "full", "randn",
     "add", "sub", "mul", "div", "neg", "abs_", "exp", "log", "sqrt", "square",
     "relu", "sigmoid", "tanh_", "gelu", "silu",
-    "matmul", "transpose", "linear", "fused_attention", "blas",
+    "matmul", "transpose", "linear", "fused_attention", "blas", "serving",
     "Stream", "Event", "stream", "current_stream", "default_stream",
 ]

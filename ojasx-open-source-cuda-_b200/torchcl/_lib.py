@@ -87,6 +87,65 @@ class GraphNode(ctypes.Structure):
                 ("name", ctypes.c_char * 128)]
 
 
+KV_FORMATS = {"bfloat16": 1, "float16": 2, "int8": 3, "float8": 4}
+
+
+class KVCacheDesc(ctypes.Structure):
+    _fields_ = [
+        ("k", ctypes.c_void_p), ("v", ctypes.c_void_p),
+        ("k_scale", ctypes.c_void_p), ("v_scale", ctypes.c_void_p),
+        ("num_pages", ctypes.c_int64),
+        ("page_size", ctypes.c_int32), ("kv_heads", ctypes.c_int32),
+        ("head_dim", ctypes.c_int32), ("format", ctypes.c_int32),
+    ]
+
+
+class Rows(ctypes.Structure):
+    _fields_ = [("data", ctypes.c_void_p), ("stride_t", ctypes.c_int64), ("stride_h", ctypes.c_int64)]
+
+
+class QkDesc(ctypes.Structure):
+    _fields_ = [
+        ("tokens", ctypes.c_int64),
+        ("q_heads", ctypes.c_int32), ("kv_heads", ctypes.c_int32),
+        ("head_dim", ctypes.c_int32), ("rotary_dim", ctypes.c_int32),
+        ("interleaved", ctypes.c_int32), ("dtype", ctypes.c_int32),
+        ("dtype_weight", ctypes.c_int32), ("positions_int64", ctypes.c_int32),
+        ("eps", ctypes.c_float), ("reserved", ctypes.c_int32),
+        ("q", Rows), ("k", Rows),
+        ("q_weight", ctypes.c_void_p), ("k_weight", ctypes.c_void_p),
+        ("table", ctypes.c_void_p), ("table_rows", ctypes.c_int64),
+        ("positions", ctypes.c_void_p),
+    ]
+
+
+class TreeAttentionDesc(ctypes.Structure):
+    _fields_ = [
+        ("cache", KVCacheDesc),
+        ("q", ctypes.c_void_p), ("out", ctypes.c_void_p),
+        ("q_stride_b", ctypes.c_int64), ("q_stride_t", ctypes.c_int64), ("q_stride_h", ctypes.c_int64),
+        ("dtype", ctypes.c_int32), ("batch", ctypes.c_int32),
+        ("tokens", ctypes.c_int32), ("q_heads", ctypes.c_int32),
+        ("page_table", ctypes.c_void_p), ("context_lens", ctypes.c_void_p),
+        ("draft_lens", ctypes.c_void_p), ("mask", ctypes.c_void_p),
+        ("mask_stride_b", ctypes.c_int64),
+        ("table_width", ctypes.c_int32), ("scale", ctypes.c_float),
+    ]
+
+
+class VerifyDesc(ctypes.Structure):
+    _fields_ = [
+        ("target", ctypes.c_void_p), ("draft", ctypes.c_void_p),
+        ("target_stride_b", ctypes.c_int64), ("target_stride_t", ctypes.c_int64),
+        ("draft_stride_b", ctypes.c_int64), ("draft_stride_t", ctypes.c_int64),
+        ("vocab", ctypes.c_int64),
+        ("token_ids", ctypes.c_void_p), ("parents", ctypes.c_void_p), ("uniforms", ctypes.c_void_p),
+        ("path", ctypes.c_void_p), ("count", ctypes.c_void_p), ("next_token", ctypes.c_void_p),
+        ("batch", ctypes.c_int32), ("tokens", ctypes.c_int32),
+        ("dtype", ctypes.c_int32), ("reserved", ctypes.c_int32),
+    ]
+
+
 NODE_TYPES = {0: "other", 1: "kernel", 2: "memset", 3: "memcpy"}
 
 _P = ctypes.c_void_p
@@ -139,6 +198,19 @@ _SIGS = {
                        ctypes.c_int64, ctypes.c_int32, _P], ctypes.c_int),
     "ojx_sum_columns": ([_P, ctypes.c_int32, _P, ctypes.c_int32, ctypes.c_int64, ctypes.c_int64,
                          ctypes.c_int64, _P], ctypes.c_int),
+    "ojx_qk_norm_rope": ([ctypes.POINTER(QkDesc), _P, _P, _P], ctypes.c_int),
+    "ojx_qk_norm_rope_backward": ([ctypes.POINTER(QkDesc), ctypes.POINTER(Rows), ctypes.POINTER(Rows),
+                                   _P, _P, _P, _P, _P], ctypes.c_int),
+    "ojx_qkv_to_cache": ([ctypes.POINTER(QkDesc), ctypes.POINTER(Rows), _P, ctypes.POINTER(KVCacheDesc),
+                          _P, ctypes.c_int32, _P], ctypes.c_int),
+    "ojx_kv_append": ([ctypes.POINTER(KVCacheDesc), ctypes.POINTER(Rows), ctypes.POINTER(Rows),
+                       ctypes.c_int32, ctypes.c_int64, _P, ctypes.c_int32, _P], ctypes.c_int),
+    "ojx_kv_read": ([ctypes.POINTER(KVCacheDesc), _P, _P, ctypes.c_int32, ctypes.c_int64, _P,
+                     ctypes.c_int32, _P], ctypes.c_int),
+    "ojx_kv_keep_path": ([ctypes.POINTER(KVCacheDesc), _P, ctypes.c_int32, _P, _P, _P, ctypes.c_int64,
+                          ctypes.c_int32, _P], ctypes.c_int),
+    "ojx_tree_attention": ([ctypes.POINTER(TreeAttentionDesc), _P], ctypes.c_int),
+    "ojx_verify_drafts": ([ctypes.POINTER(VerifyDesc), _P], ctypes.c_int),
     "ojx_ipc_get_handle": ([_P, _P], ctypes.c_int),
     "ojx_ipc_open_handle": ([_P, ctypes.POINTER(_P)], ctypes.c_int),
     "ojx_ipc_close_handle": ([_P], ctypes.c_int),

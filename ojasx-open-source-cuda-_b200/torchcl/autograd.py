@@ -126,4 +126,29 @@ class LinearFunction(torch.autograd.Function):
         return grad_x, grad_w, grad_bias
 
 
-__all__ = ["MatmulFunction", "LinearFunction"]
+class QKNormRopeFunction(torch.autograd.Function):
+    """torchcl.serving.qk_norm_rope with its gradient.  Saves its inputs only: the norms
+    are recomputed in the pass that reads the rows for their gradient.
+
+        forward   y = rotate(w * x * r),  r = 1 / sqrt(mean(x^2) + eps)
+        backward  h = w * rotate_back(dy);  dx = r h - x r^3 mean(h x)
+                  dw = sum over tokens and heads of rotate_back(dy) * x * r
+    """
+
+    @staticmethod
+    def forward(ctx, q, k, q_weight, k_weight, table, positions, eps=1e-6, interleaved=False):
+        from torchcl.serving import _qk_forward
+        ctx.save_for_backward(q, k, q_weight, k_weight, table, positions)
+        ctx._eps, ctx._interleaved = eps, interleaved
+        return _qk_forward(q, k, q_weight, k_weight, table, positions, eps, interleaved)
+
+    @staticmethod
+    def backward(ctx, grad_q, grad_k):
+        from torchcl.serving import _qk_backward
+        q, k, q_weight, k_weight, table, positions = ctx.saved_tensors
+        grads = _qk_backward(grad_q, grad_k, q, k, q_weight, k_weight, table, positions, ctx._eps,
+                             ctx._interleaved, want_weights=any(ctx.needs_input_grad[2:4]))
+        return (*grads, None, None, None, None)
+
+
+__all__ = ["MatmulFunction", "LinearFunction", "QKNormRopeFunction"]

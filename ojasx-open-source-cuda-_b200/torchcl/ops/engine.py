@@ -20,6 +20,7 @@ from torchcl.runtime.memory import CLBuffer, get_buffer_pool, note_use
 
 _TORCH_TO_OJX = {torch.float32: L.F32, torch.bfloat16: L.BF16, torch.float16: L.F16}
 _OJX_TO_TORCH = {v: k for k, v in _TORCH_TO_OJX.items()}
+INDEX_DTYPES = (torch.int32, torch.int64)  # stored on the device as index arrays, not computed with
 _ITEMSIZE = {L.F32: 4, L.BF16: 2, L.F16: 2}
 
 
@@ -67,7 +68,8 @@ class OpenCLEngine:
         if t.device.type != "cpu":
             t = t.cpu()
         t = t.contiguous()
-        ojx_dtype(t.dtype)
+        if t.dtype not in INDEX_DTYPES:
+            ojx_dtype(t.dtype)
         return self._pool.host_to_device(t)
 
     def buffer_to_tensor(self, cl_buf: CLBuffer, shape: tuple, dtype: torch.dtype = torch.float32

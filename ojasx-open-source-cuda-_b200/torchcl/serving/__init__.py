@@ -1,0 +1,474 @@
+"""Serving operators: what a decoding step needs between its GEMMs.
+
+    qk_norm_rope     RMS norm of each query and key head and the position rotation, one pass
+                     (differentiable)
+    qkv_to_cache     the same, with keys and values written to a paged cache
+    KVCache          pages of keys and values in bf16, fp16, int8 or e4m3: append, read, keep_path
+    tree_attention   attention of the newest tokens (one, a chunk, or a tree of drafts) over a cache
+    verify_drafts    acceptance of drafted tokens against the target's probabilities
+
+Every function takes device tensors of either kind, and returns the same kind: torchcl
+handles (launched on torchcl's current stream) or torch CUDA tensors (launched on torch's
+current stream of the current device; strided views are read in place when their last
+dimension is dense).  Integer arguments beside handles may also be CPU tensors; they are
+uploaded.  Calls are asynchronous.  An index that lies outside its range on the device is
+skipped and reported as ValueError by the next torchcl.synchronize() or to_cpu().
+The reference has no counterpart of these functions.
+"""
+from __future__ import annotations
+
+import ctypes
+import math
+
+import torch
+
+from torchcl import _lib as L
+from torchcl.api import _get_buf, _get_dtype, _get_shape, _wrap_output, is_opencl_tensor, to_opencl
+from torchcl.ops.engine import ojx_dtype
+from torchcl.runtime.context import get_queue
+from torchcl.runtime.memory import CLBuffer, get_buffer_pool, note_use
+
+_FORMAT_DTYPES = {"bfloat16": torch.bfloat16, "float16": torch.float16, "int8": torch.int8,
+                  "float8": torch.float8_e4m3fn}
+_INTS = (torch.int32, torch.int64)
+_ref = ctypes.byref
+
+
+# ── device arguments ──────────────────────────────────────────────────────────
+
+def _on_torch(t) -> bool:
+    """True for a torch CUDA tensor, False for a torchcl handle, ValueError otherwise."""
+    if isinstance(t, torch.Tensor) and t.is_cuda:
+        if t.device.index != torch.cuda.current_device():
+            raise ValueError(f"tensor on {t.device}, but the current device is cuda:{torch.cuda.current_device()}")
+        return True
+    if is_opencl_tensor(t):
+        return False
+    raise ValueError("expected a device tensor: a torchcl handle or a torch CUDA tensor")
+
+
+def _strides(shape) -> tuple:
+    out, acc = [], 1
+    for d in reversed(shape):
+        out.append(acc)
+        acc *= max(int(d), 1)
+    return tuple(reversed(out))
+
+
+class _Arg:
+    """Address, shape, strides and dtype of one device tensor, and what keeps it alive."""
+
+    __slots__ = ("ptr", "shape", "strides", "dtype", "keep")
+
+    def __init__(self, t, on_torch: bool, name: str, dtypes=None, integer=False):
+        if integer and not on_torch and isinstance(t, torch.Tensor) and not is_opencl_tensor(t) and not t.is_cuda:
+            t = to_opencl(t)
+        if _on_torch(t) != on_torch:
+            raise ValueError(f"{name}: torch CUDA tensors and torchcl handles cannot be mixed in one call")
+        if on_torch:
+            if not integer and t.dim() and t.shape[-1] > 1 and t.stride(-1) != 1 or integer and not t.is_contiguous():
+                t = t.contiguous()
+            self.ptr, self.shape, self.strides, self.dtype = t.data_ptr(), tuple(t.shape), t.stride(), t.dtype
+            self.keep = t
+        else:
+            buf = _get_buf(t)
+            self.ptr, self.shape, self.dtype = buf.buffer, _get_shape(t), _get_dtype(t)
+            self.strides = _strides(self.shape)
+            self.keep = (t, buf)
+        if dtypes is not None and self.dtype not in dtypes:
+            raise ValueError(f"{name}: dtype {self.dtype}, expected one of {[str(d) for d in dtypes]}")
+
+
+def _stream(on_torch: bool):
+    return torch.cuda.current_stream().cuda_stream if on_torch else get_queue()
+
+
+def _empty(shape, dtype, on_torch: bool):
+    """(tensor or handle, address) of a new dense output."""
+    if on_torch:
+        out = torch.empty(shape, dtype=dtype, device="cuda")
+        return out, out.data_ptr()
+    numel = math.prod(shape)
+    buf = get_buffer_pool().allocate(numel * torch.empty(0, dtype=dtype).element_size(), dtype, tuple(shape))
+    return _wrap_output(buf, tuple(shape), dtype), buf.buffer
+
+
+def _rows(t, on_torch, name, heads_dims=None):
+    """_Arg and L.Rows of [..., heads, head_dim] rows, leading dimensions as one."""
+    if on_torch and isinstance(t, torch.Tensor) and t.is_cuda and t.dim() > 3:
+        t = t.reshape(-1, *t.shape[-2:])
+    a = _Arg(t, on_torch, name)
+    if len(a.shape) < 3:
+        raise ValueError(f"{name}: expected [tokens, heads, head_dim], got {a.shape}")
+    tokens = math.prod(a.shape[:-2])
+    if heads_dims is not None and (tokens, *a.shape[-2:]) != heads_dims:
+        raise ValueError(f"{name}: shape {a.shape} does not match {heads_dims} rows")
+    return a, L.Rows(a.ptr, a.strides[-3], a.strides[-2]), tokens
+
+
+# ── norms and rotations ────────────────────────────────────────────────────────
+
+def rope_table(positions: int, rotary_dim: int, theta: float = 10000.0) -> torch.Tensor:
+    """float32 [positions, rotary_dim] on the CPU: the cosines, then the sines, of
+    position * theta^(-2i / rotary_dim), computed in 64 bits and rounded once."""
+    if rotary_dim < 0 or rotary_dim % 2:
+        raise ValueError(f"rotary_dim {rotary_dim} is not an even number")
+    freq = theta ** (-torch.arange(0, rotary_dim, 2, dtype=torch.float64) / max(rotary_dim, 1))
+    angle = torch.arange(positions, dtype=torch.float64)[:, None] * freq
+    return torch.cat([angle.cos(), angle.sin()], dim=1).float()
+
+
+def _qk_desc(on_torch, q, k, q_weight, k_weight, table, positions, eps, interleaved):
+    """(L.QkDesc, shape of q, shape of k, dtype, what must stay alive)."""
+    qa, qrows, tokens = _rows(q, on_torch, "q")
+    heads, dim = qa.shape[-2:]
+    ka, krows, _ = _rows(k, on_torch, "k", (tokens, _get_shape(k)[-2] if len(_get_shape(k)) > 2 else -1, dim))
+    if ka.dtype != qa.dtype:
+        raise ValueError("q and k must share a dtype")
+    wa = [None if w is None else _Arg(w, on_torch, n) for w, n in ((q_weight, "q_weight"), (k_weight, "k_weight"))]
+    for w, n in zip(wa, ("q_weight", "k_weight")):
+        if w is not None and w.shape != (dim,):
+            raise ValueError(f"{n}: shape {w.shape}, expected ({dim},)")
+    given = [w.dtype for w in wa if w is not None]
+    if len(set(given)) > 1:
+        raise ValueError("q_weight and k_weight must share a dtype")
+    ta = _Arg(table, on_torch, "table", (torch.float32,))
+    if len(ta.shape) != 2 or ta.shape[1] > dim or ta.shape[1] % 2:
+        raise ValueError(f"table: shape {ta.shape} is not [positions, rotary_dim] with an even rotary_dim <= {dim}")
+    if ta.strides[0] != ta.shape[1] and ta.shape[0] > 1:
+        ta = _Arg(table.contiguous(), on_torch, "table", (torch.float32,))
+    pa = _Arg(positions, on_torch, "positions", _INTS, integer=True)
+    if math.prod(pa.shape) != tokens:
+        raise ValueError(f"positions: {pa.shape} for {tokens} tokens")
+    d = L.QkDesc()
+    d.tokens, d.q_heads, d.kv_heads, d.head_dim, d.rotary_dim = tokens, heads, ka.shape[-2], dim, ta.shape[1]
+    d.interleaved, d.dtype = int(bool(interleaved)), ojx_dtype(qa.dtype)
+    d.dtype_weight = ojx_dtype(given[0]) if given else d.dtype
+    d.positions_int64, d.eps = int(pa.dtype == torch.int64), eps
+    d.q, d.k = qrows, krows
+    d.q_weight, d.k_weight = (w.ptr if w is not None else None for w in wa)
+    d.table, d.table_rows, d.positions = ta.ptr, ta.shape[0], pa.ptr
+    return d, qa.dtype, given[0] if given else qa.dtype, (qa, ka, wa, ta, pa)
+
+
+def _qk_forward(q, k, q_weight, k_weight, table, positions, eps, interleaved):
+    on_torch = _on_torch(q)
+    d, dtype, _, keep = _qk_desc(on_torch, q, k, q_weight, k_weight, table, positions, eps, interleaved)
+    q_out, qp = _empty(_get_shape(q), dtype, on_torch)
+    k_out, kp = _empty(_get_shape(k), dtype, on_torch)
+    L.check(L.lib().ojx_qk_norm_rope(_ref(d), qp, kp, _stream(on_torch)), "qk_norm_rope")
+    return q_out, k_out
+
+
+def _qk_backward(gq, gk, q, k, q_weight, k_weight, table, positions, eps, interleaved, want_weights=True):
+    """(dq, dk, dq_weight, dk_weight) of qk_norm_rope; the weights' None where not wanted."""
+    on_torch = _on_torch(q)
+    d, dtype, wdtype, keep = _qk_desc(on_torch, q, k, q_weight, k_weight, table, positions, eps, interleaved)
+    ga, gq_rows, _ = _rows(gq, on_torch, "grad of q", (d.tokens, d.q_heads, d.head_dim))
+    gb, gk_rows, _ = _rows(gk, on_torch, "grad of k", (d.tokens, d.kv_heads, d.head_dim))
+    if ga.dtype != dtype or gb.dtype != dtype:
+        raise ValueError("gradients must have the dtype of q and k")
+    dq, dqp = _empty(_get_shape(q), dtype, on_torch)
+    dk, dkp = _empty(_get_shape(k), dtype, on_torch)
+    out, ptrs = [], []
+    for w in (q_weight, k_weight):
+        t, p = _empty((d.head_dim,), wdtype, on_torch) if w is not None and want_weights else (None, None)
+        out.append(t)
+        ptrs.append(p)
+    L.check(L.lib().ojx_qk_norm_rope_backward(_ref(d), _ref(gq_rows), _ref(gk_rows), dqp, dkp, *ptrs,
+                                              _stream(on_torch)), "qk_norm_rope backward")
+    return dq, dk, out[0], out[1]
+
+
+def qk_norm_rope(q, k, q_weight, k_weight, table, positions, eps: float = 1e-6, interleaved: bool = False):
+    """Norm and rotate query and key heads in one pass: for every row x of q and k,
+    y = rotate(weight * x / sqrt(mean(x^2) + eps)).
+
+    q [..., q_heads, head_dim] and k [..., kv_heads, head_dim] share their leading
+    dimensions (the tokens) and a dtype (float32, bfloat16, float16); weights are
+    [head_dim] or None (ones); table is rope_table(...) on the device, its width the
+    number of rotated elements; positions holds one row of it per token (int32 or int64;
+    a position outside the table gives NaN and ValueError at the next synchronize).
+    Pairs are (i, i + rotary_dim/2), or (2i, 2i + 1) when `interleaved`.  Sums run in
+    fp32; outputs are rounded once to the inputs' dtype.  Returns dense (q, k).
+    Differentiable in q, k and the weights (QKNormRopeFunction)."""
+    if torch.is_grad_enabled() and any(getattr(t, "requires_grad", False) for t in (q, k, q_weight, k_weight)):
+        from torchcl.autograd import QKNormRopeFunction
+        return QKNormRopeFunction.apply(q, k, q_weight, k_weight, table, positions, eps, interleaved)
+    return _qk_forward(q, k, q_weight, k_weight, table, positions, eps, interleaved)
+
+
+def qkv_to_cache(q, k, v, q_weight, k_weight, table, positions, cache: "KVCache", slots, eps: float = 1e-6,
+                 interleaved: bool = False):
+    """qk_norm_rope for serving: returns the normed and rotated q; the normed and rotated
+    k (unrounded) and v go straight into `cache` at `slots` ([tokens], int32 or int64;
+    a negative slot skips the token's keys and values)."""
+    on_torch = _on_torch(q)
+    d, dtype, _, keep = _qk_desc(on_torch, q, k, q_weight, k_weight, table, positions, eps, interleaved)
+    va, v_rows, _ = _rows(v, on_torch, "v", (d.tokens, d.kv_heads, d.head_dim))
+    if va.dtype != dtype:
+        raise ValueError("q, k and v must share a dtype")
+    sa = _Arg(slots, on_torch, "slots", _INTS, integer=True)
+    if math.prod(sa.shape) != d.tokens:
+        raise ValueError(f"slots: {sa.shape} for {d.tokens} tokens")
+    q_out, qp = _empty(_get_shape(q), dtype, on_torch)
+    L.check(L.lib().ojx_qkv_to_cache(_ref(d), _ref(v_rows), qp, _ref(cache._use()), sa.ptr,
+                                     int(sa.dtype == torch.int64), _stream(on_torch)), "qkv_to_cache")
+    return q_out
+
+
+# ── the cache ────────────────────────────────────────────────────────────────
+
+class KVCache:
+    """Keys and values in pages [num_pages, kv_heads, page_size, head_dim].
+
+    format "bfloat16" or "float16" stores rows as they are; "int8" and "float8" (e4m3)
+    store eight bits an element and one float32 step per row (a head of a token):
+    step = max|x| / 127 or / 448, read back as stored * step.  A row with a NaN or an
+    infinity reads back as NaN.  Token slot s is row s % page_size of page s // page_size;
+    which pages make up a sequence is the caller's page table.  head_dim is a multiple of
+    16 up to 512 (64 or 128 for tree_attention).
+
+    The constructor takes zeroed pages from torchcl's pool; from_pages wraps tensors that
+    exist.  Calls that share a cache are ordered by their streams, as for any buffer; a
+    slot given twice in one call holds one of the two."""
+
+    def __init__(self, num_pages: int, page_size: int, kv_heads: int, head_dim: int, format: str = "int8"):
+        if format not in _FORMAT_DTYPES:
+            raise ValueError(f"unknown cache format {format!r}: one of {sorted(_FORMAT_DTYPES)}")
+        if min(num_pages, page_size, kv_heads) < 1:
+            raise ValueError("a cache has at least one page, row and head")
+        if head_dim < 16 or head_dim > 512 or head_dim % 16:
+            raise ValueError(f"head_dim {head_dim} is not a multiple of 16 up to 512")
+        pool = get_buffer_pool()
+        rows = num_pages * page_size * kv_heads
+        quantised = format in ("int8", "float8")
+        self._pages = [pool.allocate(rows * head_dim * (1 if quantised else 2)) for _ in "kv"]
+        self._pages += [pool.allocate(rows * 4) for _ in "kv"] if quantised else [None, None]
+        for buf in self._pages:
+            if buf is not None:
+                pool.zero_fill(buf)
+        self._owned = True
+        self._set(num_pages, page_size, kv_heads, head_dim, format)
+
+    def __del__(self):
+        if getattr(self, "_owned", False):
+            for buf in self._pages:
+                try:
+                    get_buffer_pool().free(buf)
+                except Exception:
+                    pass
+
+    @classmethod
+    def from_pages(cls, k_pages, v_pages, k_scale=None, v_scale=None) -> "KVCache":
+        """A cache over dense torch CUDA tensors: pages [num_pages, kv_heads, page_size,
+        head_dim] of bfloat16, float16, int8 or float8_e4m3fn, and for the last two the
+        steps, float32 [num_pages, kv_heads, page_size]."""
+        formats = {v: k for k, v in _FORMAT_DTYPES.items()}
+        for t, n in ((k_pages, "k_pages"), (v_pages, "v_pages")):
+            if not (isinstance(t, torch.Tensor) and t.is_cuda and t.is_contiguous() and t.dim() == 4):
+                raise ValueError(f"{n}: expected a dense 4-D CUDA tensor")
+            if t.dtype not in formats:
+                raise ValueError(f"{n}: dtype {t.dtype}, expected one of {[str(d) for d in formats]}")
+        if k_pages.shape != v_pages.shape or k_pages.dtype != v_pages.dtype:
+            raise ValueError("k_pages and v_pages must share shape and dtype")
+        fmt = formats[k_pages.dtype]
+        if (fmt in ("int8", "float8")) != (k_scale is not None) or (k_scale is None) != (v_scale is None):
+            raise ValueError("steps belong to 8-bit pages, and only to them")
+        for t, n in ((k_scale, "k_scale"), (v_scale, "v_scale")):
+            if t is not None and not (t.is_cuda and t.is_contiguous() and t.dtype == torch.float32
+                                      and t.shape == k_pages.shape[:3]):
+                raise ValueError(f"{n}: expected dense float32 {tuple(k_pages.shape[:3])}")
+        self = cls.__new__(cls)
+        self._owned = False
+        self._pages = [k_pages, v_pages, k_scale, v_scale]
+        pages, heads, size, dim = k_pages.shape
+        if min(pages, heads, size) < 1:
+            raise ValueError("a cache has at least one page, row and head")
+        if dim < 16 or dim > 512 or dim % 16:
+            raise ValueError(f"head_dim {dim} is not a multiple of 16 up to 512")
+        self._set(pages, size, heads, dim, fmt)
+        return self
+
+    def _set(self, num_pages, page_size, kv_heads, head_dim, format):
+        self.num_pages, self.page_size, self.kv_heads = num_pages, page_size, kv_heads
+        self.head_dim, self.format = head_dim, format
+        addr = [None if b is None else b.buffer if isinstance(b, CLBuffer) else b.data_ptr() for b in self._pages]
+        self._desc = L.KVCacheDesc(*addr, num_pages, page_size, kv_heads, head_dim, L.KV_FORMATS[format])
+
+    def _use(self) -> "L.KVCacheDesc":
+        for buf in self._pages:
+            if isinstance(buf, CLBuffer):
+                note_use(buf)  # a graph being captured must keep it
+        return self._desc
+
+    def append(self, k, v, slots) -> None:
+        """Write keys and values [tokens, kv_heads, head_dim] (float32, bfloat16 or
+        float16) to `slots` ([tokens], int32 or int64; a negative slot is skipped)."""
+        on_torch = _on_torch(k)
+        ka, k_rows, n = _rows(k, on_torch, "k")
+        if ka.shape[-2:] != (self.kv_heads, self.head_dim):
+            raise ValueError(f"k: rows {ka.shape[-2:]}, the cache holds {(self.kv_heads, self.head_dim)}")
+        va, v_rows, _ = _rows(v, on_torch, "v", (n, self.kv_heads, self.head_dim))
+        if va.dtype != ka.dtype:
+            raise ValueError("k and v must share a dtype")
+        sa = _Arg(slots, on_torch, "slots", _INTS, integer=True)
+        if math.prod(sa.shape) != n:
+            raise ValueError(f"slots: {sa.shape} for {n} tokens")
+        L.check(L.lib().ojx_kv_append(_ref(self._use()), _ref(k_rows), _ref(v_rows), ojx_dtype(ka.dtype), n, sa.ptr,
+                                      int(sa.dtype == torch.int64), _stream(on_torch)), "KVCache.append")
+
+    def read(self, slots, dtype: torch.dtype = torch.bfloat16):
+        """(k, v), dense [tokens, kv_heads, head_dim] of `dtype`, as the cache holds them
+        at `slots`; a negative slot gives zeros."""
+        on_torch = _on_torch(slots)
+        code = ojx_dtype(dtype)
+        sa = _Arg(slots, on_torch, "slots", _INTS, integer=True)
+        n = math.prod(sa.shape)
+        shape = (*sa.shape, self.kv_heads, self.head_dim)
+        k, kp = _empty(shape, dtype, on_torch)
+        v, vp = _empty(shape, dtype, on_torch)
+        L.check(L.lib().ojx_kv_read(_ref(self._use()), kp, vp, code, n, sa.ptr, int(sa.dtype == torch.int64),
+                                    _stream(on_torch)), "KVCache.read")
+        return k, v
+
+    def keep_path(self, page_table, context_lens, path, count) -> None:
+        """After verify_drafts: move the accepted nodes' rows, at context_lens[b] +
+        path[b][0..count[b]], to context_lens[b] + 0, 1, ...; the sequence then holds
+        context_lens[b] + 1 + count[b] tokens."""
+        on_torch = _on_torch(path)
+        pa = _Arg(path, on_torch, "path", (torch.int32,), integer=True)
+        ta = _Arg(page_table, on_torch, "page_table", (torch.int32,), integer=True)
+        ca = _Arg(context_lens, on_torch, "context_lens", (torch.int32,), integer=True)
+        na = _Arg(count, on_torch, "count", (torch.int32,), integer=True)
+        if len(pa.shape) != 2 or len(ta.shape) != 2:
+            raise ValueError("path is [batch, tokens] and page_table [batch, pages]")
+        batch, tokens = pa.shape
+        if ta.shape[0] != batch or ca.shape != (batch,) or na.shape != (batch,):
+            raise ValueError(f"page_table {ta.shape}, context_lens {ca.shape}, count {na.shape} for {batch} sequences")
+        L.check(L.lib().ojx_kv_keep_path(_ref(self._use()), ta.ptr, ta.shape[1], ca.ptr, pa.ptr, na.ptr, batch, tokens,
+                                         _stream(on_torch)), "KVCache.keep_path")
+
+
+# ── attention over the cache ─────────────────────────────────────────────────
+
+def tree_mask(parents) -> torch.Tensor:
+    """The ancestors of each node of draft trees, as tree_attention's mask: int64
+    [..., tokens, ceil(tokens / 64)] on the CPU; bit j % 64 of word j / 64 of row i is set
+    when node j is i or an ancestor of i.  parents [tokens] or [batch, tokens]; a negative
+    parent starts a tree.  ValueError unless parents[i] < i."""
+    p = torch.as_tensor(parents).cpu().long()
+    tokens = p.shape[-1]
+    rows = p.reshape(math.prod(p.shape[:-1]), tokens)
+    if bool((rows >= torch.arange(tokens)).any()):
+        raise ValueError("a node's parent must come before it")
+    words = (tokens + 63) // 64
+    out = torch.zeros(*rows.shape, words, dtype=torch.int64)
+    at = torch.arange(rows.shape[0])
+    for i in range(tokens):
+        known = rows[:, i] >= 0
+        out[known, i] = out[at[known], rows[known, i]]
+        bit = 1 << (i % 64)
+        out[:, i, i // 64] |= bit - (1 << 64) if i % 64 == 63 else bit
+    return out.reshape(*p.shape, words)
+
+
+def tree_attention(q, cache: KVCache, page_table, context_lens, mask=None, draft_lens=None,
+                   scale: float | None = None):
+    """softmax(scale q k^T) v of each sequence's newest tokens over its pages.
+
+    q [batch, tokens, q_heads, head_dim], bfloat16 or float16 (a 16-bit cache has the same
+    dtype); head h reads key head h // (q_heads / kv_heads).  Key position j of sequence b
+    is row j % page_size of page page_table[b][j // page_size].  Query i sees positions
+    0 .. context_lens[b] - 1 and, of the new tokens j < draft_lens[b] (default: all), which
+    have been written at context_lens[b] + j, those whose bit is set in mask (tree_mask;
+    [tokens, words] or [batch, tokens, words]) or, without a mask, j <= i.  tokens = 1
+    without a mask is a decoding step.  Queries i >= draft_lens[b], and queries that see
+    nothing, give zeros; nothing a query does not see reaches it, whatever it holds.
+    Returns dense [batch, tokens, q_heads, head_dim]."""
+    on_torch = _on_torch(q)
+    qa = _Arg(q, on_torch, "q", (torch.bfloat16, torch.float16))
+    if len(qa.shape) != 4 or qa.shape[3] != cache.head_dim:
+        raise ValueError(f"q: shape {qa.shape} is not [batch, tokens, q_heads, {cache.head_dim}]")
+    batch, tokens, heads, dim = qa.shape
+    if heads % cache.kv_heads:
+        raise ValueError(f"{heads} query heads do not share {cache.kv_heads} key heads evenly")
+    ta = _Arg(page_table, on_torch, "page_table", (torch.int32,), integer=True)
+    ca = _Arg(context_lens, on_torch, "context_lens", (torch.int32,), integer=True)
+    if len(ta.shape) != 2 or ta.shape[0] != batch or ca.shape != (batch,):
+        raise ValueError(f"page_table {ta.shape} and context_lens {ca.shape} for {batch} sequences")
+    da = ma = None
+    if draft_lens is not None:
+        da = _Arg(draft_lens, on_torch, "draft_lens", (torch.int32,), integer=True)
+        if da.shape != (batch,):
+            raise ValueError(f"draft_lens {da.shape} for {batch} sequences")
+    if mask is not None:
+        ma = _Arg(mask, on_torch, "mask", (torch.int64,), integer=True)
+        rows = (tokens, (tokens + 63) // 64)
+        if ma.shape not in (rows, (batch, *rows)):
+            raise ValueError(f"mask: shape {ma.shape} is neither {rows} nor {(batch, *rows)}")
+    out, op = _empty(qa.shape, qa.dtype, on_torch)
+    d = L.TreeAttentionDesc()
+    d.cache = cache._use()
+    d.q, d.out = qa.ptr, op
+    d.q_stride_b, d.q_stride_t, d.q_stride_h = qa.strides[:3]
+    d.dtype, d.batch, d.tokens, d.q_heads = ojx_dtype(qa.dtype), batch, tokens, heads
+    d.page_table, d.table_width, d.context_lens = ta.ptr, ta.shape[1], ca.ptr
+    d.draft_lens = da.ptr if da is not None else None
+    if ma is not None:
+        d.mask, d.mask_stride_b = ma.ptr, math.prod(ma.shape[1:]) if len(ma.shape) == 3 else 0
+    d.scale = dim ** -0.5 if scale is None else scale
+    L.check(L.lib().ojx_tree_attention(_ref(d), _stream(on_torch)), "tree_attention")
+    return out
+
+
+# ── verification ─────────────────────────────────────────────────────────────
+
+def verify_drafts(target_probs, tokens, parents, uniforms, draft_probs=None):
+    """Which drafts the target accepts, and the token that follows them.
+
+    tokens and parents, int32 [batch, nodes]: node 0 is the root, node i > 0 carries
+    tokens[b][i], drafted after node parents[b][i] < i (a negative token: no node).
+    target_probs and draft_probs [batch, nodes, vocab] (float32, bfloat16 or float16)
+    hold the target's and the draft's probabilities of the token after each node;
+    without draft_probs a draft counts as certain (the draft's likeliest tokens).
+    uniforms float32 [batch, nodes] in [0, 1): u_i decides node i, u_0 the next token.
+    Nodes are tried in order, when their parent is the node reached; a rejection leaves
+    max(p - q, 0) (or p without the token), renormalised, to the next child and finally to
+    the next token, so accepted tokens and the next one are distributed as the target's.
+    Returns int32 path [batch, nodes] (the root and the accepted nodes, then -1), count
+    [batch] (accepted drafts) and next_token [batch] (-1: the row holds no probability).
+    Sums are exact in units of 2^-38, so results do not depend on the launch shape."""
+    on_torch = _on_torch(target_probs)
+    pa = _Arg(target_probs, on_torch, "target_probs")
+    if len(pa.shape) != 3:
+        raise ValueError(f"target_probs: shape {pa.shape} is not [batch, nodes, vocab]")
+    batch, nodes, vocab = pa.shape
+    qa = None
+    if draft_probs is not None:
+        qa = _Arg(draft_probs, on_torch, "draft_probs", (pa.dtype,))
+        if qa.shape != pa.shape:
+            raise ValueError(f"draft_probs: shape {qa.shape}, target_probs has {pa.shape}")
+    xa = _Arg(tokens, on_torch, "tokens", (torch.int32,), integer=True)
+    ra = _Arg(parents, on_torch, "parents", (torch.int32,), integer=True)
+    ua = _Arg(uniforms, on_torch, "uniforms", (torch.float32,))
+    for a, n in ((xa, "tokens"), (ra, "parents"), (ua, "uniforms")):
+        if a.shape != (batch, nodes):
+            raise ValueError(f"{n}: shape {a.shape}, expected {(batch, nodes)}")
+    if ua.strides != _strides(ua.shape):
+        ua = _Arg(uniforms.contiguous(), on_torch, "uniforms")
+    path, path_p = _empty((batch, nodes), torch.int32, on_torch)
+    count, count_p = _empty((batch,), torch.int32, on_torch)
+    token, token_p = _empty((batch,), torch.int32, on_torch)
+    d = L.VerifyDesc()
+    d.target, d.target_stride_b, d.target_stride_t = pa.ptr, pa.strides[0], pa.strides[1]
+    if qa is not None:
+        d.draft, d.draft_stride_b, d.draft_stride_t = qa.ptr, qa.strides[0], qa.strides[1]
+    d.vocab, d.token_ids, d.parents, d.uniforms = vocab, xa.ptr, ra.ptr, ua.ptr
+    d.path, d.count, d.next_token = path_p, count_p, token_p
+    d.batch, d.tokens, d.dtype = batch, nodes, ojx_dtype(pa.dtype)
+    L.check(L.lib().ojx_verify_drafts(_ref(d), _stream(on_torch)), "verify_drafts")
+    return path, count, token
+
+
+__all__ = ["KVCache", "qk_norm_rope", "qkv_to_cache", "rope_table", "tree_attention", "tree_mask", "verify_drafts"]
