@@ -4,6 +4,7 @@
 #include <algorithm>
 #include "qk_cache.cuh"
 #include "tree_attention.cuh"
+#include "tree_attention_tc.cuh"
 #include "verify.cuh"
 
 namespace ojx {
@@ -174,8 +175,38 @@ static int launch_tree(TaParams& p, cudaStream_t s) {
   return st;
 }
 
+template <int FMT, int D, int QT>
+static int launch_tree_tc(TaParams& p, cudaStream_t s) {
+  using L = TcLayout<FMT, D, QT>;
+  auto kern = tree_attention_tc_kernel<FMT, D, QT>;
+  int st = ensure_smem_attr(reinterpret_cast<const void*>(kern), L::SMEM);
+  if (st) return st;
+  const int rows = p.tokens * p.group, tile_rows = QT * TC_BN;
+  p.row_tiles = (rows + tile_rows - 1) / tile_rows;
+  const int64_t per_seq = static_cast<int64_t>(p.cache.kv_heads) * p.row_tiles;
+  const int64_t most = p.batch * per_seq * ((static_cast<int64_t>(p.width) * p.cache.page_size + TC_BN - 1) / TC_BN);
+  if (per_seq > INT32_MAX) return set_error(OJX_ERR_INVALID, "ojx_tree_attention: too many rows");
+  const int ctas = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(most, current_props().sm_count)));
+  const size_t slots = static_cast<size_t>(ctas) * 2 * tile_rows;
+  char* ws = static_cast<char*>(stream_workspace(s, slots * (D * 4 + 8), 8, false));
+  if (!ws) return workspace_error();
+  p.part_o = reinterpret_cast<float*>(ws);
+  p.part_ml = reinterpret_cast<float2*>(ws + slots * D * 4);
+  kern<<<ctas, TC_THREADS, L::SMEM, s>>>(p, g_wait_budget.load());
+  if ((st = launched("tree_attention_tc launch"))) return st;
+  const int64_t all = static_cast<int64_t>(p.batch) * p.cache.kv_heads * rows;
+  tree_attention_parts_kernel<D><<<static_cast<unsigned>((all + 3) / 4), 128, 0, s>>>(p, tile_rows, TC_BN, ctas);
+  return launched("tree_attention parts launch");
+}
+
 template <int FMT>
 static int launch_tree_fmt(TaParams& p, cudaStream_t s) {
+  const int rows = p.tokens * p.group;
+  if (rows > 32) {
+    const bool two = rows > 128;
+    if (p.cache.head_dim == 64) return two ? launch_tree_tc<FMT, 64, 2>(p, s) : launch_tree_tc<FMT, 64, 1>(p, s);
+    return two ? launch_tree_tc<FMT, 128, 2>(p, s) : launch_tree_tc<FMT, 128, 1>(p, s);
+  }
   const bool wide = p.tokens * p.group > 16;  // more than one 16-row tile
   if (p.cache.head_dim == 64) return wide ? launch_tree<FMT, 64, 2>(p, s) : launch_tree<FMT, 64, 1>(p, s);
   return wide ? launch_tree<FMT, 128, 2>(p, s) : launch_tree<FMT, 128, 1>(p, s);
@@ -360,7 +391,8 @@ int ojx_tree_attention(const ojx_tree_attention_desc* d, ojx_stream stream) {
   if (!d->q || !d->out || !d->context_lens || (d->table_width > 0 && !d->page_table))
     return set_error(OJX_ERR_INVALID, "ojx_tree_attention: NULL pointer");
   if (static_cast<int64_t>(d->tokens) * d->q_heads > INT32_MAX / 2 ||
-      static_cast<int64_t>(d->table_width) * c.page_size > INT32_MAX / 2)
+      static_cast<int64_t>(d->table_width) * c.page_size > INT32_MAX / 2 ||
+      c.num_pages * c.page_size > INT32_MAX / c.kv_heads)
     return set_error(OJX_ERR_INVALID, "ojx_tree_attention: too large");
   TaParams p{};
   p.cache = c;

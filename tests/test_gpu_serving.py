@@ -360,6 +360,9 @@ ATTEND = [  # contexts, drafts, tokens, q heads, kv heads, dim, dtype, page, mas
     ([40, 3, 0], [48, 1, 47], 48, 8, 2, 128, "bf16", 64, "tree"), ([300], [64], 64, 8, 1, 128, "f16", 128, "tree"),
     ([200, 0], [70, 70], 70, 2, 1, 64, "bf16", 16, "random"), ([0, 0, 9], [5, 0, 3], 5, 2, 2, 128, "f16", 4, "random"),
     ([77], [130], 130, 3, 1, 128, "bf16", 16, None), ([2500], [2], 2, 16, 1, 64, "bf16", 256, "tree"),
+    ([1300, 2, 128, 0, 640], [33, 7, 1, 40, 12], 40, 8, 2, 64, "f16", 16, "tree"), ([3000], [100], 100, 4, 2, 128, "bf16", 32, None),
+    ([384, 900], [66, 65], 66, 2, 1, 128, "f16", 5, "random"), ([4100, 130], [16, 16], 16, 16, 2, 64, "bf16", 64, "tree"),
+    ([126, 127, 128, 129], [2, 1, 5, 3], 5, 16, 1, 128, "bf16", 16, "tree"), ([0, 0], [0, 0], 9, 8, 1, 64, "f16", 3, None),
     ([1], [1], 1, 40, 1, 128, "bf16", 1, None), ([0, 0], [0, 0], 3, 2, 1, 64, "f16", 3, None),
 ]
 
