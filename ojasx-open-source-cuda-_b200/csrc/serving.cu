@@ -2,6 +2,7 @@
 // checks, launch shapes and workspaces.  A translation unit of its own, with its own
 // device error word, so that it compiles beside the GEMM kernels.
 #include <algorithm>
+#include "tmap.h"
 #include "qk_cache.cuh"
 #include "tree_attention.cuh"
 #include "tree_attention_tc.cuh"
@@ -185,14 +186,27 @@ static int launch_tree_tc(TaParams& p, cudaStream_t s) {
   p.row_tiles = (rows + tile_rows - 1) / tile_rows;
   const int64_t per_seq = static_cast<int64_t>(p.cache.kv_heads) * p.row_tiles;
   const int64_t most = p.batch * per_seq * ((static_cast<int64_t>(p.width) * p.cache.page_size + TC_BN - 1) / TC_BN);
-  if (per_seq > INT32_MAX) return set_error(OJX_ERR_INVALID, "ojx_tree_attention: too many rows");
+  if (per_seq > INT32_MAX || most > INT32_MAX) return set_error(OJX_ERR_INVALID, "ojx_tree_attention: too large");
   const int ctas = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(most, current_props().sm_count)));
   const size_t slots = static_cast<size_t>(ctas) * 2 * tile_rows;
   char* ws = static_cast<char*>(stream_workspace(s, slots * (D * 4 + 8), 8, false));
   if (!ws) return workspace_error();
   p.part_o = reinterpret_cast<float*>(ws);
   p.part_ml = reinterpret_cast<float2*>(ws + slots * D * 4);
-  kern<<<ctas, TC_THREADS, L::SMEM, s>>>(p, g_wait_budget.load());
+  // A TMA box holds rows of one page, so the page size decides its rows; the swizzle's
+  // pattern spans eight.
+  CUtensorMap tk{}, tv{};
+  p.box_rows = 0;
+  if (!L::QUANT && p.cache.page_size % 8 == 0) {
+    int r = 64;
+    while (p.cache.page_size % r) r /= 2;
+    const CUtensorMapDataType dt = FMT == TA_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
+    const int64_t all = p.cache.num_pages * p.cache.kv_heads * p.cache.page_size;
+    if ((st = make_tmap_2d_sw128(&tk, dt, 2, p.cache.k, D, all, D * 2, 64, r))) return st;
+    if ((st = make_tmap_2d_sw128(&tv, dt, 2, p.cache.v, D, all, D * 2, 64, r))) return st;
+    p.box_rows = r;
+  }
+  kern<<<ctas, TC_THREADS, L::SMEM, s>>>(tk, tv, p, g_wait_budget.load());
   if ((st = launched("tree_attention_tc launch"))) return st;
   const int64_t all = static_cast<int64_t>(p.batch) * p.cache.kv_heads * rows;
   tree_attention_parts_kernel<D><<<static_cast<unsigned>((all + 3) / 4), 128, 0, s>>>(p, tile_rows, TC_BN, ctas);

@@ -4,20 +4,24 @@
 // A persistent CTA takes an equal share of all 128-key tiles of the call (TaSplit): runs
 // of tiles of consecutive segments (sequence, key head, QT x 128 rows).
 //
-//   warps 0-3    producers: page lookups, cp.async of K and V rows into the MMA's swizzled
-//                layout; 8-bit rows land in a private ring first and are widened to f16.
+//   warp 13      loader: page lookups, and TMA copies of K and V.  16-bit rows go straight
+//                into the MMA's swizzled layout (boxes of 8 to 64 rows of one page); runs of
+//                8-bit rows land in a ring of half tiles, with their steps.
+//   warps 0-3    8-bit rows: widen them to f16 in the MMA's layout.  16-bit rows: zero what
+//                must not reach a product in a sequence's last tiles; or, where the page size
+//                is no multiple of eight rows, load all rows themselves with cp.async.
 //   warps 4-11   softmax of unit 0 (4-7) and 1 (8-11), one row per thread (TMEM lane).
 //                QT = 2: a unit is a tile of 128 rows and sees every key tile.  QT = 1: both
 //                units share the rows and take alternate key tiles, joined at the end.
-//   warp 12      MMA issuer (13-15 are idle): O_t += P_t V of a unit's tile, then S_t = Q K^T
+//   warp 12      MMA issuer (14, 15 are idle): O_t += P_t V of a unit's tile, then S_t = Q K^T
 //                of its next one, while the other unit is in its softmax.
 //
 // Tensor memory: S_0 [0,128), S_1 [128,256), O_0 [256, 256+D), O_1 [256+D, 256+2D).  A
 // softmax row holds its 128 scores in registers and writes the weights P_t, two 16-bit
 // values a column, over S_t, from where the second product reads them (its A operand);
 // shared memory is left to K and V.  bf16 values need bf16 weights, whose eight bits would
-// double the output's rounding: columns 64-127 take the weights' next eight bits and a
-// second product adds them.
+// double the output's rounding: each 32 columns keep the weights' next eight bits in their
+// second half, and a second product adds them.
 // K and V are produced in the order in which the MMAs consume them.
 #pragma once
 #include "tree_attention.cuh"
@@ -27,8 +31,8 @@ namespace ojx {
 constexpr int TC_BN = 128;
 constexpr int TC_PRODUCERS = 128;
 constexpr int TC_THREADS = 512;
-// Registers a thread after the split: 128 at launch (65,536 / 512), then 4 x 32 x (80 + 56)
-// + 8 x 32 x 184 = 64,512, within the launch's 65,536.
+// Registers a thread after the split: 128 at launch (65,536 / 512), then 4 x 32 x (112 + 72)
+// + 8 x 32 x 160 = 64,512, within the launch's 65,536.
 
 template <int FMT, int D, int QT>
 struct TcLayout {
@@ -36,23 +40,25 @@ struct TcLayout {
   static constexpr int DB = D / 64;
   static constexpr int LEAD = QT == 1 ? 2 : 1;          // K tiles before the first V tile
   static constexpr int TILE = TC_BN * D * 2;            // a K or V tile as the MMA reads it
-  static constexpr int SLACK = 512;                     // to round the base up (it is aligned already, see the kernel)
-  static constexpr int FIT = (227 * 1024 - 256 - SLACK - 2048 - QT * TILE) / TILE;  // tile buffers
+  static constexpr int BARS = 512;
+  static constexpr int SLACK = 256;                     // to round the base up (it is aligned already, see the kernel)
+  static constexpr int FIT = (227 * 1024 - BARS - SLACK - 2048 - QT * TILE) / TILE;  // tile buffers
   static constexpr int KST = QUANT ? 2 : D == 64 ? 4 : 3;
-  static constexpr int VST = QUANT ? (D == 64 || QT == 1 ? 2 : 1) : D == 64 ? 4 : FIT - 3;
+  static constexpr int VST = QUANT ? 2 : D == 64 ? 4 : FIT - 3;
   static_assert(QUANT || KST + VST <= FIT, "shared memory");
   static constexpr int HALF = 64 * D;                   // half a tile of 8-bit rows
-  static constexpr int HALVES = !QUANT ? 0 : D == 64 ? 12 : 6;    // ring of them
+  static constexpr int HALVES = !QUANT ? 0 : D == 64 ? 12 : QT == 1 ? 6 : 3;  // ring of them
   static constexpr int STEPS = !QUANT ? 0 : (QT == 1 ? 3 : 2) + KST;  // tiles whose steps are kept
+  static constexpr int STEP_BYTES = 1568;
   static constexpr int RAWSTEP_RING = QUANT ? 4 : 0;
   static constexpr int OFF_K = QT * TILE;
   static constexpr int OFF_V = OFF_K + KST * TILE;
   static constexpr int OFF_RAW = OFF_V + VST * TILE;
   static constexpr int OFF_ROWS = OFF_RAW + HALVES * HALF;        // 4 x 128 row numbers
-  static constexpr int OFF_STEPS = OFF_ROWS + 4 * 512;            // [STEPS][3][128] floats
-  static constexpr int OFF_RAWSTEP = OFF_STEPS + STEPS * 1536;
+  static constexpr int OFF_STEPS = OFF_ROWS + (QUANT ? 0 : 4 * 512);            // [STEPS][3][128] floats, [2][4] ints
+  static constexpr int OFF_RAWSTEP = OFF_STEPS + STEPS * STEP_BYTES;
   static constexpr int OFF_BAR = OFF_RAWSTEP + RAWSTEP_RING * 1024;
-  static constexpr int SMEM = OFF_BAR + 256 + SLACK;
+  static constexpr int SMEM = OFF_BAR + BARS + SLACK;
   static_assert(SMEM <= 227 * 1024, "shared memory");
 };
 
@@ -81,9 +87,9 @@ __device__ __forceinline__ int ta_tiles(const TaParams& p, int b, int unit) {
 }
 
 // Where a CTA's share begins: sequence, tiles before that sequence, first and last tile.
+// (A call has fewer than 2^31 tiles.)
 struct TaShare {
-  int b;
-  long long base, u, end;
+  int b, base, u, end;
 };
 // By one warp; the lanes take equal strips of sequences.
 __device__ __forceinline__ TaShare ta_share_of(const TaParams& p, int per_seq, int unit, int cta, int ctas) {
@@ -102,8 +108,8 @@ __device__ __forceinline__ TaShare ta_share_of(const TaParams& p, int per_seq, i
   }
   const long long total = __shfl_sync(0xffffffffu, run, 31) * per_seq;
   TaShare s;
-  s.u = total * cta / ctas;
-  s.end = total * (cta + 1) / ctas;
+  s.u = static_cast<int>(total * cta / ctas);
+  s.end = static_cast<int>(total * (cta + 1) / ctas);
   s.b = 0;
   s.base = 0;
   const bool here = s.u < s.end && (run - mine) * per_seq <= s.u && s.u < run * per_seq;
@@ -116,7 +122,7 @@ __device__ __forceinline__ TaShare ta_share_of(const TaParams& p, int per_seq, i
       base += n;
     }
     s.b = b;
-    s.base = base;
+    s.base = static_cast<int>(base);
   }
   const unsigned who = __ballot_sync(0xffffffffu, here);
   const int src = who ? __ffs(who) - 1 : 0;
@@ -148,17 +154,17 @@ struct TaWalk {
   }
   __device__ __forceinline__ bool next(const TaParams& p, int per_seq, int unit, TaPart& o) {
     if (s.u >= s.end) return false;
-    while (s.u >= s.base + static_cast<long long>(tiles) * per_seq) {  // (ends: u < end <= all tiles)
-      s.base += static_cast<long long>(tiles) * per_seq;
+    while (s.u >= s.base + tiles * per_seq) {  // (ends: u < end <= all tiles)
+      s.base += tiles * per_seq;
       ++s.b;
       load(p, unit);
     }
-    const int at = static_cast<int>(s.u - s.base);
+    const int at = s.u - s.base;
     o.b = s.b;
     o.seg = at / tiles;
     o.t0 = at - o.seg * tiles;
     o.tiles = tiles;
-    o.n = static_cast<int>(min(static_cast<long long>(tiles - o.t0), s.end - s.u));
+    o.n = min(tiles - o.t0, s.end - s.u);
     o.ctx = ctx;
     o.drafts = drafts;
     o.first = first;
@@ -202,6 +208,32 @@ __device__ __forceinline__ float4 tc_lds4f(uint32_t a) {
   asm volatile("ld.shared.v4.f32 {%0,%1,%2,%3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(a) : "memory");
   return v;
 }
+// Two float32 operations an instruction.
+__device__ __forceinline__ uint64_t tc_pair(float a, float b) {
+  uint64_t r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+  return r;
+}
+__device__ __forceinline__ float2 tc_split(uint64_t v) {
+  float2 r;
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(v));
+  return r;
+}
+__device__ __forceinline__ uint64_t tc_fma2(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+__device__ __forceinline__ uint64_t tc_mul2(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ uint64_t tc_add2(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
 // Zeroes the non-finite 16-bit elements of a word; true if there were any.
 template <bool BF>
 __device__ __forceinline__ bool tc_clean(uint32_t& w) {
@@ -212,8 +244,68 @@ __device__ __forceinline__ bool tc_clean(uint32_t& w) {
   return any;
 }
 
+// The order in which a CTA's K and V tiles are produced, that of their use: within a part,
+// V(i - lead) then K(i) for i = 0 .. n + lead - 1.
+// `while (c.next(...))` visits them (one call site, so that the code exists once a role).
+struct TcCursor {
+  TaWalk walk;
+  TaPart part;
+  int i, lead;
+  bool v;           // V or K
+  uint32_t kc, vc;  // tiles of K and V before this one, over all parts
+  __device__ __forceinline__ void begin(const TaWalk& w, int ahead) {
+    walk = w;
+    lead = ahead;
+    part.n = 0;
+    i = ahead;  // past a part without tiles
+    v = true;
+    kc = vc = 0xffffffffu;
+    first = true;
+  }
+  bool first;
+  __device__ __forceinline__ bool next(const TaParams& p, int per_seq) {
+    if (first) {
+      first = false;
+      kc = vc = 0;
+    } else if (v) {
+      ++vc;
+      v = false;
+    } else {
+      ++kc;
+      v = true;
+      ++i;
+    }
+    while (true) {
+      if (i >= part.n + lead) {
+        if (!walk.next(p, per_seq, TC_BN, part)) return false;
+        i = 0;
+        v = true;
+      } else if (v && i < lead) {
+        v = false;
+      } else if (!v && i >= part.n) {
+        v = true;
+        ++i;
+      } else {
+        return true;
+      }
+    }
+  }
+  __device__ __forceinline__ uint32_t number() const { return v ? vc : kc; }
+  __device__ __forceinline__ int tile() const { return part.t0 + (v ? i - lead : i); }
+  __device__ __forceinline__ bool tail() const { return (tile() + 1) * TC_BN > part.ctx; }
+  // Number (as K tile) of the V tile at the cursor: i - lead of the min(i, n) before it here.
+  __device__ __forceinline__ uint32_t k_number() const { return kc - static_cast<uint32_t>(min(i, part.n) - (i - lead)); }
+};
+
+// Asynchronous copies of this thread so far arrive on `bar` when they have landed.
+__device__ __forceinline__ void tc_copies_arrive(uint32_t bar) {
+  asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(bar) : "memory");
+}
+
 template <int FMT, int D, int QT>
-__global__ void __launch_bounds__(TC_THREADS, 1) tree_attention_tc_kernel(const TaParams p, uint64_t budget) {
+__global__ void __launch_bounds__(TC_THREADS, 1) tree_attention_tc_kernel(const __grid_constant__ CUtensorMap tmK,
+                                                                          const __grid_constant__ CUtensorMap tmV,
+                                                                          const TaParams p, uint64_t budget) {
   using L = TcLayout<FMT, D, QT>;
   constexpr bool QUANT = L::QUANT, BF = FMT == TA_BF16;
   constexpr int KST = L::KST, VST = L::VST, LEAD = L::LEAD;
@@ -236,11 +328,15 @@ __global__ void __launch_bounds__(TC_THREADS, 1) tree_attention_tc_kernel(const 
   auto s_full = [&](int t) { return bar0 + 8u * (18 + t); };
   auto p_full = [&](int t) { return bar0 + 8u * (20 + t); };
   auto pv_done = [&](int t) { return bar0 + 8u * (22 + t); };
-  volatile int* s_abort = reinterpret_cast<volatile int*>(bars + 24);
-  uint32_t* s_tmem = reinterpret_cast<uint32_t*>(bars + 25);
-  volatile int* s_odd = reinterpret_cast<volatile int*>(bars + 26);  // a hidden non-finite value was met
-  TaShare* s_share = reinterpret_cast<TaShare*>(bars + 27);
-  static_assert(27 * 8 + sizeof(TaShare) <= 256 && KST <= 4 && VST <= 4, "barrier area");
+  auto v_land = [&](int s) { return bar0 + 8u * (24 + s); };  // TMA of a tile to be cleaned
+  auto raw_full = [&](int s) { return bar0 + 8u * (28 + s); };
+  auto raw_empty = [&](int s) { return bar0 + 8u * (40 + s); };
+  volatile int* s_abort = reinterpret_cast<volatile int*>(bars + 52);
+  uint32_t* s_tmem = reinterpret_cast<uint32_t*>(bars + 53);
+  volatile int* s_odd = reinterpret_cast<volatile int*>(bars + 54);  // a hidden non-finite value was met
+  TaShare* s_share = reinterpret_cast<TaShare*>(bars + 55);
+  static_assert(55 * 8 + sizeof(TaShare) <= L::BARS && KST <= 4 && VST <= 4 && L::HALVES <= 12, "barrier area");
+  const bool tma = !QUANT && p.box_rows > 0;
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int rows = p.tokens * p.group;
@@ -250,12 +346,17 @@ __global__ void __launch_bounds__(TC_THREADS, 1) tree_attention_tc_kernel(const 
     mbar_init(q_full, 8);
     mbar_init(done_bar, 1);
     for (int s = 0; s < KST; ++s) {
-      mbar_init(k_full(s), 4);
+      mbar_init(k_full(s), tma ? 1 : 4);
       mbar_init(k_empty(s), 1);
     }
     for (int s = 0; s < VST; ++s) {
       mbar_init(v_full(s), 4);
       mbar_init(v_empty(s), 1);
+      mbar_init(v_land(s), 1);
+    }
+    for (int s = 0; s < L::HALVES; ++s) {
+      mbar_init(raw_full(s), 33);
+      mbar_init(raw_empty(s), 4);
     }
     for (int t = 0; t < 2; ++t) {
       mbar_init(s_full(t), 1);
@@ -278,80 +379,147 @@ __global__ void __launch_bounds__(TC_THREADS, 1) tree_attention_tc_kernel(const 
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = *s_tmem;
-  TaWalk walk;
-  walk.begin(p, *s_share, TC_BN);
-  TaPart part;
 
   if (warp < 4) {
-    // ── producers ────────────────────────────────────────────────────────
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 80;");
+    // ── widening, cleaning, or loading by cp.async ─────────────────────────────────
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 112;");
     const int tid = threadIdx.x;
-    const uint8_t* kbase = static_cast<const uint8_t*>(p.cache.k);
-    const uint8_t* vbase = static_cast<const uint8_t*>(p.cache.v);
-    volatile int32_t* s_rows = reinterpret_cast<volatile int32_t*>(smem + L::OFF_ROWS);
-    // The sequence of copies: within a part, V(i - LEAD) then K(i) for i = 0 .. n + LEAD - 1.
-    struct Cursor {
-      TaWalk walk;
-      TaPart part;
-      int i;        // position in the part
-      bool v, live;  // K or V next; anything left
-      uint32_t kc, vc;  // tiles of K and V before this one, over all parts
-    };
-    auto settle = [&](Cursor& c) {  // move on to the next copy that exists
-      while (c.live) {
-        if (c.i >= c.part.n + LEAD) {
-          c.live = c.walk.next(p, per_seq, TC_BN, c.part);
-          c.i = 0;
-          c.v = true;
-        } else if (c.v && c.i < LEAD) {
-          c.v = false;
-        } else if (!c.v && c.i >= c.part.n) {
-          c.v = true;
-          ++c.i;
-        } else {
-          return;
+    TaWalk walk;
+    walk.begin(p, *s_share, TC_BN);
+    TcCursor in;
+    if constexpr (QUANT) {
+      constexpr int CPR = D / 16, PER = 64 * CPR / 128;  // 16-byte pieces per row; per thread and half
+      const int col = tid % CPR, row0 = tid / CPR;
+      uint32_t half_n = 0;
+      bool ok = true;
+      in.begin(walk, LEAD);
+      while (ok && in.next(p, per_seq)) {
+        const bool v = in.v, tail = in.tail();
+        const uint32_t n = in.number();
+        const int left = in.part.ctx + in.part.drafts - in.tile() * TC_BN;  // rows that exist
+        ok = __all_sync(0xffffffffu, mbar_wait(v ? v_empty(n % VST) : k_empty(n % KST), ((n / (v ? VST : KST)) & 1u) ^ 1u, budget, s_abort));
+        const uint32_t to = v ? sV0 + (n % VST) * L::TILE : sK0 + (n % KST) * L::TILE;
+#pragma unroll 1
+        for (int half = 0; half < 2 && ok; ++half, ++half_n) {
+          const int slot = half_n % L::HALVES;
+          ok = __all_sync(0xffffffffu, mbar_wait(raw_full(slot), (half_n / L::HALVES) & 1u, budget, s_abort));
+          if (!ok) break;
+          const uint4* raw = reinterpret_cast<const uint4*>(smem + L::OFF_RAW + slot * L::HALF) + tid;
+          uint4 w[PER];
+#pragma unroll
+          for (int i = 0; i < PER; ++i) w[i] = raw[i * 128];
+          if (!v && (tid >> 6) == half) {  // the row's steps, and the values' offset of the reference
+            const float2 st = *reinterpret_cast<const float2*>(smem + L::OFF_RAWSTEP + (n & 3) * 1024 + tid * 8);
+            float ks = st.x, vs = st.y;
+            if (tail && !(fabsf(ks) < INFINITY && fabsf(vs) < INFINITY)) {
+              ks = vs = 0.0f;  // as for the values: kept from rows that do not see the key
+              *s_odd = 1;
+            }
+            float* d = reinterpret_cast<float*>(smem + L::OFF_STEPS + (n % L::STEPS) * L::STEP_BYTES) + tid;
+            d[0] = ks == 0.0f ? 1.17549435e-38f : ks;  // (a row of zeros: its products are zero, and a hidden score stays -inf)
+            d[128] = vs;
+            d[256] = fminf(fmaxf(__log2f(vs), -60.0f), 60.0f);
+            // the largest and the smallest power of two among the rows' steps
+            const int e = min(max(static_cast<int>((__float_as_uint(vs) >> 23) & 255) - 127, -60), 60);
+            const int big = __reduce_max_sync(0xffffffffu, vs > 0.0f ? e : -1000);
+            const int small = __reduce_min_sync(0xffffffffu, vs > 0.0f ? e : 1000);
+            if (lane == 0) {
+              int* range = reinterpret_cast<int*>(smem + L::OFF_STEPS + (n % L::STEPS) * L::STEP_BYTES + 1536);
+              range[warp] = big;
+              range[4 + warp] = small;
+            }
+          }
+          if (tail) {
+#pragma unroll
+            for (int i = 0; i < PER; ++i)
+              if (half * 64 + row0 + i * (128 / CPR) >= left) w[i] = make_uint4(0, 0, 0, 0);
+          }
+          __syncwarp();
+          if (lane == 0) mbar_arrive(raw_empty(slot));
+#pragma unroll
+          for (int i = 0; i < PER; ++i) {
+            const int r = half * 64 + row0 + i * (128 / CPR);
+            const uint32_t x[4] = {w[i].x, w[i].y, w[i].z, w[i].w};
+            uint32_t y[8];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              y[2 * e] = ta_widen<FMT>(x[e]);
+              y[2 * e + 1] = ta_widen<FMT>(x[e] >> 16);
+            }
+            if (FMT == TA_FP8 && v && tail) {
+              bool any = false;
+#pragma unroll
+              for (int e = 0; e < 8; ++e) any |= tc_clean<false>(y[e]);
+              if (any) *s_odd = 1;
+            }
+            const int c = 2 * col;  // 16-byte chunk of the widened row
+            const uint32_t line = to + (v ? ((r >> 6) * L::DB + (c >> 3)) * 8192 + (r & 63) * 128 : (c >> 3) * 16384 + r * 128);
+            tc_sts128(line + (((c & 7) ^ (r & 7)) << 4), y[0], y[1], y[2], y[3]);
+            tc_sts128(line + ((((c + 1) & 7) ^ (r & 7)) << 4), y[4], y[5], y[6], y[7]);
+          }
         }
+        if (!ok) break;
+        fence_proxy_async_smem();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(v ? v_full(n % VST) : k_full(n % KST));
       }
-    };
-    auto advance = [&](Cursor& c) {
-      if (c.v) {
-        ++c.vc;
-        c.v = false;
-      } else {
-        ++c.kc;
-        c.v = true;
-        ++c.i;
+    } else if (tma) {
+      // V tiles with drafts or the sequence's end: rows beyond the end hold whatever the page
+      // does, and a hidden key's NaN or infinity would reach a row through 0 * value.  Both
+      // are zeroed; the softmax warps give visible ones back.
+      constexpr int CPR = D / 8;
+      const int col = tid % CPR;
+      uint32_t vn = 0, landed = 0;  // bit s: parity of stage s's next landing
+      bool ok = true;
+      TaPart part;
+      while (ok && walk.next(p, per_seq, TC_BN, part)) {
+        for (int j = max(0, part.ctx / TC_BN - part.t0); j < part.n && ok; ++j) {
+          const uint32_t n = vn + j;
+          // (a barrier of its own: these warps see only some of a stage's tiles)
+          ok = __all_sync(0xffffffffu, mbar_wait(v_land(n % VST), (landed >> (n % VST)) & 1u, budget, s_abort));
+          if (!ok) break;
+          landed ^= 1u << (n % VST);
+          const int left = part.ctx + part.drafts - (part.t0 + j) * TC_BN;
+#pragma unroll 1
+          for (int r = tid / CPR; r < TC_BN; r += 128 / CPR) {
+            const uint32_t a = sV0 + (n % VST) * L::TILE + ((r >> 6) * L::DB + (col >> 3)) * 8192 + (r & 63) * 128 + (((col & 7) ^ (r & 7)) << 4);
+            if (r >= left) {
+              tc_sts128(a, 0, 0, 0, 0);
+              continue;
+            }
+            uint4 x = ta_lds128(a);
+            if (tc_clean<BF>(x.x) | tc_clean<BF>(x.y) | tc_clean<BF>(x.z) | tc_clean<BF>(x.w)) {
+              tc_sts128(a, x.x, x.y, x.z, x.w);
+              *s_odd = 1;
+            }
+          }
+          fence_proxy_async_smem();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(v_full(n % VST));
+        }
+        vn += part.n;
       }
-      settle(c);
-    };
-    // Number (as K tile) of the V tile at the cursor: i - LEAD of the min(i, n) issued here.
-    auto k_number = [&](const Cursor& c) { return c.kc - static_cast<uint32_t>(min(c.i, c.part.n) - (c.i - LEAD)); };
-    // Row numbers of K tile `c`, for its copies and those of its V tile later.  The barrier
-    // also tells every producer whether one of them gave up, so that all stop together.
-    bool fail = false;
-    auto rows_of = [&](const Cursor& c) {
-      const int key = (c.part.t0 + c.i) * TC_BN + tid;
-      int row = -1;
-      if (key < c.part.ctx + c.part.drafts) {
-        const int pg = key / p.cache.page_size;
-        const int id = p.page_table[static_cast<int64_t>(c.part.b) * p.width + pg];
-        if (id >= 0 && id < p.cache.num_pages)
-          row = (id * p.cache.kv_heads + c.part.seg / p.row_tiles) * p.cache.page_size + (key - pg * p.cache.page_size);
-        else
-          index_error();
-      }
-      s_rows[(c.kc & 3) * 128 + tid] = row;
-      fail = named_bar_red_or(2, TC_PRODUCERS, fail);
-      return row;
-    };
-    Cursor in;
-    in.walk = walk;
-    in.i = 0;
-    in.v = true;
-    in.kc = in.vc = 0;
-    in.live = in.walk.next(p, per_seq, TC_BN, in.part);
-    settle(in);
-    if constexpr (!QUANT) {
+    } else {
+      const uint8_t* kbase = static_cast<const uint8_t*>(p.cache.k);
+      const uint8_t* vbase = static_cast<const uint8_t*>(p.cache.v);
+      volatile int32_t* s_rows = reinterpret_cast<volatile int32_t*>(smem + L::OFF_ROWS);
+      // Row numbers of the K tile at the cursor, for its copies and those of its V tile later.
+      // The barrier also tells every producer whether one gave up, so that all stop together.
+      bool fail = false;
+      auto rows_of = [&]() {
+        const int key = in.tile() * TC_BN + tid;
+        int row = -1;
+        if (key < in.part.ctx + in.part.drafts) {
+          const int pg = key / p.cache.page_size;
+          const int id = p.page_table[static_cast<int64_t>(in.part.b) * p.width + pg];
+          if (id >= 0 && id < p.cache.num_pages)
+            row = (id * p.cache.kv_heads + in.part.seg / p.row_tiles) * p.cache.page_size + (key - pg * p.cache.page_size);
+          else
+            index_error();
+        }
+        s_rows[(in.kc & 3) * 128 + tid] = row;
+        fail = named_bar_red_or(2, TC_PRODUCERS, fail);
+      };
       constexpr int CPR = D / 8;                     // 16-byte chunks per row
       constexpr int COPIES = TC_BN * CPR / TC_PRODUCERS;
       constexpr int LAG = KST + VST - 1;             // groups in flight before the oldest is handed over
@@ -386,11 +554,12 @@ __global__ void __launch_bounds__(TC_THREADS, 1) tree_attention_tc_kernel(const 
         for (int i = 0; i < LAG; ++i) q_item[i] = q_item[i + 1];
         --pending;
       };
-      while (in.live) {
+      in.begin(walk, LEAD);
+      while (in.next(p, per_seq)) {
         const bool v = in.v;
         const uint32_t n = v ? in.vc : in.kc;
         if (!v) {
-          rows_of(in);
+          rows_of();
           if (fail) break;
         }
         const uint32_t bar = v ? v_empty(n % VST) : k_empty(n % KST);
@@ -401,12 +570,9 @@ __global__ void __launch_bounds__(TC_THREADS, 1) tree_attention_tc_kernel(const 
           while (pending) hand_over();
           fail = !__all_sync(0xffffffffu, mbar_wait(bar, par, budget, s_abort));
         }
-        if (fail) {  // on to the next K tile's barrier
-          advance(in);
-          continue;
-        }
+        if (fail) continue;  // on to the next K tile's barrier
         const uint8_t* base = v ? vbase : kbase;
-        const uint32_t tile = v ? k_number(in) : n;
+        const uint32_t tile = v ? in.k_number() : n;
 #pragma unroll
         for (int i = 0; i < COPIES; ++i) {
           const int r = tid / CPR + i * (TC_PRODUCERS / CPR);
@@ -414,8 +580,7 @@ __global__ void __launch_bounds__(TC_THREADS, 1) tree_attention_tc_kernel(const 
           ta_copy16(where(v, n, r), base + (row < 0 ? 0 : static_cast<int64_t>(row) * (D * 2) + col * 16), row >= 0);
         }
         ta_commit();
-        const int at = v ? in.i - LEAD : in.i;
-        const bool tail = (in.part.t0 + at + 1) * TC_BN > in.part.ctx;
+        const bool tail = in.tail();
 #pragma unroll
         for (int i = 0; i <= LAG; ++i)
           if (i == pending) q_item[i] = (n << 2) | (tail ? 2u : 0u) | (v ? 1u : 0u);
@@ -423,166 +588,216 @@ __global__ void __launch_bounds__(TC_THREADS, 1) tree_attention_tc_kernel(const 
           ta_wait<LAG>();
           hand_over();
         }
-        advance(in);
       }
       ta_wait<0>();
       while (pending && !fail) hand_over();
-    } else {
-      // 8-bit rows: a thread copies 16-byte pieces into its own places of a ring of half
-      // tiles, and later widens the pieces it copied (so no exchange is needed).
-      constexpr int CPR = D / 16, PER = 64 * CPR / TC_PRODUCERS;  // pieces per row; per thread and half
-      constexpr int RING = L::HALVES;
-      const int col = tid % CPR, row0 = tid / CPR;
-      const uint32_t raw = sbase + L::OFF_RAW, rawstep = sbase + L::OFF_RAWSTEP;
-      Cursor out = in;
-      int in_half = 0;
-      uint32_t in_n = 0;
-      auto issue = [&]() {
-        if (in.live) {
-          int row = 0;
-          if (!in.v && in_half == 0) {
-            row = rows_of(in);
-            if (fail) in.live = false;
-            const uint32_t d = rawstep + (in.kc % L::RAWSTEP_RING) * 1024 + tid * 8;
-            ta_copy4(d, p.cache.k_scale + max(row, 0), row >= 0);
-            ta_copy4(d + 4, p.cache.v_scale + max(row, 0), row >= 0);
-          }
-          const uint32_t tile = in.v ? k_number(in) : in.kc;
-          const uint8_t* base = in.v ? vbase : kbase;
-          const uint32_t slot = raw + (in_n % RING) * L::HALF;
-#pragma unroll
-          for (int i = 0; i < PER; ++i) {
-            const int r = in_half * 64 + row0 + i * (TC_PRODUCERS / CPR);
-            const int rr = s_rows[(tile & 3) * 128 + r];
-            ta_copy16(slot + (i * TC_PRODUCERS + tid) * 16, base + (rr < 0 ? 0 : static_cast<int64_t>(rr) * D + col * 16), rr >= 0);
-          }
-          ++in_n;
-          if (in_half == 0) {
-            in_half = 1;
-          } else {
-            in_half = 0;
-            advance(in);
-          }
-        }
-        ta_commit();
-      };
-      for (int i = 0; i < RING; ++i) issue();
-      uint32_t out_n = 0;
-      while (out.live) {  // (after a failure: keeps step with the other producers' barriers)
-        const bool v = out.v;
-        const uint32_t n = v ? out.vc : out.kc;
-        const int at = v ? out.i - LEAD : out.i;
-        const bool tail = (out.part.t0 + at + 1) * TC_BN > out.part.ctx;
-        if (!fail) fail = !__all_sync(0xffffffffu, mbar_wait(v ? v_empty(n % VST) : k_empty(n % KST), ((n / (v ? VST : KST)) & 1u) ^ 1u, budget, s_abort));
-#pragma unroll 1
-        for (int half = 0; half < 2; ++half) {
-          ta_wait<RING - 1>();
-          if (fail) {
-            ++out_n;
-            issue();
-            continue;
-          }
-          const uint32_t slot = raw + (out_n % RING) * L::HALF;
-          uint4 w[PER];
-#pragma unroll
-          for (int i = 0; i < PER; ++i) w[i] = ta_lds128(slot + (i * TC_PRODUCERS + tid) * 16);
-          if (!v && half == 0) {  // the row's steps, and the values' offset of the reference
-            const uint32_t d = rawstep + (n % L::RAWSTEP_RING) * 1024 + tid * 8;
-            const float ks = ld_shared_f32(d), vs = ld_shared_f32(d + 4);
-            const uint32_t to = sbase + L::OFF_STEPS + (n % L::STEPS) * 1536 + tid * 4;
-            st_shared_f32(to, ks);
-            st_shared_f32(to + 512, vs);
-            st_shared_f32(to + 1024, fminf(fmaxf(__log2f(vs), -60.0f), 60.0f));
-          }
-#pragma unroll
-          for (int i = 0; i < PER; ++i) {
-            const int r = half * 64 + row0 + i * (TC_PRODUCERS / CPR);
-            const uint32_t x[4] = {w[i].x, w[i].y, w[i].z, w[i].w};
-            uint32_t y[8];
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-              y[2 * e] = ta_widen<FMT>(x[e]);
-              y[2 * e + 1] = ta_widen<FMT>(x[e] >> 16);
-            }
-            if (FMT == TA_FP8 && v && tail) {
-              bool any = false;
-#pragma unroll
-              for (int e = 0; e < 8; ++e) any |= tc_clean<false>(y[e]);
-              if (any) *s_odd = 1;
-            }
-            const int c = 2 * col;  // 16-byte chunk of the widened row
-            const uint32_t line = v ? sV0 + (n % VST) * L::TILE + ((r >> 6) * L::DB + (c >> 3)) * 8192 + (r & 63) * 128 : sK0 + (n % KST) * L::TILE + (c >> 3) * 16384 + r * 128;
-            tc_sts128(line + (((c & 7) ^ (r & 7)) << 4), y[0], y[1], y[2], y[3]);
-            tc_sts128(line + ((((c + 1) & 7) ^ (r & 7)) << 4), y[4], y[5], y[6], y[7]);
-          }
-          ++out_n;
-          issue();
-        }
-        fence_proxy_async_smem();
-        __syncwarp();
-        if (lane == 0 && !fail) mbar_arrive(v ? v_full(n % VST) : k_full(n % KST));
-        advance(out);
-      }
-      ta_wait<0>();
     }
   } else if (warp >= 12) {
     // ── MMA issuer (warps 13-15 only give up registers) ────────────────────────
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
     if (warp == 12 && lane == 0) {
       constexpr uint32_t IDESC_S = make_idesc(MFMT, 0, 0, TC_BN, TC_BN);
       constexpr uint32_t IDESC_PV = make_idesc(MFMT, 0, 1, TC_BN, D);
       uint32_t kn = 0, pn[2] = {0, 0}, parts = 0;
       bool ok = true;
+      TaWalk walk;
+      walk.begin(p, *s_share, TC_BN);
+      TaPart part;
       while (ok && walk.next(p, per_seq, TC_BN, part)) {
         const int steps = QT * part.n;
         ok = mbar_wait(q_full, parts & 1u, budget, s_abort);
         ++parts;
-        auto issue_s = [&](int i) {
+        // (from -2: the first scores of both units; S_t of step i + 2 lies over P_t of step i,
+        // and the MMAs run in order)
+        for (int i = -2; i < steps && ok; ++i) {
           const int t = i & 1;
-          const uint32_t j = kn + (QT == 1 ? i : i >> 1);
-          if ((QT == 1 || t == 0) && !mbar_wait(k_full(j % KST), (j / KST) & 1u, budget, s_abort)) return false;
-          tc_fence_after();
-          const uint32_t sK = sK0 + (j % KST) * L::TILE, sQt = sQ + (QT == 1 ? 0 : t) * L::TILE;
-#pragma unroll
-          for (int ks = 0; ks < D / 16; ++ks) {
-            const uint32_t off = (ks >> 2) * 16384 + (ks & 3) * 32;
-            mma_f16(tmem + t * TC_BN, make_sw128_desc(sQt + off, 16, 1024), make_sw128_desc(sK + off, 16, 1024), IDESC_S,
-                    ks > 0 ? 1u : 0u);
-          }
-          mma_commit(s_full(t));
-          if (QT == 1 || t == 1) mma_commit(k_empty(j % KST));
-          return true;
-        };
-        for (int i = 0; i < 2 && i < steps && ok; ++i) ok = issue_s(i);
-        for (int i = 0; i < steps && ok; ++i) {
-          const int t = i & 1;
-          const uint32_t j = kn + (QT == 1 ? i : i >> 1);
-          if ((QT == 1 || t == 0) && !(ok = mbar_wait(v_full(j % VST), (j / VST) & 1u, budget, s_abort))) break;
-          if (!(ok = mbar_wait(p_full(t), pn[t] & 1u, budget, s_abort))) break;
-          tc_fence_after();
-          const uint32_t sV = sV0 + (j % VST) * L::TILE;
-#pragma unroll
-          for (int lo = 0; lo < (BF ? 2 : 1); ++lo)
+          if (i >= 0) {
+            const uint32_t j = kn + (QT == 1 ? i : i >> 1);
+            if ((QT == 1 || t == 0) && !(ok = mbar_wait(v_full(j % VST), (j / VST) & 1u, budget, s_abort))) break;
+            if (!(ok = mbar_wait(p_full(t), pn[t] & 1u, budget, s_abort))) break;
+            tc_fence_after();
+            const uint64_t bd = make_sw128_desc(sV0 + (j % VST) * L::TILE, 8192, 1024);
+            const uint32_t dO = tmem + 2 * TC_BN + t * D, aP = tmem + t * TC_BN;
 #pragma unroll
             for (int ks = 0; ks < TC_BN / 16; ++ks) {
-              const uint64_t bd = make_sw128_desc(sV + (ks >> 2) * (L::DB * 8192) + (ks & 3) * 2048, 8192, 1024);
-              mma_f16_ts(tmem + 2 * TC_BN + t * D, tmem + t * TC_BN + lo * 64 + ks * 8, bd, IDESC_PV,
-                         (i > 1 || ks > 0 || lo > 0) ? 1u : 0u);
+              const uint64_t b = bd + (((ks >> 2) * (L::DB * 8192) + (ks & 3) * 2048) >> 4);
+              mma_f16_ts(dO, aP + (ks >> 1) * 32 + (ks & 1) * 8, b, IDESC_PV, (i > 1 || ks > 0) ? 1u : 0u);
+              if constexpr (BF) mma_f16_ts(dO, aP + (ks >> 1) * 32 + (ks & 1) * 8 + 16, b, IDESC_PV, 1u);
             }
-          ++pn[t];
-          if (QT == 1 || t == 1) mma_commit(v_empty(j % VST));
-          if (i + 2 < steps) ok = issue_s(i + 2);  // (over P_t: the MMAs run in order)
-          else mma_commit(pv_done(t));
+            ++pn[t];
+            if (QT == 1 || t == 1) mma_commit(v_empty(j % VST));
+            if (i + 2 >= steps) mma_commit(pv_done(t));
+          }
+          if (i + 2 < steps) {
+            const uint32_t j = kn + (QT == 1 ? i + 2 : (i + 2) >> 1);
+            if ((QT == 1 || t == 0) && !(ok = mbar_wait(k_full(j % KST), (j / KST) & 1u, budget, s_abort))) break;
+            tc_fence_after();
+            const uint64_t ad = make_sw128_desc(sQ + (QT == 1 ? 0 : t) * L::TILE, 16, 1024);
+            const uint64_t bd = make_sw128_desc(sK0 + (j % KST) * L::TILE, 16, 1024);
+#pragma unroll
+            for (int ks = 0; ks < D / 16; ++ks) {
+              const uint32_t off = ((ks >> 2) * 16384 + (ks & 3) * 32) >> 4;
+              mma_f16(tmem + t * TC_BN, ad + off, bd + off, IDESC_S, ks > 0 ? 1u : 0u);
+            }
+            mma_commit(s_full(t));
+            if (QT == 1 || t == 1) mma_commit(k_empty(j % KST));
+          }
         }
         kn += part.n;
       }
       mma_commit(done_bar);  // every MMA must complete before TMEM is released
       mbar_wait_drain(done_bar, 0, budget);
+    } else if (warp == 13 && (QUANT || tma)) {
+      // ── loader ─────────────────────────────────────────────────────────
+      TcCursor c;
+      {
+        TaWalk walk;
+        walk.begin(p, *s_share, TC_BN);
+        c.begin(walk, LEAD);
+      }
+      bool ok = true;
+      if constexpr (!QUANT) {
+        // One box a lane: box_rows rows of one page x 64 columns.  Rows past the end start
+        // outside the tensor and read as zeros.
+        const int R = p.box_rows, ko = (lane / L::DB) * R, db = lane % L::DB;
+        const bool on = lane < TC_BN / R * L::DB;
+        const int rows_all = static_cast<int>(p.cache.num_pages) * p.cache.kv_heads * p.cache.page_size;
+        auto row_of = [&]() {
+          const int key = c.tile() * TC_BN + ko;
+          if (!on || key >= c.part.ctx + c.part.drafts) return rows_all;
+          const int pg = key / p.cache.page_size;
+          const int id = p.page_table[static_cast<int64_t>(c.part.b) * p.width + pg];
+          if (id < 0 || id >= p.cache.num_pages) {
+            index_error();
+            return rows_all;
+          }
+          return (id * p.cache.kv_heads + c.part.seg / p.row_tiles) * p.cache.page_size + (key - pg * p.cache.page_size);
+        };
+        uint32_t used = 0, parity = 0;  // bit s: K stage s, 8 + s: V stage s, 16 + s: its landings
+        bool have = false, more = true, v = false, tail = false;  // an item looked up before; another one after it
+        uint32_t n = 0;
+        int row = 0;
+        while (true) {
+          const bool v0 = v, tail0 = tail;
+          const uint32_t n0 = n;
+          const int row0 = row;
+          if (more && (more = c.next(p, per_seq))) {
+            v = c.v;
+            n = c.number();
+            tail = c.tail();
+            row = row_of();
+          }
+          if (!have) {
+            have = more;
+            if (!more) break;
+            continue;
+          }
+          have = more;
+          const uint32_t st = n0 % (v0 ? VST : KST), ph = (n0 / (v0 ? VST : KST)) & 1u;
+          ok = __all_sync(0xffffffffu, mbar_wait(v0 ? v_empty(st) : k_empty(st), ph ^ 1u, budget, s_abort));
+          if (!ok) break;
+          const uint32_t full = !v0 ? k_full(st) : tail0 ? v_land(st) : v_full(st);
+          if (lane == 0) mbar_arrive_expect_tx(full, L::TILE);
+          if (v0 && !tail0 && lane >= 1 && lane < 4) mbar_arrive(full);  // (v_full counts four, the cleaning warps)
+          __syncwarp();
+          if (on) {
+            const uint32_t dst = v0 ? sV0 + st * L::TILE + ((ko >> 6) * L::DB + db) * 8192 + (ko & 63) * 128
+                                    : sK0 + st * L::TILE + db * 16384 + ko * 128;
+            tma_load_2d(dst, v0 ? &tmV : &tmK, full, db * 64, row0);
+          }
+          if (v0 && tail0) {  // phases of v_land count its own uses
+            used = (used | 1u << (16 + st)) & ~(1u << (8 + st));  // (the stage's last load counts)
+            parity ^= 1u << (16 + st);
+          } else {
+            used |= 1u << (v0 ? 8 + st : st);
+            if (v0) used &= ~(1u << (16 + st));
+            parity = (parity & ~(1u << (v0 ? 8 + st : st))) | (ph << (v0 ? 8 + st : st));
+          }
+          if (!have) break;
+        }
+        __syncwarp();
+        for (int s = 0; s < 4; ++s) {  // let every copy land before the CTA may exit
+          if ((used >> s) & 1) mbar_wait_drain(k_full(s), (parity >> s) & 1, budget);
+          if ((used >> (8 + s)) & 1) mbar_wait_drain(v_full(s), (parity >> (8 + s)) & 1, budget);
+          if ((used >> (16 + s)) & 1) mbar_wait_drain(v_land(s), ((parity >> (16 + s)) & 1) ^ 1, budget);
+        }
+      } else {
+        // Half tiles of 64 rows; a lane copies the run of a page that starts at its row, if
+        // one does, for rows lane and lane + 32.
+        uint32_t half_n = 0, used = 0, parity = 0;
+        int half = 1;  // of the item looked up last
+        bool have = false, more = true;
+        int row_a = 0, len_a = 0, own_a = -1, row_b = 0, len_b = 0, own_b = -1;
+        // first row and rows of the copy that starts at row r of the half; the key's own row
+        auto run_of = [&](int r, int& row, int& len, int& own) {
+          row = len = 0;
+          own = -1;
+          const int key = c.tile() * TC_BN + half * 64 + r, hi = c.part.ctx + c.part.drafts;
+          if (key >= hi) return;
+          const int ps = p.cache.page_size, pg = key / ps, at = key - pg * ps;
+          const int id = p.page_table[static_cast<int64_t>(c.part.b) * p.width + pg];
+          if (id < 0 || id >= p.cache.num_pages) {
+            index_error();
+            return;
+          }
+          own = row = (id * p.cache.kv_heads + c.part.seg / p.row_tiles) * ps + at;
+          if (r == 0 || at == 0) len = min(min(ps - at, 64 - r), hi - key);
+        };
+        bool v = false;
+        uint32_t n = 0;
+        while (true) {
+          const bool v0 = v;
+          const uint32_t n0 = n;
+          const int h = half, ra = row_a, la = len_a, oa = own_a, rb = row_b, lb = len_b, ob = own_b;
+          half ^= 1;
+          if (half == 0 && more) more = c.next(p, per_seq);
+          if (more) {
+            v = c.v;
+            n = c.number();
+            run_of(lane, row_a, len_a, own_a);
+            run_of(lane + 32, row_b, len_b, own_b);
+          }
+          if (!have) {
+            have = more;
+            if (!more) break;
+            continue;
+          }
+          have = more;
+          const int slot = half_n % L::HALVES;
+          const uint32_t ph = (half_n / L::HALVES) & 1u;
+          ok = __all_sync(0xffffffffu, mbar_wait(raw_empty(slot), ph ^ 1u, budget, s_abort));
+          if (!ok) break;
+          const uint32_t full = raw_full(slot), dst = sbase + L::OFF_RAW + slot * L::HALF;
+          const uint32_t bytes = __reduce_add_sync(0xffffffffu, (la + lb) * D);
+          if (lane == 0) mbar_arrive_expect_tx(full, bytes);
+          __syncwarp();
+          const uint8_t* base = static_cast<const uint8_t*>(v0 ? p.cache.v : p.cache.k);
+          if (la) bulk_load_g2s(dst + lane * D, base + static_cast<int64_t>(ra) * D, la * D, full);
+          if (lb) bulk_load_g2s(dst + (lane + 32) * D, base + static_cast<int64_t>(rb) * D, lb * D, full);
+          if (!v0) {
+            const uint32_t d = sbase + L::OFF_RAWSTEP + (n0 & 3) * 1024 + (h * 64 + lane) * 8;
+            ta_copy4(d, p.cache.k_scale + max(oa, 0), oa >= 0);
+            ta_copy4(d + 4, p.cache.v_scale + max(oa, 0), oa >= 0);
+            ta_copy4(d + 256, p.cache.k_scale + max(ob, 0), ob >= 0);
+            ta_copy4(d + 260, p.cache.v_scale + max(ob, 0), ob >= 0);
+            tc_copies_arrive(full);
+          } else {
+            mbar_arrive(full);
+          }
+          used |= 1u << slot;
+          parity = (parity & ~(1u << slot)) | (ph << slot);
+          ++half_n;
+          if (!have) break;
+        }
+        __syncwarp();
+        for (int s = 0; s < L::HALVES; ++s)
+          if ((used >> s) & 1) mbar_wait_drain(raw_full(s), (parity >> s) & 1, budget);
+      }
     }
     __syncwarp();
   } else {
     // ── softmax ──────────────────────────────────────────────────────────
-    asm volatile("setmaxnreg.inc.sync.aligned.u32 184;");
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 160;");
     const int t = (warp - 4) >> 2;
     const int quarter = warp & 3;
     const int lrow = quarter * 32 + lane;
@@ -590,6 +805,9 @@ __global__ void __launch_bounds__(TC_THREADS, 1) tree_attention_tc_kernel(const 
     float2* s_ml = reinterpret_cast<float2*>(smem);  // [2][128], in Q's place between parts
     uint32_t steps_done = 0, tile_no = 0, ended = 0;  // this unit's steps, all key tiles, parts with a step, before the part
     bool ok = true;
+    TaWalk walk;
+    walk.begin(p, *s_share, TC_BN);
+    TaPart part;
     while (walk.next(p, per_seq, TC_BN, part)) {
       const int kvh = part.seg / p.row_tiles, rt = part.seg % p.row_tiles;
       const int gr = rt * QT * TC_BN + (QT == 1 ? 0 : t * TC_BN) + lrow;
@@ -670,85 +888,113 @@ __global__ void __launch_bounds__(TC_THREADS, 1) tree_attention_tc_kernel(const 
           if (lane == 0) mbar_arrive(p_full(t));
           continue;
         }
-        uint32_t r[TC_BN];
-#pragma unroll
-        for (int c = 0; c < TC_BN; c += 16) tmem_ld16(trow + t * TC_BN + c, *reinterpret_cast<uint32_t(*)[16]>(&r[c]));
-        tmem_wait_ld();
         const int k0 = (part.t0 + j) * TC_BN;
-        const bool all = k0 + TC_BN <= part.ctx;
-        uint32_t see[4] = {0xffffffffu, 0xffffffffu, 0xffffffffu, 0xffffffffu};
-        if (!all) {
+        if (k0 + TC_BN > part.ctx) {  // drafts, or the end: what the row does not see scores -inf
+#pragma unroll 1
+          for (int c = 0; c < TC_BN; c += 16) {
+            const uint32_t see = ta_visible(p, part.b, token, k0 + c, part.ctx, hi);
+            uint32_t w[16];
+            tmem_ld16(trow + t * TC_BN + c, w);
+            tmem_wait_ld();
 #pragma unroll
-          for (int w = 0; w < 4; ++w) see[w] = ta_visible(p, part.b, token, k0 + 32 * w, part.ctx, hi);
-        }
-        const uint32_t steps = sbase + L::OFF_STEPS + ((tile_no + j) % (L::STEPS ? L::STEPS : 1)) * 1536;
-        float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-#pragma unroll
-        for (int c = 0; c < TC_BN; c += 4) {
-          float4 ks = make_float4(1, 1, 1, 1), lv = make_float4(0, 0, 0, 0);
-          if (QUANT) {
-            ks = tc_lds4f(steps + c * 4);
-            lv = tc_lds4f(steps + 1024 + c * 4);
+            for (int e = 0; e < 16; ++e) w[e] = (see >> e) & 1 ? w[e] : 0xff800000u;
+            tmem_st16(trow + t * TC_BN + c, w);
           }
-          const float kk[4] = {ks.x, ks.y, ks.z, ks.w}, ll[4] = {lv.x, lv.y, lv.z, lv.w};
+          tmem_wait_st();
+        }
+        // Two passes over the scores in tensor memory, 64 columns an iteration: the loops stay
+        // small, for what bounds a fully unrolled row is the fetching of its instructions.
+        const ulonglong2* steps = reinterpret_cast<const ulonglong2*>(smem + L::OFF_STEPS + ((tile_no + j) % (L::STEPS ? L::STEPS : 1)) * L::STEP_BYTES);
+        // Value steps of one tile seldom differ by more than 2^8: then the largest stands for
+        // all (weights keep 2^-22 of the largest, f16's range), and no offset is read a key.
+        float above = 0.0f;
+        bool narrow = true;
+        if (QUANT) {
+          const int4 big = *reinterpret_cast<const int4*>(steps + 96), small = *reinterpret_cast<const int4*>(steps + 98);
+          const int hi_e = max(max(big.x, big.y), max(big.z, big.w)), lo_e = min(min(small.x, small.y), min(small.z, small.w));
+          narrow = hi_e - lo_e <= 8;
+          above = hi_e > -1000 ? static_cast<float>(hi_e + 1) : -60.0f;
+        }
+        const uint32_t tS = trow + t * TC_BN;
+        const uint64_t rs2 = tc_pair(row_scale, row_scale);
+        float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll 1
+        for (int c0 = 0; c0 < TC_BN; c0 += 64) {
+          uint32_t r[64];
 #pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            float x = __uint_as_float(r[c + e]);
-            if (QUANT) {
-              x *= kk[e];
-              r[c + e] = __float_as_uint(x);
+          for (int c = 0; c < 64; c += 16) tmem_ld16(tS + c0 + c, *reinterpret_cast<uint32_t(*)[16]>(&r[c]));
+          tmem_wait_ld();
+          if (narrow) {
+#pragma unroll
+            for (int c = 0; c < 64; c += 4) {
+              float2 a = make_float2(__uint_as_float(r[c]), __uint_as_float(r[c + 1]));
+              float2 b = make_float2(__uint_as_float(r[c + 2]), __uint_as_float(r[c + 3]));
+              if (QUANT) {
+                const ulonglong2 ks = steps[(c0 + c) / 4];
+                a = tc_split(tc_mul2(tc_pair(a.x, a.y), ks.x));
+                b = tc_split(tc_mul2(tc_pair(b.x, b.y), ks.y));
+              }
+              mx[(c >> 2) & 3] = fmaxf(fmaxf(mx[(c >> 2) & 3], fmaxf(a.x, a.y)), fmaxf(b.x, b.y));
             }
-            const float y = QUANT ? fmaf(x, row_scale, ll[e]) : x;
-            if (all) mx[e] = fmaxf(mx[e], y);
-            else if ((see[(c + e) >> 5] >> ((c + e) & 31)) & 1) mx[e] = fmaxf(mx[e], y);
+          } else {
+#pragma unroll
+            for (int c = 0; c < 64; c += 4) {  // (into the units of `top` below)
+              const float4 ks = reinterpret_cast<const float4*>(steps)[(c0 + c) / 4], lv = reinterpret_cast<const float4*>(steps)[64 + (c0 + c) / 4];
+              mx[0] = fmaxf(mx[0], fmaf(__uint_as_float(r[c]) * ks.x, row_scale, lv.x));
+              mx[1] = fmaxf(mx[1], fmaf(__uint_as_float(r[c + 1]) * ks.y, row_scale, lv.y));
+              mx[2] = fmaxf(mx[2], fmaf(__uint_as_float(r[c + 2]) * ks.z, row_scale, lv.z));
+              mx[3] = fmaxf(mx[3], fmaf(__uint_as_float(r[c + 3]) * ks.w, row_scale, lv.w));
+            }
           }
         }
         float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
-        if (!QUANT) top *= row_scale;  // positive: the largest stays the largest
+        if (narrow) top = fmaf(top, row_scale, above);  // (row_scale is positive: the largest stays the largest)
         const bool raise = valid && top > m_run + 8.0f;
         const float m_new = raise ? top : m_run;
         const float m_use = m_new == -INFINITY ? 0.0f : m_new;
         const float alpha = raise ? ta_exp2(m_run - m_use) : 1.0f;
-        float sum[4] = {0, 0, 0, 0};
+        const uint64_t neg2 = tc_pair(-m_use, -m_use);
+        uint64_t sum2[2] = {0, 0};
         // (S_t in tensor memory means that the unit's last product is complete, O_t with it)
+#pragma unroll 1
+        for (int c0 = 0; c0 < TC_BN; c0 += 64) {
+          uint32_t r[64];
 #pragma unroll
-        for (int c = 0; c < TC_BN / 8; ++c) {
-          float vs[8];
-          if (QUANT) {
-            const float4 a = tc_lds4f(steps + 512 + c * 32), b4 = tc_lds4f(steps + 512 + c * 32 + 16);
-            vs[0] = a.x, vs[1] = a.y, vs[2] = a.z, vs[3] = a.w, vs[4] = b4.x, vs[5] = b4.y, vs[6] = b4.z, vs[7] = b4.w;
-          }
+          for (int c = 0; c < 64; c += 16) tmem_ld16(tS + c0 + c, *reinterpret_cast<uint32_t(*)[16]>(&r[c]));
+          tmem_wait_ld();
+          // keys 32 k .. of the tile become columns 32 k .. 32 k + 15 (+ 16: their next bits)
 #pragma unroll
-          for (int i = 0; i < 8; i += 2) {
-            const int kk = 8 * c + i;
-            float e0 = ta_exp2(fmaf(__uint_as_float(r[kk]), row_scale, -m_use));
-            float e1 = ta_exp2(fmaf(__uint_as_float(r[kk + 1]), row_scale, -m_use));
-            if (!all) {
-              e0 = (see[kk >> 5] >> (kk & 31)) & 1 ? e0 : 0.0f;
-              e1 = (see[kk >> 5] >> ((kk + 1) & 31)) & 1 ? e1 : 0.0f;
+          for (int c = 0; c < 64; c += 32) {
+            uint32_t hi_w[16], lo_w[BF ? 16 : 1];
+#pragma unroll
+            for (int e = 0; e < 32; e += 4) {
+              ulonglong2 ks = make_ulonglong2(0, 0), vs = ks;
+              if (QUANT) {
+                ks = steps[(c0 + c + e) / 4];
+                vs = steps[32 + (c0 + c + e) / 4];
+              }
+#pragma unroll
+              for (int h = 0; h < 2; ++h) {
+                uint64_t x = tc_pair(__uint_as_float(r[c + e + 2 * h]), __uint_as_float(r[c + e + 2 * h + 1]));
+                if (QUANT) x = tc_mul2(x, h ? ks.y : ks.x);
+                const float2 a = tc_split(tc_fma2(x, rs2, neg2));
+                uint64_t w2 = tc_pair(ta_exp2(a.x), ta_exp2(a.y));
+                sum2[h] = tc_add2(sum2[h], w2);
+                if (QUANT) w2 = tc_mul2(w2, h ? vs.y : vs.x);
+                const float2 w = tc_split(w2);
+                const uint32_t pk = ta_pack(w.x, w.y, BF);
+                hi_w[e / 2 + h] = pk;
+                if (BF) lo_w[e / 2 + h] = ta_pack(w.x - __uint_as_float(pk << 16), w.y - __uint_as_float(pk & 0xffff0000u), true);
+              }
             }
-            sum[(kk >> 1) & 3] += e0 + e1;
-            if (QUANT) {
-              // (hidden: 0, whatever the step)
-              e0 = !all && !((see[kk >> 5] >> (kk & 31)) & 1) ? 0.0f : e0 * vs[i];
-              e1 = !all && !((see[kk >> 5] >> ((kk + 1) & 31)) & 1) ? 0.0f : e1 * vs[i + 1];
-            }
-            // pairs replace the scores in place: r[k] the weights, r[k + 1] their next bits
-            const uint32_t w = ta_pack(e0, e1, BF);
-            r[kk] = w;
-            if (BF) r[kk + 1] = ta_pack(e0 - __uint_as_float(w << 16), e1 - __uint_as_float(w & 0xffff0000u), true);
+            tmem_st16(tS + c0 + c, hi_w);
+            if constexpr (BF) tmem_st16(tS + c0 + c + 16, lo_w);
           }
-          if (c % 4 == 3) {
-            uint32_t pk[16];
-#pragma unroll
-            for (int i = 0; i < 16; ++i) pk[i] = r[8 * (c - 3) + 2 * i];
-            tmem_st16(trow + t * TC_BN + (c - 3) * 4, pk);
-            if (BF) {
-#pragma unroll
-              for (int i = 0; i < 16; ++i) pk[i] = r[8 * (c - 3) + 2 * i + 1];
-              tmem_st16(trow + t * TC_BN + 64 + (c - 3) * 4, pk);
-            }
-          }
+        }
+        float sum[4];
+        {
+          const float2 a = tc_split(sum2[0]), b = tc_split(sum2[1]);
+          sum[0] = a.x, sum[1] = a.y, sum[2] = b.x, sum[3] = b.y;
         }
         l_run = l_run * alpha + ((sum[0] + sum[1]) + (sum[2] + sum[3]));
         m_run = m_new;
@@ -818,13 +1064,19 @@ __global__ void __launch_bounds__(TC_THREADS, 1) tree_attention_tc_kernel(const 
             }
           }
           if (odd && valid) {  // give the non-finite values to the rows that see them
-            const int from = max(part.ctx, part.t0 * TC_BN), to = min(hi, (part.t0 + part.n) * TC_BN);
+            const int from = max(part.ctx / TC_BN, part.t0) * TC_BN, to = min(hi, (part.t0 + part.n) * TC_BN);
             for (int key = from; key < to; ++key) {
               if (!(ta_visible(p, part.b, token, key, part.ctx, hi) & 1)) continue;
               const int pg = key / p.cache.page_size;
               const int id = p.page_table[static_cast<int64_t>(part.b) * p.width + pg];
               if (id < 0 || id >= p.cache.num_pages) continue;
-              const int64_t at = ((static_cast<int64_t>(id) * p.cache.kv_heads + kvh) * p.cache.page_size + key % p.cache.page_size) * D + c;
+              const int64_t row = (static_cast<int64_t>(id) * p.cache.kv_heads + kvh) * p.cache.page_size + key % p.cache.page_size;
+              const int64_t at = row * D + c;
+              if (QUANT) {
+                const float k0 = p.cache.k_scale[row] * 0.0f, v0 = p.cache.v_scale[row] * 0.0f;  // 0, or NaN
+#pragma unroll
+                for (int e = 0; e < 16; ++e) acc[e] += k0 + v0;
+              }
               for (int i = 0; i < 16; ++i) {
                 float v;
                 if (QUANT) v = dequantise_one(static_cast<const uint8_t*>(p.cache.v)[at + i], 1.0f, p.cache.format);
@@ -884,7 +1136,8 @@ __global__ void __launch_bounds__(TC_THREADS, 1) tree_attention_tc_kernel(const 
 }
 
 // Joins the parts of segments that more than one CTA took, and writes the zeros of
-// sequences without keys.  One warp per row.
+// sequences without keys.  One warp per row; the parts' factors sit in the lanes, so the
+// loads of a pass over 32 parts do not wait for one another.
 template <int D>
 __global__ void __launch_bounds__(128) tree_attention_parts_kernel(const TaParams p, int tile_rows, int unit, int ctas) {
   const int lane = threadIdx.x & 31;
@@ -916,26 +1169,33 @@ __global__ void __launch_bounds__(128) tree_attention_parts_kernel(const TaParam
   auto owner = [&](long long u) { return static_cast<int>(((u + 1) * ctas - 1) / total); };
   const int c0 = owner(u0), c1 = owner(u0 + tiles - 1);
   if (c0 == c1) return;  // written by its CTA
+  const bool first0 = total * c0 / ctas == u0;
   auto slot_of = [&](int c) {
-    const int which = c > c0 || total * c / ctas == u0 ? 0 : 1;
-    return (static_cast<int64_t>(c) * 2 + which) * tile_rows + r % tile_rows;
+    return (static_cast<int64_t>(c) * 2 + (c > c0 || first0 ? 0 : 1)) * tile_rows + r % tile_rows;
   };
-  float top = -INFINITY;
-  for (int c = c0 + lane; c <= c1; c += 32)
-    if (total * c / ctas < total * (c + 1) / ctas) top = fmaxf(top, p.part_ml[slot_of(c)].x);
-  for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-  float acc[D / 32], l = 0.0f;
+  float ref = -INFINITY, acc[D / 32], l = 0.0f;
 #pragma unroll
   for (int i = 0; i < D / 32; ++i) acc[i] = 0.0f;
-  for (int c = c0; c <= c1; ++c) {
-    if (total * c / ctas >= total * (c + 1) / ctas) continue;  // a CTA without tiles
-    const int64_t slot = slot_of(c);
-    const float2 ml = p.part_ml[slot];
-    const float f = ta_share(ml.x, ml.y, top);
-    if (f != 0.0f) {
-      l += f * ml.y;
+  for (int c = c0; c <= c1; c += 32) {
+    const int mine = c + lane;
+    float2 ml = make_float2(-INFINITY, 0.0f);
+    if (mine <= c1 && total * mine / ctas < total * (mine + 1) / ctas) ml = p.part_ml[slot_of(mine)];  // (or no tiles)
+    float top = fmaxf(ref, ml.x);
+    for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+    const float keep = ta_share(ref, l, top), f = ta_share(ml.x, ml.y, top);
+    float part = f != 0.0f ? f * ml.y : 0.0f;
+    for (int o = 16; o > 0; o >>= 1) part += __shfl_xor_sync(0xffffffffu, part, o);
+    l = (keep != 0.0f ? l * keep : 0.0f) + part;
 #pragma unroll
-      for (int i = 0; i < D / 32; ++i) acc[i] += f * p.part_o[slot * D + lane + 32 * i];
+    for (int i = 0; i < D / 32; ++i) acc[i] = keep != 0.0f ? acc[i] * keep : 0.0f;
+    ref = top;
+    const int n = min(32, c1 - c + 1);
+#pragma unroll 8
+    for (int k = 0; k < n; ++k) {
+      const float g = __shfl_sync(0xffffffffu, f, k);
+      const float* o = p.part_o + slot_of(c + k) * D + lane;
+#pragma unroll
+      for (int i = 0; i < D / 32; ++i) acc[i] += g != 0.0f ? g * o[32 * i] : 0.0f;
     }
   }
 #pragma unroll
