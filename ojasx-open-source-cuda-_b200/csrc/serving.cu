@@ -423,6 +423,9 @@ int ojx_tree_attention(const ojx_tree_attention_desc* d, ojx_stream stream) {
   p.mask_sb = d->mask_stride_b;
   p.words = (d->tokens + 63) / 64;
   p.scale_log2 = d->scale * 1.4426950408889634f;
+  p.page_shift = -1;
+  for (int i = 0; i < 31; ++i)
+    if (c.page_size == 1 << i) p.page_shift = i;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   if (c.format == OJX_KV_F16) return launch_tree_fmt<TA_F16>(p, s);
   if (c.format == OJX_KV_BF16) return launch_tree_fmt<TA_BF16>(p, s);

@@ -32,6 +32,7 @@ struct TaParams {
   int words;
   float scale_log2;
   int row_tiles, splits;
+  int page_shift;  // log2 of the page size, or -1
   int box_rows;    // rows of a TMA box (16-bit caches on tcgen05), 0: no TMA
   float* part_o;   // [segment][split][rows][D], unnormalised
   float2* part_ml;  // [segment][split][rows]: reference, sum

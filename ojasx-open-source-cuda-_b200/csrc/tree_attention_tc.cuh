@@ -44,18 +44,18 @@ struct TcLayout {
   static constexpr int SLACK = 256;                     // to round the base up (it is aligned already, see the kernel)
   static constexpr int FIT = (227 * 1024 - BARS - SLACK - 2048 - QT * TILE) / TILE;  // tile buffers
   static constexpr int KST = QUANT ? 2 : D == 64 ? 4 : 3;
-  static constexpr int VST = QUANT ? 2 : D == 64 ? 4 : FIT - 3;
+  static constexpr int VST = QUANT ? (D == 128 && QT == 2 ? 1 : 2) : D == 64 ? 4 : FIT - 3;
   static_assert(QUANT || KST + VST <= FIT, "shared memory");
-  static constexpr int HALF = 64 * D;                   // half a tile of 8-bit rows
-  static constexpr int HALVES = !QUANT ? 0 : D == 64 ? 12 : QT == 1 ? 6 : 3;  // ring of them
+  static constexpr int RAW = TC_BN * D;                 // a tile of 8-bit rows
+  static constexpr int RAWS = !QUANT ? 0 : D == 64 ? 6 : 3;  // ring of them
   static constexpr int STEPS = !QUANT ? 0 : (QT == 1 ? 3 : 2) + KST;  // tiles whose steps are kept
   static constexpr int STEP_BYTES = 1568;
   static constexpr int RAWSTEP_RING = QUANT ? 4 : 0;
   static constexpr int OFF_K = QT * TILE;
   static constexpr int OFF_V = OFF_K + KST * TILE;
   static constexpr int OFF_RAW = OFF_V + VST * TILE;
-  static constexpr int OFF_ROWS = OFF_RAW + HALVES * HALF;        // 4 x 128 row numbers
-  static constexpr int OFF_STEPS = OFF_ROWS + (QUANT ? 0 : 4 * 512);            // [STEPS][3][128] floats, [2][4] ints
+  static constexpr int OFF_ROWS = OFF_RAW + RAWS * RAW;             // 4 x 128 row numbers (8 bits: and lengths)
+  static constexpr int OFF_STEPS = OFF_ROWS + (QUANT ? 2 : 1) * 4 * 512;            // [STEPS][3][128] floats, [2][4] ints
   static constexpr int OFF_RAWSTEP = OFF_STEPS + STEPS * STEP_BYTES;
   static constexpr int OFF_BAR = OFF_RAWSTEP + RAWSTEP_RING * 1024;
   static constexpr int SMEM = OFF_BAR + BARS + SLACK;
@@ -134,6 +134,7 @@ __device__ __forceinline__ TaShare ta_share_of(const TaParams& p, int per_seq, i
 // One segment's part of a CTA's share.
 struct TaPart {
   int b, seg, t0, n, tiles;  // sequence, segment in it, first tile, tiles here, tiles in all
+  int kvh;                   // the segment's key head
   int ctx, drafts;
   bool first;                // first part of this CTA
 };
@@ -163,6 +164,7 @@ struct TaWalk {
     o.b = s.b;
     o.seg = at / tiles;
     o.t0 = at - o.seg * tiles;
+    o.kvh = o.seg / p.row_tiles;
     o.tiles = tiles;
     o.n = min(tiles - o.t0, s.end - s.u);
     o.ctx = ctx;
@@ -335,7 +337,7 @@ __global__ void __launch_bounds__(TC_THREADS, 1) tree_attention_tc_kernel(const 
   uint32_t* s_tmem = reinterpret_cast<uint32_t*>(bars + 53);
   volatile int* s_odd = reinterpret_cast<volatile int*>(bars + 54);  // a hidden non-finite value was met
   TaShare* s_share = reinterpret_cast<TaShare*>(bars + 55);
-  static_assert(55 * 8 + sizeof(TaShare) <= L::BARS && KST <= 4 && VST <= 4 && L::HALVES <= 12, "barrier area");
+  static_assert(55 * 8 + sizeof(TaShare) <= L::BARS && KST <= 4 && VST <= 4 && L::RAWS <= 12, "barrier area");
   const bool tma = !QUANT && p.box_rows > 0;
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -354,7 +356,7 @@ __global__ void __launch_bounds__(TC_THREADS, 1) tree_attention_tc_kernel(const 
       mbar_init(v_empty(s), 1);
       mbar_init(v_land(s), 1);
     }
-    for (int s = 0; s < L::HALVES; ++s) {
+    for (int s = 0; s < L::RAWS; ++s) {
       mbar_init(raw_full(s), 33);
       mbar_init(raw_empty(s), 4);
     }
@@ -388,77 +390,83 @@ __global__ void __launch_bounds__(TC_THREADS, 1) tree_attention_tc_kernel(const 
     walk.begin(p, *s_share, TC_BN);
     TcCursor in;
     if constexpr (QUANT) {
-      constexpr int CPR = D / 16, PER = 64 * CPR / 128;  // 16-byte pieces per row; per thread and half
+      constexpr int CPR = D / 16, PER = TC_BN * CPR / 128;  // 16-byte pieces per row; per thread
       const int col = tid % CPR, row0 = tid / CPR;
-      uint32_t half_n = 0;
+      uint32_t raw_n = 0;
       bool ok = true;
       in.begin(walk, LEAD);
       while (ok && in.next(p, per_seq)) {
         const bool v = in.v, tail = in.tail();
         const uint32_t n = in.number();
         const int left = in.part.ctx + in.part.drafts - in.tile() * TC_BN;  // rows that exist
-        ok = __all_sync(0xffffffffu, mbar_wait(v ? v_empty(n % VST) : k_empty(n % KST), ((n / (v ? VST : KST)) & 1u) ^ 1u, budget, s_abort));
-        const uint32_t to = v ? sV0 + (n % VST) * L::TILE : sK0 + (n % KST) * L::TILE;
-#pragma unroll 1
-        for (int half = 0; half < 2 && ok; ++half, ++half_n) {
-          const int slot = half_n % L::HALVES;
-          ok = __all_sync(0xffffffffu, mbar_wait(raw_full(slot), (half_n / L::HALVES) & 1u, budget, s_abort));
-          if (!ok) break;
-          const uint4* raw = reinterpret_cast<const uint4*>(smem + L::OFF_RAW + slot * L::HALF) + tid;
-          uint4 w[PER];
+        const int slot = raw_n % L::RAWS;
+        ok = __all_sync(0xffffffffu, mbar_wait(raw_full(slot), (raw_n / L::RAWS) & 1u, budget, s_abort));
+        if (!ok) break;
+        ++raw_n;
+        const uint4* raw = reinterpret_cast<const uint4*>(smem + L::OFF_RAW + slot * L::RAW) + tid;
+        uint4 w[PER];
 #pragma unroll
-          for (int i = 0; i < PER; ++i) w[i] = raw[i * 128];
-          if (!v && (tid >> 6) == half) {  // the row's steps, and the values' offset of the reference
-            const float2 st = *reinterpret_cast<const float2*>(smem + L::OFF_RAWSTEP + (n & 3) * 1024 + tid * 8);
-            float ks = st.x, vs = st.y;
-            if (tail && !(fabsf(ks) < INFINITY && fabsf(vs) < INFINITY)) {
-              ks = vs = 0.0f;  // as for the values: kept from rows that do not see the key
-              *s_odd = 1;
-            }
-            float* d = reinterpret_cast<float*>(smem + L::OFF_STEPS + (n % L::STEPS) * L::STEP_BYTES) + tid;
-            d[0] = ks == 0.0f ? 1.17549435e-38f : ks;  // (a row of zeros: its products are zero, and a hidden score stays -inf)
-            d[128] = vs;
-            d[256] = fminf(fmaxf(__log2f(vs), -60.0f), 60.0f);
-            // the largest and the smallest power of two among the rows' steps
-            const int e = min(max(static_cast<int>((__float_as_uint(vs) >> 23) & 255) - 127, -60), 60);
-            const int big = __reduce_max_sync(0xffffffffu, vs > 0.0f ? e : -1000);
-            const int small = __reduce_min_sync(0xffffffffu, vs > 0.0f ? e : 1000);
-            if (lane == 0) {
-              int* range = reinterpret_cast<int*>(smem + L::OFF_STEPS + (n % L::STEPS) * L::STEP_BYTES + 1536);
-              range[warp] = big;
-              range[4 + warp] = small;
-            }
+        for (int i = 0; i < PER; ++i) w[i] = raw[i * 128];
+        if (!v) {  // the row's steps, and the values' offset of the reference
+          const float2 st = *reinterpret_cast<const float2*>(smem + L::OFF_RAWSTEP + (n & 3) * 1024 + tid * 8);
+          float ks = st.x, vs = st.y;
+          if (tail && !(fabsf(ks) < INFINITY && fabsf(vs) < INFINITY)) {
+            ks = vs = 0.0f;  // as for the values: kept from rows that do not see the key
+            *s_odd = 1;
           }
-          if (tail) {
-#pragma unroll
-            for (int i = 0; i < PER; ++i)
-              if (half * 64 + row0 + i * (128 / CPR) >= left) w[i] = make_uint4(0, 0, 0, 0);
-          }
-          __syncwarp();
-          if (lane == 0) mbar_arrive(raw_empty(slot));
-#pragma unroll
-          for (int i = 0; i < PER; ++i) {
-            const int r = half * 64 + row0 + i * (128 / CPR);
-            const uint32_t x[4] = {w[i].x, w[i].y, w[i].z, w[i].w};
-            uint32_t y[8];
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-              y[2 * e] = ta_widen<FMT>(x[e]);
-              y[2 * e + 1] = ta_widen<FMT>(x[e] >> 16);
-            }
-            if (FMT == TA_FP8 && v && tail) {
-              bool any = false;
-#pragma unroll
-              for (int e = 0; e < 8; ++e) any |= tc_clean<false>(y[e]);
-              if (any) *s_odd = 1;
-            }
-            const int c = 2 * col;  // 16-byte chunk of the widened row
-            const uint32_t line = to + (v ? ((r >> 6) * L::DB + (c >> 3)) * 8192 + (r & 63) * 128 : (c >> 3) * 16384 + r * 128);
-            tc_sts128(line + (((c & 7) ^ (r & 7)) << 4), y[0], y[1], y[2], y[3]);
-            tc_sts128(line + ((((c + 1) & 7) ^ (r & 7)) << 4), y[4], y[5], y[6], y[7]);
+          float* d = reinterpret_cast<float*>(smem + L::OFF_STEPS + (n % L::STEPS) * L::STEP_BYTES) + tid;
+          d[0] = ks == 0.0f ? 1.17549435e-38f : ks;  // (a row of zeros: its products are zero, and a hidden score stays -inf)
+          d[128] = vs;
+          d[256] = fminf(fmaxf(__log2f(vs), -60.0f), 60.0f);
+          // the largest and the smallest power of two among the rows' steps
+          const int e = min(max(static_cast<int>((__float_as_uint(vs) >> 23) & 255) - 127, -60), 60);
+          const int big = __reduce_max_sync(0xffffffffu, vs > 0.0f ? e : -1000);
+          const int small = __reduce_min_sync(0xffffffffu, vs > 0.0f ? e : 1000);
+          if (lane == 0) {
+            int* range = reinterpret_cast<int*>(smem + L::OFF_STEPS + (n % L::STEPS) * L::STEP_BYTES + 1536);
+            range[warp] = big;
+            range[4 + warp] = small;
           }
         }
+        if (tail) {
+#pragma unroll
+          for (int i = 0; i < PER; ++i)
+            if (row0 + i * (128 / CPR) >= left) w[i] = make_uint4(0, 0, 0, 0);
+        }
+        __syncwarp();
+        if (lane == 0) mbar_arrive(raw_empty(slot));
+        ok = __all_sync(0xffffffffu, mbar_wait(v ? v_empty(n % VST) : k_empty(n % KST), ((n / (v ? VST : KST)) & 1u) ^ 1u, budget, s_abort));
         if (!ok) break;
+        const uint32_t to = v ? sV0 + (n % VST) * L::TILE : sK0 + (n % KST) * L::TILE;
+        // A piece becomes two 16-byte chunks of the widened row; threads of the row's second
+        // 64 columns store theirs in the other order, so that eight of them meet no bank twice.
+        const int c = 2 * col, swap = c >> 3;
+        bool any = false;
+#pragma unroll
+        for (int i = 0; i < PER; ++i) {
+          const int r = row0 + i * (128 / CPR);
+          const uint32_t x[4] = {w[i].x, w[i].y, w[i].z, w[i].w};
+          uint32_t y[8];
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            y[2 * e] = ta_widen<FMT>(x[e]);
+            y[2 * e + 1] = ta_widen<FMT>(x[e] >> 16);
+          }
+          if (FMT == TA_FP8 && tail) {
+#pragma unroll
+            for (int e = 0; e < 8; ++e)
+              if (v) any |= tc_clean<false>(y[e]);
+          }
+          const uint32_t line = to + (v ? ((r >> 6) * L::DB + (c >> 3)) * 8192 + (r & 63) * 128 : (c >> 3) * 16384 + r * 128);
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            const int k = D == 128 ? h ^ swap : h;
+            const bool second = D == 128 ? k != 0 : h != 0;
+            tc_sts128(line + ((((c + k) & 7) ^ (r & 7)) << 4), second ? y[4] : y[0], second ? y[5] : y[1], second ? y[6] : y[2],
+                      second ? y[7] : y[3]);
+          }
+        }
+        if (any) *s_odd = 1;
         fence_proxy_async_smem();
         __syncwarp();
         if (lane == 0) mbar_arrive(v ? v_full(n % VST) : k_full(n % KST));
@@ -513,7 +521,7 @@ __global__ void __launch_bounds__(TC_THREADS, 1) tree_attention_tc_kernel(const 
           const int pg = key / p.cache.page_size;
           const int id = p.page_table[static_cast<int64_t>(in.part.b) * p.width + pg];
           if (id >= 0 && id < p.cache.num_pages)
-            row = (id * p.cache.kv_heads + in.part.seg / p.row_tiles) * p.cache.page_size + (key - pg * p.cache.page_size);
+            row = (id * p.cache.kv_heads + in.part.kvh) * p.cache.page_size + (key - pg * p.cache.page_size);
           else
             index_error();
         }
@@ -662,37 +670,27 @@ __global__ void __launch_bounds__(TC_THREADS, 1) tree_attention_tc_kernel(const 
         const int R = p.box_rows, ko = (lane / L::DB) * R, db = lane % L::DB;
         const bool on = lane < TC_BN / R * L::DB;
         const int rows_all = static_cast<int>(p.cache.num_pages) * p.cache.kv_heads * p.cache.page_size;
-        auto row_of = [&]() {
-          const int key = c.tile() * TC_BN + ko;
-          if (!on || key >= c.part.ctx + c.part.drafts) return rows_all;
-          const int pg = key / p.cache.page_size;
-          const int id = p.page_table[static_cast<int64_t>(c.part.b) * p.width + pg];
-          if (id < 0 || id >= p.cache.num_pages) {
-            index_error();
-            return rows_all;
-          }
-          return (id * p.cache.kv_heads + c.part.seg / p.row_tiles) * p.cache.page_size + (key - pg * p.cache.page_size);
-        };
         uint32_t used = 0, parity = 0;  // bit s: K stage s, 8 + s: V stage s, 16 + s: its landings
-        bool have = false, more = true, v = false, tail = false;  // an item looked up before; another one after it
-        uint32_t n = 0;
-        int row = 0;
-        while (true) {
-          const bool v0 = v, tail0 = tail;
-          const uint32_t n0 = n;
-          const int row0 = row;
-          if (more && (more = c.next(p, per_seq))) {
-            v = c.v;
-            n = c.number();
-            tail = c.tail();
-            row = row_of();
+        volatile int32_t* rows_at = reinterpret_cast<volatile int32_t*>(smem + L::OFF_ROWS) + lane;
+        while (c.next(p, per_seq)) {
+          const bool v0 = c.v, tail0 = c.tail();
+          const uint32_t n0 = c.number();
+          int row0;
+          if (v0) {
+            row0 = rows_at[(c.k_number() & 3) * 128];  // as found for the keys
+          } else {
+            const int key = c.tile() * TC_BN + ko;
+            row0 = rows_all;
+            if (on && key < c.part.ctx + c.part.drafts) {
+              const int pg = p.page_shift >= 0 ? key >> p.page_shift : key / p.cache.page_size;
+              const int id = p.page_table[static_cast<int64_t>(c.part.b) * p.width + pg];
+              if (id >= 0 && id < p.cache.num_pages)
+                row0 = (id * p.cache.kv_heads + c.part.kvh) * p.cache.page_size + (key - pg * p.cache.page_size);
+              else
+                index_error();
+            }
+            rows_at[(n0 & 3) * 128] = row0;
           }
-          if (!have) {
-            have = more;
-            if (!more) break;
-            continue;
-          }
-          have = more;
           const uint32_t st = n0 % (v0 ? VST : KST), ph = (n0 / (v0 ? VST : KST)) & 1u;
           ok = __all_sync(0xffffffffu, mbar_wait(v0 ? v_empty(st) : k_empty(st), ph ^ 1u, budget, s_abort));
           if (!ok) break;
@@ -713,7 +711,6 @@ __global__ void __launch_bounds__(TC_THREADS, 1) tree_attention_tc_kernel(const 
             if (v0) used &= ~(1u << (16 + st));
             parity = (parity & ~(1u << (v0 ? 8 + st : st))) | (ph << (v0 ? 8 + st : st));
           }
-          if (!have) break;
         }
         __syncwarp();
         for (int s = 0; s < 4; ++s) {  // let every copy land before the CTA may exit
@@ -722,75 +719,78 @@ __global__ void __launch_bounds__(TC_THREADS, 1) tree_attention_tc_kernel(const 
           if ((used >> (16 + s)) & 1) mbar_wait_drain(v_land(s), ((parity >> (16 + s)) & 1) ^ 1, budget);
         }
       } else {
-        // Half tiles of 64 rows; a lane copies the run of a page that starts at its row, if
-        // one does, for rows lane and lane + 32.
-        uint32_t half_n = 0, used = 0, parity = 0;
-        int half = 1;  // of the item looked up last
-        bool have = false, more = true;
-        int row_a = 0, len_a = 0, own_a = -1, row_b = 0, len_b = 0, own_b = -1;
-        // first row and rows of the copy that starts at row r of the half; the key's own row
-        auto run_of = [&](int r, int& row, int& len, int& own) {
-          row = len = 0;
-          own = -1;
-          const int key = c.tile() * TC_BN + half * 64 + r, hi = c.part.ctx + c.part.drafts;
-          if (key >= hi) return;
-          const int ps = p.cache.page_size, pg = key / ps, at = key - pg * ps;
-          const int id = p.page_table[static_cast<int64_t>(c.part.b) * p.width + pg];
-          if (id < 0 || id >= p.cache.num_pages) {
-            index_error();
-            return;
+        // A lane copies the runs of a page that start at its rows lane + 32 q of the tile.
+        uint32_t raw_n = 0, used = 0, parity = 0;
+        volatile int32_t* rows_at = reinterpret_cast<volatile int32_t*>(smem + L::OFF_ROWS) + lane;
+        while (c.next(p, per_seq)) {
+          const bool v0 = c.v;
+          const uint32_t n0 = c.number(), ring = ((v0 ? c.k_number() : n0) & 3) * 256;
+          int own[4], len[4];  // the key's row (-1: none), and the rows of the copy that starts there
+          if (v0) {  // as found for the keys
+#pragma unroll
+            for (int q = 0; q < 4; ++q) {
+              own[q] = rows_at[ring + 64 * q];
+              len[q] = rows_at[ring + 64 * q + 32];
+            }
+          } else {
+            const int hi = c.part.ctx + c.part.drafts;
+            int id[4], at[4];
+#pragma unroll
+            for (int q = 0; q < 4; ++q) {
+              const int key = c.tile() * TC_BN + lane + 32 * q;
+              id[q] = -1;
+              at[q] = 0;
+              if (key < hi) {
+                const int pg = p.page_shift >= 0 ? key >> p.page_shift : key / p.cache.page_size;
+                at[q] = key - pg * p.cache.page_size;
+                id[q] = p.page_table[static_cast<int64_t>(c.part.b) * p.width + pg];
+                if (id[q] < 0) id[q] = INT32_MAX;
+              }
+            }
+#pragma unroll
+            for (int q = 0; q < 4; ++q) {
+              const int r = lane + 32 * q;
+              own[q] = -1;
+              len[q] = 0;
+              if (id[q] >= p.cache.num_pages) {
+                index_error();
+              } else if (id[q] >= 0) {
+                own[q] = (id[q] * p.cache.kv_heads + c.part.kvh) * p.cache.page_size + at[q];
+                if (r == 0 || at[q] == 0) len[q] = min(min(p.cache.page_size - at[q], TC_BN - r), hi - c.tile() * TC_BN - r);
+              }
+              rows_at[ring + 64 * q] = own[q];
+              rows_at[ring + 64 * q + 32] = len[q];
+            }
           }
-          own = row = (id * p.cache.kv_heads + c.part.seg / p.row_tiles) * ps + at;
-          if (r == 0 || at == 0) len = min(min(ps - at, 64 - r), hi - key);
-        };
-        bool v = false;
-        uint32_t n = 0;
-        while (true) {
-          const bool v0 = v;
-          const uint32_t n0 = n;
-          const int h = half, ra = row_a, la = len_a, oa = own_a, rb = row_b, lb = len_b, ob = own_b;
-          half ^= 1;
-          if (half == 0 && more) more = c.next(p, per_seq);
-          if (more) {
-            v = c.v;
-            n = c.number();
-            run_of(lane, row_a, len_a, own_a);
-            run_of(lane + 32, row_b, len_b, own_b);
-          }
-          if (!have) {
-            have = more;
-            if (!more) break;
-            continue;
-          }
-          have = more;
-          const int slot = half_n % L::HALVES;
-          const uint32_t ph = (half_n / L::HALVES) & 1u;
+          const int slot = raw_n % L::RAWS;
+          const uint32_t ph = (raw_n / L::RAWS) & 1u;
           ok = __all_sync(0xffffffffu, mbar_wait(raw_empty(slot), ph ^ 1u, budget, s_abort));
           if (!ok) break;
-          const uint32_t full = raw_full(slot), dst = sbase + L::OFF_RAW + slot * L::HALF;
-          const uint32_t bytes = __reduce_add_sync(0xffffffffu, (la + lb) * D);
+          const uint32_t full = raw_full(slot), dst = sbase + L::OFF_RAW + slot * L::RAW;
+          const uint32_t bytes = __reduce_add_sync(0xffffffffu, (len[0] + len[1] + len[2] + len[3]) * D);
           if (lane == 0) mbar_arrive_expect_tx(full, bytes);
           __syncwarp();
           const uint8_t* base = static_cast<const uint8_t*>(v0 ? p.cache.v : p.cache.k);
-          if (la) bulk_load_g2s(dst + lane * D, base + static_cast<int64_t>(ra) * D, la * D, full);
-          if (lb) bulk_load_g2s(dst + (lane + 32) * D, base + static_cast<int64_t>(rb) * D, lb * D, full);
+#pragma unroll
+          for (int q = 0; q < 4; ++q)
+            if (len[q]) bulk_load_g2s(dst + (lane + 32 * q) * D, base + static_cast<int64_t>(own[q]) * D, len[q] * D, full);
           if (!v0) {
-            const uint32_t d = sbase + L::OFF_RAWSTEP + (n0 & 3) * 1024 + (h * 64 + lane) * 8;
-            ta_copy4(d, p.cache.k_scale + max(oa, 0), oa >= 0);
-            ta_copy4(d + 4, p.cache.v_scale + max(oa, 0), oa >= 0);
-            ta_copy4(d + 256, p.cache.k_scale + max(ob, 0), ob >= 0);
-            ta_copy4(d + 260, p.cache.v_scale + max(ob, 0), ob >= 0);
+#pragma unroll
+            for (int q = 0; q < 4; ++q) {
+              const uint32_t d = sbase + L::OFF_RAWSTEP + (n0 & 3) * 1024 + (lane + 32 * q) * 8;
+              ta_copy4(d, p.cache.k_scale + max(own[q], 0), own[q] >= 0);
+              ta_copy4(d + 4, p.cache.v_scale + max(own[q], 0), own[q] >= 0);
+            }
             tc_copies_arrive(full);
           } else {
             mbar_arrive(full);
           }
           used |= 1u << slot;
           parity = (parity & ~(1u << slot)) | (ph << slot);
-          ++half_n;
-          if (!have) break;
+          ++raw_n;
         }
         __syncwarp();
-        for (int s = 0; s < L::HALVES; ++s)
+        for (int s = 0; s < L::RAWS; ++s)
           if ((used >> s) & 1) mbar_wait_drain(raw_full(s), (parity >> s) & 1, budget);
       }
     }
@@ -809,7 +809,7 @@ __global__ void __launch_bounds__(TC_THREADS, 1) tree_attention_tc_kernel(const 
     walk.begin(p, *s_share, TC_BN);
     TaPart part;
     while (walk.next(p, per_seq, TC_BN, part)) {
-      const int kvh = part.seg / p.row_tiles, rt = part.seg % p.row_tiles;
+      const int kvh = part.kvh, rt = part.seg - kvh * p.row_tiles;
       const int gr = rt * QT * TC_BN + (QT == 1 ? 0 : t * TC_BN) + lrow;
       const int itok = gr / p.group;
       const bool valid = gr < rows && itok < part.drafts;
