@@ -97,18 +97,19 @@ __device__ __forceinline__ uint32_t ta_pack(float a, float b, bool bf) {
   const __half2 h = __floats2half2_rn(a, b);
   return *reinterpret_cast<const uint32_t*>(&h);
 }
-// Two stored 8-bit values (the low half of w) as an f16 pair, exactly.
+// Four stored 8-bit values as two f16 pairs, exactly.
 template <int FMT>
-__device__ __forceinline__ uint32_t ta_widen(uint32_t w) {
+__device__ __forceinline__ void ta_widen4(uint32_t w, uint32_t& lo, uint32_t& hi) {
   if constexpr (FMT == TA_FP8) {
-    uint32_t r;
-    asm("{.reg .b16 lo, hi; mov.b32 {lo, hi}, %1; cvt.rn.f16x2.e4m3x2 %0, lo;}" : "=r"(r) : "r"(w));
-    return r;
+    asm("{.reg .b16 a, b; mov.b32 {a, b}, %2; cvt.rn.f16x2.e4m3x2 %0, a; cvt.rn.f16x2.e4m3x2 %1, b;}" : "=r"(lo), "=r"(hi) : "r"(w));
   } else {
     // byte + 128 becomes the low bits of 1024 + byte + 128; subtract 1152
-    const uint32_t biased = __byte_perm(w ^ 0x80808080u, 0x64646464u, 0x4140);
-    const __half2 h = __hsub2(*reinterpret_cast<const __half2*>(&biased), __float2half2_rn(1152.0f));
-    return *reinterpret_cast<const uint32_t*>(&h);
+    const uint32_t x = w ^ 0x80808080u;
+    const uint32_t a = __byte_perm(x, 0x64646464u, 0x4140), b = __byte_perm(x, 0x64646464u, 0x4342);
+    const __half2 off = __float2half2_rn(1152.0f);
+    const __half2 ha = __hsub2(*reinterpret_cast<const __half2*>(&a), off), hb = __hsub2(*reinterpret_cast<const __half2*>(&b), off);
+    lo = *reinterpret_cast<const uint32_t*>(&ha);
+    hi = *reinterpret_cast<const uint32_t*>(&hb);
   }
 }
 
@@ -318,7 +319,8 @@ __global__ void __launch_bounds__(TaLayout<FMT, D, MT>::NW * 32, 1) tree_attenti
           const uint32_t ww[4] = {w.x, w.y, w.z, w.w};
 #pragma unroll
           for (int c = 0; c < 4; ++c) {
-            const uint32_t b0 = ta_widen<FMT>(ww[c]), b1 = ta_widen<FMT>(ww[c] >> 16);
+            uint32_t b0, b1;
+            ta_widen4<FMT>(ww[c], b0, b1);
 #pragma unroll
             for (int m = 0; m < MT; ++m) ta_mma<false>(s[m][j], qf[m][4 * i + c], b0, b1);
           }
@@ -444,8 +446,8 @@ __global__ void __launch_bounds__(TaLayout<FMT, D, MT>::NW * 32, 1) tree_attenti
           for (int q = 0; q < 2; ++q) {
             const uint32_t u = __byte_perm(w[2 * q], w[2 * q + 1], 0x5140);  // columns 0, 1 of both rows
             const uint32_t v = __byte_perm(w[2 * q], w[2 * q + 1], 0x7362);  // columns 2, 3
-            vb[0][q] = ta_widen<FMT>(u), vb[1][q] = ta_widen<FMT>(u >> 16);
-            vb[2][q] = ta_widen<FMT>(v), vb[3][q] = ta_widen<FMT>(v >> 16);
+            ta_widen4<FMT>(u, vb[0][q], vb[1][q]);
+            ta_widen4<FMT>(v, vb[2][q], vb[3][q]);
           }
         }
         if (FMT != TA_INT8 && !all) {
@@ -492,7 +494,8 @@ __global__ void __launch_bounds__(TaLayout<FMT, D, MT>::NW * 32, 1) tree_attenti
                 const uint32_t word = ta_lds32(a & ~3u) >> (8 * (a & 3));
                 float v;
                 if constexpr (QUANT) {
-                  const uint32_t h = ta_widen<FMT>(word & 0xffu);
+                  uint32_t h, unused;
+                  ta_widen4<FMT>(word & 0xffu, h, unused);
                   v = __half2float(__ushort_as_half(static_cast<unsigned short>(h & 0xffffu)));
                 } else if constexpr (BF) {
                   v = __uint_as_float(word << 16);

@@ -391,7 +391,10 @@ __global__ void __launch_bounds__(TC_THREADS, 1) tree_attention_tc_kernel(const 
     TcCursor in;
     if constexpr (QUANT) {
       constexpr int CPR = D / 16, PER = TC_BN * CPR / 128;  // 16-byte pieces per row; per thread
-      const int col = tid % CPR, row0 = tid / CPR;
+      // Eight neighbouring threads take four pieces of each of two rows, from other halves of
+      // the row: then neither their reads nor their two stores each meet a bank twice.
+      const int col = D == 128 ? ((tid & 7) + ((tid >> 3) & 1) * 4) & 7 : tid % CPR;
+      const int row0 = D == 128 ? (tid >> 4) * 2 + ((tid >> 2) & 1) : tid / CPR;
       uint32_t raw_n = 0;
       bool ok = true;
       in.begin(walk, LEAD);
@@ -403,7 +406,7 @@ __global__ void __launch_bounds__(TC_THREADS, 1) tree_attention_tc_kernel(const 
         ok = __all_sync(0xffffffffu, mbar_wait(raw_full(slot), (raw_n / L::RAWS) & 1u, budget, s_abort));
         if (!ok) break;
         ++raw_n;
-        const uint4* raw = reinterpret_cast<const uint4*>(smem + L::OFF_RAW + slot * L::RAW) + tid;
+        const uint4* raw = reinterpret_cast<const uint4*>(smem + L::OFF_RAW + slot * L::RAW) + row0 * CPR + col;
         uint4 w[PER];
 #pragma unroll
         for (int i = 0; i < PER; ++i) w[i] = raw[i * 128];
@@ -438,9 +441,7 @@ __global__ void __launch_bounds__(TC_THREADS, 1) tree_attention_tc_kernel(const 
         ok = __all_sync(0xffffffffu, mbar_wait(v ? v_empty(n % VST) : k_empty(n % KST), ((n / (v ? VST : KST)) & 1u) ^ 1u, budget, s_abort));
         if (!ok) break;
         const uint32_t to = v ? sV0 + (n % VST) * L::TILE : sK0 + (n % KST) * L::TILE;
-        // A piece becomes two 16-byte chunks of the widened row; threads of the row's second
-        // 64 columns store theirs in the other order, so that eight of them meet no bank twice.
-        const int c = 2 * col, swap = c >> 3;
+        const int c = 2 * col;  // a piece becomes two 16-byte chunks of the widened row
         bool any = false;
 #pragma unroll
         for (int i = 0; i < PER; ++i) {
@@ -448,23 +449,15 @@ __global__ void __launch_bounds__(TC_THREADS, 1) tree_attention_tc_kernel(const 
           const uint32_t x[4] = {w[i].x, w[i].y, w[i].z, w[i].w};
           uint32_t y[8];
 #pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            y[2 * e] = ta_widen<FMT>(x[e]);
-            y[2 * e + 1] = ta_widen<FMT>(x[e] >> 16);
-          }
+          for (int e = 0; e < 4; ++e) ta_widen4<FMT>(x[e], y[2 * e], y[2 * e + 1]);
           if (FMT == TA_FP8 && tail) {
 #pragma unroll
             for (int e = 0; e < 8; ++e)
               if (v) any |= tc_clean<false>(y[e]);
           }
           const uint32_t line = to + (v ? ((r >> 6) * L::DB + (c >> 3)) * 8192 + (r & 63) * 128 : (c >> 3) * 16384 + r * 128);
-#pragma unroll
-          for (int h = 0; h < 2; ++h) {
-            const int k = D == 128 ? h ^ swap : h;
-            const bool second = D == 128 ? k != 0 : h != 0;
-            tc_sts128(line + ((((c + k) & 7) ^ (r & 7)) << 4), second ? y[4] : y[0], second ? y[5] : y[1], second ? y[6] : y[2],
-                      second ? y[7] : y[3]);
-          }
+          tc_sts128(line + (((c & 7) ^ (r & 7)) << 4), y[0], y[1], y[2], y[3]);
+          tc_sts128(line + ((((c + 1) & 7) ^ (r & 7)) << 4), y[4], y[5], y[6], y[7]);
         }
         if (any) *s_odd = 1;
         fence_proxy_async_smem();
