@@ -250,6 +250,33 @@ def lib() -> ctypes.CDLL:
     return _lib
 
 
+_torch_binding = None
+TORCH_BINDING_PATH = _LIB_DIR / "ojx_torch.so"
+
+
+def torch_binding():
+    """The compiled binding of the serving operators for torch CUDA tensors
+    (csrc/torch_binding.cpp), bound to the loaded library's entries.  Raises if it has
+    not been built."""
+    global _torch_binding
+    if _torch_binding is None:
+        L = lib()
+        with _lock:
+            if _torch_binding is None:
+                import importlib.util
+                if not TORCH_BINDING_PATH.exists():
+                    raise RuntimeError(f"{TORCH_BINDING_PATH} not found; build it with "
+                                       "`python ojasx-open-source-cuda-_b200/build.py`")
+                spec = importlib.util.spec_from_file_location("ojx_torch", TORCH_BINDING_PATH)
+                mod = importlib.util.module_from_spec(spec)
+                spec.loader.exec_module(mod)
+                names = ("ojx_qk_norm_rope", "ojx_qk_norm_rope_backward", "ojx_qkv_to_cache", "ojx_kv_append",
+                         "ojx_kv_read", "ojx_tree_attention", "ojx_verify_drafts", "ojx_last_error")
+                mod.bind({n: ctypes.cast(getattr(L, n), ctypes.c_void_p).value for n in names})
+                _torch_binding = mod
+    return _torch_binding
+
+
 def last_error() -> str:
     msg = lib().ojx_last_error()
     return msg.decode(errors="replace") if msg else ""

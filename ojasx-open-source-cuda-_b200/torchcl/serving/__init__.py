@@ -36,6 +36,11 @@ _ref = ctypes.byref
 
 # ── device arguments ──────────────────────────────────────────────────────────
 
+def _cuda(t) -> bool:
+    """Whether a call is one of torch CUDA tensors: those go through the compiled binding."""
+    return isinstance(t, torch.Tensor) and t.is_cuda
+
+
 def _on_torch(t) -> bool:
     """True for a torch CUDA tensor, False for a torchcl handle, ValueError otherwise."""
     if isinstance(t, torch.Tensor) and t.is_cuda:
@@ -152,6 +157,8 @@ def _qk_desc(on_torch, q, k, q_weight, k_weight, table, positions, eps, interlea
 
 
 def _qk_forward(q, k, q_weight, k_weight, table, positions, eps, interleaved):
+    if _cuda(q):
+        return L.torch_binding().qk_forward(q, k, q_weight, k_weight, table, positions, eps, interleaved)
     on_torch = _on_torch(q)
     d, dtype, _, keep = _qk_desc(on_torch, q, k, q_weight, k_weight, table, positions, eps, interleaved)
     q_out, qp = _empty(_get_shape(q), dtype, on_torch)
@@ -162,6 +169,9 @@ def _qk_forward(q, k, q_weight, k_weight, table, positions, eps, interleaved):
 
 def _qk_backward(gq, gk, q, k, q_weight, k_weight, table, positions, eps, interleaved, want_weights=True):
     """(dq, dk, dq_weight, dk_weight) of qk_norm_rope; the weights' None where not wanted."""
+    if _cuda(q):
+        return L.torch_binding().qk_backward(gq, gk, q, k, q_weight, k_weight, table, positions, eps, interleaved,
+                                             want_weights)
     on_torch = _on_torch(q)
     d, dtype, wdtype, keep = _qk_desc(on_torch, q, k, q_weight, k_weight, table, positions, eps, interleaved)
     ga, gq_rows, _ = _rows(gq, on_torch, "grad of q", (d.tokens, d.q_heads, d.head_dim))
@@ -192,6 +202,8 @@ def qk_norm_rope(q, k, q_weight, k_weight, table, positions, eps: float = 1e-6, 
     Pairs are (i, i + rotary_dim/2), or (2i, 2i + 1) when `interleaved`.  Sums run in
     fp32; outputs are rounded once to the inputs' dtype.  Returns dense (q, k).
     Differentiable in q, k and the weights (QKNormRopeFunction)."""
+    if _cuda(q):
+        return L.torch_binding().qk_norm_rope(q, k, q_weight, k_weight, table, positions, eps, interleaved)
     if torch.is_grad_enabled() and any(getattr(t, "requires_grad", False) for t in (q, k, q_weight, k_weight)):
         from torchcl.autograd import QKNormRopeFunction
         return QKNormRopeFunction.apply(q, k, q_weight, k_weight, table, positions, eps, interleaved)
@@ -203,6 +215,9 @@ def qkv_to_cache(q, k, v, q_weight, k_weight, table, positions, cache: "KVCache"
     """qk_norm_rope for serving: returns the normed and rotated q; the normed and rotated
     k (unrounded) and v go straight into `cache` at `slots` ([tokens], int32 or int64;
     a negative slot skips the token's keys and values)."""
+    if _cuda(q):
+        return L.torch_binding().qkv_to_cache(q, k, v, q_weight, k_weight, table, positions, cache._address(), slots, eps,
+                                              interleaved)
     on_torch = _on_torch(q)
     d, dtype, _, keep = _qk_desc(on_torch, q, k, q_weight, k_weight, table, positions, eps, interleaved)
     va, v_rows, _ = _rows(v, on_torch, "v", (d.tokens, d.kv_heads, d.head_dim))
@@ -294,17 +309,27 @@ class KVCache:
         self.num_pages, self.page_size, self.kv_heads = num_pages, page_size, kv_heads
         self.head_dim, self.format = head_dim, format
         addr = [None if b is None else b.buffer if isinstance(b, CLBuffer) else b.data_ptr() for b in self._pages]
+        self._pooled = any(isinstance(b, CLBuffer) for b in self._pages)
         self._desc = L.KVCacheDesc(*addr, num_pages, page_size, kv_heads, head_dim, L.KV_FORMATS[format])
 
+        self._where = ctypes.addressof(self._desc)
+
     def _use(self) -> "L.KVCacheDesc":
-        for buf in self._pages:
-            if isinstance(buf, CLBuffer):
-                note_use(buf)  # a graph being captured must keep it
+        if self._pooled:
+            for buf in self._pages:
+                if buf is not None:
+                    note_use(buf)  # a graph being captured must keep it
         return self._desc
+
+    def _address(self) -> int:
+        self._use()
+        return self._where
 
     def append(self, k, v, slots) -> None:
         """Write keys and values [tokens, kv_heads, head_dim] (float32, bfloat16 or
         float16) to `slots` ([tokens], int32 or int64; a negative slot is skipped)."""
+        if _cuda(k):
+            return L.torch_binding().kv_append(self._address(), k, v, slots)
         on_torch = _on_torch(k)
         ka, k_rows, n = _rows(k, on_torch, "k")
         if ka.shape[-2:] != (self.kv_heads, self.head_dim):
@@ -321,6 +346,8 @@ class KVCache:
     def read(self, slots, dtype: torch.dtype = torch.bfloat16):
         """(k, v), dense [tokens, kv_heads, head_dim] of `dtype`, as the cache holds them
         at `slots`; a negative slot gives zeros."""
+        if _cuda(slots):
+            return L.torch_binding().kv_read(self._address(), slots, dtype)
         on_torch = _on_torch(slots)
         code = ojx_dtype(dtype)
         sa = _Arg(slots, on_torch, "slots", _INTS, integer=True)
@@ -386,6 +413,8 @@ def tree_attention(q, cache: KVCache, page_table, context_lens, mask=None, draft
     without a mask is a decoding step.  Queries i >= draft_lens[b], and queries that see
     nothing, give zeros; nothing a query does not see reaches it, whatever it holds.
     Returns dense [batch, tokens, q_heads, head_dim]."""
+    if _cuda(q):
+        return L.torch_binding().tree_attention(q, cache._address(), page_table, context_lens, mask, draft_lens, scale)
     on_torch = _on_torch(q)
     qa = _Arg(q, on_torch, "q", (torch.bfloat16, torch.float16))
     if len(qa.shape) != 4 or qa.shape[3] != cache.head_dim:
@@ -439,6 +468,8 @@ def verify_drafts(target_probs, tokens, parents, uniforms, draft_probs=None):
     Returns int32 path [batch, nodes] (the root and the accepted nodes, then -1), count
     [batch] (accepted drafts) and next_token [batch] (-1: the row holds no probability).
     Sums are exact in units of 2^-38, so results do not depend on the launch shape."""
+    if _cuda(target_probs):
+        return L.torch_binding().verify_drafts(target_probs, tokens, parents, uniforms, draft_probs)
     on_torch = _on_torch(target_probs)
     pa = _Arg(target_probs, on_torch, "target_probs")
     if len(pa.shape) != 3:
