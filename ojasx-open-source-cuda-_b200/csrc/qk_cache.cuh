@@ -15,6 +15,7 @@
 // A lane holds CH elements of both halves of a pair, so the rotation needs no exchange
 // between lanes, and 32 / lanes-per-row rows share a warp.
 #pragma once
+#include <type_traits>
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <cuda_fp8.h>
@@ -120,6 +121,7 @@ struct QkParams {
   int64_t tokens;
   int D, rotary, half, npairs, lanes, norm;
   int hq, hk, hv, blocks_per_token, iters;
+  int gq, gk, gv;  // row groups (of 32 / lanes heads) of each side
   int dtype_w, pos64, slot64, k_to_cache;
   float eps;
   const void *q, *k, *v;
@@ -132,7 +134,7 @@ struct QkParams {
   ojx_kv_cache cache;
   const void* slots;
   // gradient
-  const void *gq, *gk;
+  const void *gq_data, *gk_data;
   int64_t gq_st, gq_sh, gk_st, gk_sh;
   void *dq, *dk;
   float* partial;  // [blocks][D] sums of dw: q_blocks of the query weight, then the key's
@@ -374,7 +376,7 @@ __global__ void __launch_bounds__(256) qk_grad_kernel(const QkParams p) {
   const int blocks = is_q ? p.q_blocks : gridDim.x - p.q_blocks;
   const int heads = is_q ? p.hq : p.hk;
   const T* xs = static_cast<const T*>(is_q ? p.q : p.k);
-  const T* gs = static_cast<const T*>(is_q ? p.gq : p.gk);
+  const T* gs = static_cast<const T*>(is_q ? p.gq_data : p.gk_data);
   T* dxs = static_cast<T*>(is_q ? p.dq : p.dk);
   const int64_t x_st = is_q ? p.q_st : p.k_st, x_sh = is_q ? p.q_sh : p.k_sh;
   const int64_t g_st = is_q ? p.gq_st : p.gk_st, g_sh = is_q ? p.gq_sh : p.gk_sh;
@@ -486,64 +488,486 @@ __global__ void __launch_bounds__(256) qk_grad_kernel(const QkParams p) {
   }
 }
 
+// ── two float32 operations an instruction ──────────────────────────────────────────
+__device__ __forceinline__ uint64_t f2_pair(float a, float b) {
+  uint64_t r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+  return r;
+}
+__device__ __forceinline__ float2 f2_split(uint64_t v) {
+  float2 r;
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(v));
+  return r;
+}
+__device__ __forceinline__ uint64_t f2_swap(uint64_t v) {
+  const float2 a = f2_split(v);
+  return f2_pair(a.y, a.x);
+}
+__device__ __forceinline__ uint64_t f2_fma(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+__device__ __forceinline__ uint64_t f2_mul(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ uint64_t f2_add(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+
+// Eight elements as they lie in memory, and as four float32 pairs.
+template <typename T>
+struct Eight {
+  uint4 v[8 * sizeof(T) / 16];
+  __device__ __forceinline__ void clear() {
+#pragma unroll
+    for (int i = 0; i < static_cast<int>(8 * sizeof(T) / 16); ++i) v[i] = make_uint4(0, 0, 0, 0);
+  }
+  __device__ __forceinline__ void load(const T* p) {
+#pragma unroll
+    for (int i = 0; i < static_cast<int>(8 * sizeof(T) / 16); ++i) v[i] = reinterpret_cast<const uint4*>(p)[i];
+  }
+  __device__ __forceinline__ void pairs(uint64_t (&x)[4]) const {
+    const uint32_t* w = reinterpret_cast<const uint32_t*>(v);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      if constexpr (sizeof(T) == 4) {
+        x[i] = f2_pair(__uint_as_float(w[2 * i]), __uint_as_float(w[2 * i + 1]));
+      } else if constexpr (std::is_same<T, __nv_bfloat16>::value) {
+        x[i] = f2_pair(__uint_as_float(w[i] << 16), __uint_as_float(w[i] & 0xffff0000u));
+      } else {
+        const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&w[i]));
+        x[i] = f2_pair(f.x, f.y);
+      }
+    }
+  }
+};
+// Eight float32 values to eight elements of T: one store of 32 (float32: the widest there
+// is) or 16 bytes.  (Stores of half a 32-byte sector each cost the L2 a transaction.)
+template <typename T>
+__device__ __forceinline__ void store_pairs(T* p, const uint64_t (&x)[4], bool wide) {
+  if constexpr (sizeof(T) == 4) {
+    const float2 a = f2_split(x[0]), b = f2_split(x[1]), c = f2_split(x[2]), d = f2_split(x[3]);
+    if (wide) {
+      asm volatile("st.global.v8.f32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(p), "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(c.x),
+                   "f"(c.y), "f"(d.x), "f"(d.y)
+                   : "memory");
+    } else {
+      reinterpret_cast<float4*>(p)[0] = make_float4(a.x, a.y, b.x, b.y);
+      reinterpret_cast<float4*>(p)[1] = make_float4(c.x, c.y, d.x, d.y);
+    }
+  } else {
+    uint32_t w[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const float2 f = f2_split(x[i]);
+      if constexpr (std::is_same<T, __nv_bfloat16>::value) {
+        const __nv_bfloat162 h = __floats2bfloat162_rn(f.x, f.y);
+        w[i] = *reinterpret_cast<const uint32_t*>(&h);
+      } else {
+        const __half2 h = __floats2half2_rn(f.x, f.y);
+        w[i] = *reinterpret_cast<const uint32_t*>(&h);
+      }
+    }
+    *reinterpret_cast<uint4*>(p) = make_uint4(w[0], w[1], w[2], w[3]);
+  }
+}
+__device__ __forceinline__ void load_weight(const void* w, int at, int dtype, bool on, uint64_t (&x)[4]) {
+  float v[8];
+#pragma unroll
+  for (int e = 0; e < 8; ++e) v[e] = 1.0f;
+  if (w && on) load_chunk_as<8>(w, at, dtype, v);
+#pragma unroll
+  for (int i = 0; i < 4; ++i) x[i] = f2_pair(v[2 * i], v[2 * i + 1]);
+}
+
+// The turn of a chunk pair (a, b), in pairs of elements.  Halves: (c, s) of elements 2 i,
+// 2 i + 1, the same for both chunks.  Interleaved: element pairs turn on themselves,
+// (c, c) and (-s, s), each chunk with its own four.
+template <bool INTER>
+struct Turn {
+  uint64_t c[INTER ? 8 : 4], s[INTER ? 8 : 4];
+  __device__ __forceinline__ void load(const QkParams& p, int64_t pos, bool known, bool turns, int a) {
+    float cs[8], sn[8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      cs[e] = known ? 1.0f : NAN;  // a token without a position reads as NaN
+      sn[e] = 0.0f;
+    }
+    if (turns && known) {
+      const float* row = p.table + pos * p.rotary + (INTER ? a / 2 : a);
+      if (((p.rotary & 7) | (reinterpret_cast<uintptr_t>(p.table) & 15)) == 0) {
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          const float4 x = reinterpret_cast<const float4*>(row)[h], y = reinterpret_cast<const float4*>(row + p.half)[h];
+          cs[4 * h] = x.x, cs[4 * h + 1] = x.y, cs[4 * h + 2] = x.z, cs[4 * h + 3] = x.w;
+          sn[4 * h] = y.x, sn[4 * h + 1] = y.y, sn[4 * h + 2] = y.z, sn[4 * h + 3] = y.w;
+        }
+      } else {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          cs[e] = row[e];
+          sn[e] = row[p.half + e];
+        }
+      }
+    }
+    if constexpr (INTER) {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        c[e] = f2_pair(cs[e], cs[e]);
+        s[e] = f2_pair(-sn[e], sn[e]);
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        c[i] = f2_pair(cs[2 * i], cs[2 * i + 1]);
+        s[i] = f2_pair(sn[2 * i], sn[2 * i + 1]);
+      }
+    }
+  }
+  // SIGN 1: by the angle, -1: back.
+  template <int SIGN>
+  __device__ __forceinline__ void apply(uint64_t (&a)[4], uint64_t (&b)[4]) const {
+    const uint64_t minus = f2_pair(-1.0f, -1.0f);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      if constexpr (INTER) {
+        const uint64_t sa = SIGN > 0 ? s[i] : f2_mul(s[i], minus), sb = SIGN > 0 ? s[4 + i] : f2_mul(s[4 + i], minus);
+        a[i] = f2_fma(f2_swap(a[i]), sa, f2_mul(a[i], c[i]));
+        b[i] = f2_fma(f2_swap(b[i]), sb, f2_mul(b[i], c[4 + i]));
+      } else {
+        const uint64_t n = f2_mul(s[i], minus);
+        const uint64_t u = a[i], v = b[i];
+        a[i] = f2_fma(v, SIGN > 0 ? n : s[i], f2_mul(u, c[i]));
+        b[i] = f2_fma(u, SIGN > 0 ? s[i] : n, f2_mul(v, c[i]));
+      }
+    }
+  }
+};
+
+__device__ __forceinline__ float f2_total(uint64_t v) {
+  const float2 a = f2_split(v);
+  return a.x + a.y;
+}
+
+// Forward rows in 16-byte chunks.  A group is 32 / lanes heads of one side (queries, keys,
+// values) of a token; a warp runs p.iters groups of one token with the next two groups'
+// loads in flight: at 16 warps an SM that covers HBM's latency.  One group at a time took
+// 116 us for 16384 tokens of 40 bf16 heads of 128.
+template <typename T, bool INTER, bool NORM>
+__global__ void __launch_bounds__(256, NORM ? 2 : 3) qk_rows_fast_kernel(const QkParams p) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int sub = lane / p.lanes, j = lane % p.lanes, per_warp = 32 / p.lanes;
+  const int64_t item = static_cast<int64_t>(blockIdx.x) * (blockDim.x >> 5) + warp;
+  const int64_t token = item / p.blocks_per_token;
+  if (token >= p.tokens) return;  // whole warp
+  const int first = static_cast<int>(item - token * p.blocks_per_token) * p.iters;
+  const int end = min(first + p.iters, p.gq + p.gk + p.gv);
+  const bool on = j < p.npairs;
+  int a = 0, b = 0;
+  const bool turns = on && pair_at<8, INTER>(p, j, a, b);
+
+  auto fetch = [&](int g, Eight<T>& xa, Eight<T>& xb) {
+    const bool is_q = g < p.gq, is_k = !is_q && g < p.gq + p.gk;
+    const int h = (g - (is_q ? 0 : is_k ? p.gq : p.gq + p.gk)) * per_warp + sub;
+    const int heads = is_q ? p.hq : is_k ? p.hk : p.hv;
+    xa.clear();
+    xb.clear();
+    if (g < end && on && h < heads) {
+      const T* x = is_q   ? static_cast<const T*>(p.q) + token * p.q_st + h * p.q_sh
+                   : is_k ? static_cast<const T*>(p.k) + token * p.k_st + h * p.k_sh
+                          : static_cast<const T*>(p.v) + token * p.v_st + h * p.v_sh;
+      xa.load(x + a);
+      xb.load(x + b);
+    }
+  };
+  Eight<T> a0, b0, a1, b1;
+  fetch(first, a0, b0);
+  fetch(first + 1, a1, b1);
+
+  Turn<INTER> turn;
+  uint64_t wa[4], wb[4];
+  if (NORM) {
+    const int64_t pos = load_index(p.positions, token, p.pos64);
+    const bool known = pos >= 0 && pos < p.table_rows;
+    if (!known && lane == 0) index_error();
+    turn.load(p, pos, known, turns, a);
+  }
+  const int64_t slot = p.slots ? load_index(p.slots, token, p.slot64) : -1;
+  const bool wide_q = (reinterpret_cast<uintptr_t>(p.q_out) & 31) == 0, wide_k = (reinterpret_cast<uintptr_t>(p.k_out) & 31) == 0;
+  int side = -1;  // whose weights wa and wb are
+#pragma unroll 2
+  for (int g = first; g < end; ++g) {
+    const bool is_q = g < p.gq, is_k = !is_q && g < p.gq + p.gk;  // uniform
+    const int h = (g - (is_q ? 0 : is_k ? p.gq : p.gq + p.gk)) * per_warp + sub;
+    const bool valid = h < (is_q ? p.hq : is_k ? p.hk : p.hv);
+    uint64_t xa[4], xb[4];
+    a0.pairs(xa);
+    b0.pairs(xb);
+    a0 = a1;
+    b0 = b1;
+    fetch(g + 2, a1, b1);
+    if (NORM && (is_q || is_k)) {
+      if (side != (is_q ? 0 : 1)) {
+        side = is_q ? 0 : 1;
+        load_weight(is_q ? p.qw : p.kw, a, p.dtype_w, on, wa);
+        load_weight(is_q ? p.qw : p.kw, b, p.dtype_w, on, wb);
+      }
+      uint64_t ss = f2_mul(xa[0], xa[0]);
+#pragma unroll
+      for (int i = 1; i < 4; ++i) ss = f2_fma(xa[i], xa[i], ss);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) ss = f2_fma(xb[i], xb[i], ss);
+      const float r = rsqrtf(group_sum(f2_total(ss), p.lanes) / p.D + p.eps);
+      const uint64_t r2 = f2_pair(r, r);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        xa[i] = f2_mul(f2_mul(xa[i], r2), wa[i]);
+        xb[i] = f2_mul(f2_mul(xb[i], r2), wb[i]);
+      }
+      turn.template apply<1>(xa, xb);
+    }
+    if (is_q || (is_k && !p.k_to_cache)) {
+      if (valid && on) {
+        T* out = is_q ? static_cast<T*>(p.q_out) + (token * p.hq + h) * p.D : static_cast<T*>(p.k_out) + (token * p.hk + h) * p.D;
+        store_pairs<T>(out + a, xa, is_q ? wide_q : wide_k);
+        store_pairs<T>(out + b, xb, is_q ? wide_q : wide_k);
+      }
+    } else {
+      float va[8], vb[8], amax = 0.0f;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const float2 u = f2_split(xa[i]), v = f2_split(xb[i]);
+        va[2 * i] = u.x, va[2 * i + 1] = u.y, vb[2 * i] = v.x, vb[2 * i + 1] = v.y;
+      }
+      float step = 0.0f;
+      if (p.cache.format >= OJX_KV_INT8) {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) amax = max_nan(amax, max_nan(fabsf(va[e]), fabsf(vb[e])));
+        for (int o = p.lanes >> 1; o > 0; o >>= 1) amax = max_nan(amax, __shfl_xor_sync(0xffffffffu, amax, o));
+        step = quantise_step(amax, p.cache.format);
+      }
+      const int64_t row = valid ? slot_row(p.cache, slot, h) : -1;
+      if (row >= 0 && on) {
+        void* base = is_k ? p.cache.k : p.cache.v;
+        if (p.cache.format >= OJX_KV_INT8 && j == 0) (is_k ? p.cache.k_scale : p.cache.v_scale)[row] = step;
+        store_cached<8>(base, row * p.D + a, p.cache.format, step, va);
+        store_cached<8>(base, row * p.D + b, p.cache.format, step, vb);
+      }
+    }
+  }
+}
+
+// Gradient rows in 16-byte chunks, the next group's two loads in flight; otherwise as
+// qk_grad_kernel.
+template <typename T, bool INTER>
+__global__ void __launch_bounds__(256, 2) qk_grad_fast_kernel(const QkParams p) {
+  extern __shared__ float sw[];  // [warps][D]
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5;
+  const int sub = lane / p.lanes, j = lane % p.lanes, per_warp = 32 / p.lanes;
+  const bool is_q = blockIdx.x < p.q_blocks;
+  const int block = is_q ? blockIdx.x : blockIdx.x - p.q_blocks;
+  const int blocks = is_q ? p.q_blocks : gridDim.x - p.q_blocks;
+  const int heads = is_q ? p.hq : p.hk, groups = is_q ? p.gq : p.gk;
+  const T* xs = static_cast<const T*>(is_q ? p.q : p.k);
+  const T* gs = static_cast<const T*>(is_q ? p.gq_data : p.gk_data);
+  T* dxs = static_cast<T*>(is_q ? p.dq : p.dk);
+  const int64_t x_st = is_q ? p.q_st : p.k_st, x_sh = is_q ? p.q_sh : p.k_sh;
+  const int64_t g_st = is_q ? p.gq_st : p.gk_st, g_sh = is_q ? p.gq_sh : p.gk_sh;
+  const bool wide = (reinterpret_cast<uintptr_t>(dxs) & 31) == 0;
+  const bool on = j < p.npairs;
+  int a = 0, b = 0;
+  const bool turns = on && pair_at<8, INTER>(p, j, a, b);
+  uint64_t wa[4], wb[4], da[4], db[4];
+  load_weight(is_q ? p.qw : p.kw, a, p.dtype_w, on, wa);
+  load_weight(is_q ? p.qw : p.kw, b, p.dtype_w, on, wb);
+#pragma unroll
+  for (int i = 0; i < 4; ++i) da[i] = db[i] = 0;
+
+  const int64_t stride = static_cast<int64_t>(blocks) * warps;
+  int64_t token = static_cast<int64_t>(block) * warps + warp;
+  int64_t next_token = token;  // of the loads in flight
+  int next_group = 0;
+  Eight<T> ra, rb, sa, sb;
+  auto fetch = [&]() {
+    const int h = next_group * per_warp + sub;
+    ra.clear(), rb.clear(), sa.clear(), sb.clear();
+    if (next_token < p.tokens && on && h < heads) {
+      const T* x = xs + next_token * x_st + h * x_sh;
+      const T* g = gs + next_token * g_st + h * g_sh;
+      ra.load(x + a);
+      rb.load(x + b);
+      sa.load(g + a);
+      sb.load(g + b);
+    }
+    if (++next_group == groups) next_group = 0, next_token += stride;
+  };
+  fetch();
+  Turn<INTER> turn;
+  for (; token < p.tokens; token += stride) {
+    const int64_t pos = load_index(p.positions, token, p.pos64);
+    const bool known = pos >= 0 && pos < p.table_rows;
+    if (!known && lane == 0) index_error();
+    turn.load(p, pos, known, turns, a);
+    for (int rg = 0; rg < groups; ++rg) {
+      const int h = rg * per_warp + sub;
+      uint64_t xa[4], xb[4], ga[4], gb[4];
+      ra.pairs(xa);
+      rb.pairs(xb);
+      sa.pairs(ga);
+      sb.pairs(gb);
+      fetch();
+      turn.template apply<-1>(ga, gb);
+      uint64_t ss = 0, hx = 0;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        ss = f2_fma(xa[i], xa[i], ss);
+        ss = f2_fma(xb[i], xb[i], ss);
+        hx = f2_fma(f2_mul(ga[i], wa[i]), xa[i], hx);
+        hx = f2_fma(f2_mul(gb[i], wb[i]), xb[i], hx);
+      }
+      float s1 = f2_total(ss), s2 = f2_total(hx);
+      for (int o = p.lanes >> 1; o > 0; o >>= 1) {
+        s1 += __shfl_xor_sync(0xffffffffu, s1, o);
+        s2 += __shfl_xor_sync(0xffffffffu, s2, o);
+      }
+      const float r = rsqrtf(s1 / p.D + p.eps);
+      const float back = -(r * r * s2 / p.D);
+      const uint64_t r2 = f2_pair(r, r), back2 = f2_pair(back, back);
+      if (h < heads && on) {
+        T* dx = dxs + (token * heads + h) * p.D;
+        uint64_t oa[4], ob[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          oa[i] = f2_mul(f2_fma(xa[i], back2, f2_mul(ga[i], wa[i])), r2);
+          ob[i] = f2_mul(f2_fma(xb[i], back2, f2_mul(gb[i], wb[i])), r2);
+          da[i] = f2_fma(ga[i], f2_mul(xa[i], r2), da[i]);
+          db[i] = f2_fma(gb[i], f2_mul(xb[i], r2), db[i]);
+        }
+        store_pairs<T>(dx + a, oa, wide);
+        store_pairs<T>(dx + b, ob, wide);
+      }
+    }
+  }
+  // rows of the warp, then warps of the block, in a fixed order
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    for (int o = p.lanes; o < 32; o <<= 1) {
+      da[i] = f2_add(da[i], __shfl_xor_sync(0xffffffffu, da[i], o));
+      db[i] = f2_add(db[i], __shfl_xor_sync(0xffffffffu, db[i], o));
+    }
+    if (sub == 0 && on) {
+      *reinterpret_cast<float2*>(&sw[warp * p.D + a + 2 * i]) = f2_split(da[i]);
+      *reinterpret_cast<float2*>(&sw[warp * p.D + b + 2 * i]) = f2_split(db[i]);
+    }
+  }
+  __syncthreads();
+  for (int d = threadIdx.x; d < p.D; d += blockDim.x) {
+    float s = 0.0f;
+    for (int i = 0; i < warps; ++i) s += sw[i * p.D + d];
+    p.partial[static_cast<int64_t>(blockIdx.x) * p.D + d] = s;
+  }
+}
+
 __device__ __forceinline__ void store_as(void* p, int64_t at, int dtype, float v) {
   if (dtype == OJX_F32) static_cast<float*>(p)[at] = v;
   else if (dtype == OJX_BF16) static_cast<__nv_bfloat16*>(p)[at] = __float2bfloat16_rn(v);
   else static_cast<__half*>(p)[at] = __float2half_rn(v);
 }
 
-// dw of one side: its blocks' partial sums in block order.  grid (ceil(D / 32), 2),
-// 32 x 8 threads: eight interleaved runs of blocks, joined in order.
-__global__ void __launch_bounds__(256) qk_grad_weight_kernel(const float* partial, int q_blocks, int blocks, int D,
-                                                             void* dqw, void* dkw, int dtype) {
-  __shared__ float s[8][33];
+// dw of one side: its blocks' partial sums, in 32 interleaved runs of blocks joined in
+// order.  grid (ceil(D / 32), 2), 32 x 32 threads.
+__global__ void __launch_bounds__(1024) qk_grad_weight_kernel(const float* partial, int q_blocks, int blocks, int D, void* dqw, void* dkw,
+                                                              int dtype) {
+  __shared__ float s[32][33];
   const int d = blockIdx.x * 32 + threadIdx.x;
   void* out = blockIdx.y == 0 ? dqw : dkw;
   const int lo = blockIdx.y == 0 ? 0 : q_blocks, hi = blockIdx.y == 0 ? q_blocks : blocks;
   float v = 0.0f;
-  if (d < D)
-    for (int b = lo + threadIdx.y; b < hi; b += 8) v += partial[static_cast<int64_t>(b) * D + d];
+  if (d < D) {
+#pragma unroll 4
+    for (int b = lo + threadIdx.y; b < hi; b += 32) v += partial[static_cast<int64_t>(b) * D + d];
+  }
   s[threadIdx.y][threadIdx.x] = v;
   __syncthreads();
   if (threadIdx.y == 0 && d < D && out) {
 #pragma unroll
-    for (int i = 1; i < 8; ++i) v += s[i][threadIdx.x];
+    for (int i = 1; i < 32; ++i) v += s[i][threadIdx.x];
     store_as(out, d, dtype, v);
   }
 }
 
 // Rows of the cache at `slots` as dense [n][heads][D] keys and values; a skipped slot
-// gives zeros.  One thread reads eight elements of one row.
+// gives zeros.  A thread takes eight elements of a row's key and value, and of the rows
+// two, so four loads are in flight.
 template <typename T>
 __global__ void __launch_bounds__(256) kv_read_kernel(const ojx_kv_cache c, const void* slots, int slot64, int64_t n,
                                                       T* k_out, T* v_out) {
-  const int cpr = c.head_dim / 8;
-  const int64_t per = n * c.kv_heads * cpr;
-  const int64_t i = static_cast<int64_t>(blockIdx.x) * blockDim.x + threadIdx.x;
-  if (i >= 2 * per) return;
-  const bool is_v = i >= per;
-  const int64_t r = (is_v ? i - per : i) / cpr;
-  const int at = static_cast<int>((is_v ? i - per : i) % cpr) * 8;
-  const int64_t row = slot_row(c, load_index(slots, r / c.kv_heads, slot64), static_cast<int>(r % c.kv_heads));
-  float x[8];
+  const int cpr = c.head_dim / 8, per_block = 256 / cpr;  // rows that a block takes at a time
+  const int r0 = threadIdx.x / cpr, at = (threadIdx.x - r0 * cpr) * 8;
+  if (r0 >= per_block) return;
+  const int64_t rows = n * c.kv_heads;
+  const bool wide = ((reinterpret_cast<uintptr_t>(k_out) | reinterpret_cast<uintptr_t>(v_out)) & 31) == 0;
+  int64_t r[2], row[2];
+  uint4 k[2], v[2];
+  float ks[2], vs[2];
 #pragma unroll
-  for (int e = 0; e < 8; ++e) x[e] = 0.0f;
-  if (row >= 0) {
-    const void* base = is_v ? c.v : c.k;
-    const int64_t src = row * c.head_dim + at;
-    if (c.format == OJX_KV_BF16) {
-      load_chunk<__nv_bfloat16, 8>(static_cast<const __nv_bfloat16*>(base) + src, x);
-    } else if (c.format == OJX_KV_F16) {
-      load_chunk<__half, 8>(static_cast<const __half*>(base) + src, x);
-    } else {
-      const uint2 w = *reinterpret_cast<const uint2*>(static_cast<const uint8_t*>(base) + src);
-      const float step = (is_v ? c.v_scale : c.k_scale)[row];
-#pragma unroll
-      for (int e = 0; e < 8; ++e)
-        x[e] = dequantise_one(static_cast<uint8_t>((e < 4 ? w.x : w.y) >> (8 * (e & 3))), step, c.format);
+  for (int u = 0; u < 2; ++u) {
+    r[u] = (static_cast<int64_t>(blockIdx.x) * 2 + u) * per_block + r0;
+    row[u] = -1;
+    if (r[u] < rows) {
+      const int64_t token = r[u] / c.kv_heads;
+      row[u] = slot_row(c, load_index(slots, token, slot64), static_cast<int>(r[u] - token * c.kv_heads));
     }
   }
-  store_chunk<T, 8>((is_v ? v_out : k_out) + r * c.head_dim + at, x);
+#pragma unroll
+  for (int u = 0; u < 2; ++u) {
+    k[u] = v[u] = make_uint4(0, 0, 0, 0);
+    ks[u] = vs[u] = 0.0f;
+    if (row[u] < 0) continue;
+    const int64_t src = row[u] * c.head_dim + at;
+    if (c.format >= OJX_KV_INT8) {
+      const uint2 a = *reinterpret_cast<const uint2*>(static_cast<const uint8_t*>(c.k) + src);
+      const uint2 b = *reinterpret_cast<const uint2*>(static_cast<const uint8_t*>(c.v) + src);
+      k[u].x = a.x, k[u].y = a.y, v[u].x = b.x, v[u].y = b.y;
+      ks[u] = c.k_scale[row[u]];
+      vs[u] = c.v_scale[row[u]];
+    } else {
+      k[u] = *reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(c.k) + src);
+      v[u] = *reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(c.v) + src);
+    }
+  }
+#pragma unroll
+  for (int u = 0; u < 2; ++u) {
+    if (r[u] >= rows) continue;
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const uint4 w = h ? v[u] : k[u];
+      const float step = h ? vs[u] : ks[u];
+      uint64_t x[4];
+      if (c.format == OJX_KV_BF16) {
+        Eight<__nv_bfloat16> e;
+        e.v[0] = w;
+        e.pairs(x);
+      } else if (c.format == OJX_KV_F16) {
+        Eight<__half> e;
+        e.v[0] = w;
+        e.pairs(x);
+      } else {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const uint32_t two = (i < 2 ? w.x : w.y) >> (16 * (i & 1));
+          x[i] = f2_pair(dequantise_one(static_cast<uint8_t>(two), step, c.format), dequantise_one(static_cast<uint8_t>(two >> 8), step, c.format));
+        }
+        if (row[u] < 0) x[0] = x[1] = x[2] = x[3] = 0;
+      }
+      store_pairs<T>((h ? v_out : k_out) + r[u] * c.head_dim + at, x, wide);
+    }
+  }
 }
 
 // Moves the rows of the accepted nodes path[b][0..count[b]] of the drafts at context +

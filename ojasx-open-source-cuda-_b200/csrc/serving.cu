@@ -2,6 +2,7 @@
 // checks, launch shapes and workspaces.  A translation unit of its own, with its own
 // device error word, so that it compiles beside the GEMM kernels.
 #include <algorithm>
+#include <type_traits>
 #include "tmap.h"
 #include "qk_cache.cuh"
 #include "tree_attention.cuh"
@@ -76,7 +77,10 @@ static int launch_rows(QkParams& p, int dtype, bool vec, bool inter, cudaStream_
   p.npairs = p.D / (2 * CH);
   p.lanes = std::min(32, pow2_at_least(p.npairs));
   const int per_warp = 32 / p.lanes, heads = p.hq + p.hk + p.hv;
-  const int groups = (heads + per_warp - 1) / per_warp;
+  p.gq = (p.hq + per_warp - 1) / per_warp;
+  p.gk = (p.hk + per_warp - 1) / per_warp;
+  p.gv = (p.hv + per_warp - 1) / per_warp;
+  const int groups = vec ? p.gq + p.gk + p.gv : (heads + per_warp - 1) / per_warp;
   // One warp runs all heads of a token, so that the token's cosines are read once, unless
   // that leaves SMs without work: then its heads are split over more warps.
   const int64_t want = 16ll * current_props().sm_count;
@@ -91,8 +95,9 @@ static int launch_rows(QkParams& p, int dtype, bool vec, bool inter, cudaStream_
   return for_dtype(dtype, [&](auto t) {
     using T = decltype(t);
     const unsigned gr = static_cast<unsigned>(grid);
-    if (vec && !inter) qk_rows_kernel<T, 8, 1, false><<<gr, 256, 0, s>>>(p);
-    else if (vec) qk_rows_kernel<T, 8, 1, true><<<gr, 256, 0, s>>>(p);
+    if (vec && !p.norm) qk_rows_fast_kernel<T, false, false><<<gr, 256, 0, s>>>(p);
+    else if (vec && !inter) qk_rows_fast_kernel<T, false, true><<<gr, 256, 0, s>>>(p);
+    else if (vec) qk_rows_fast_kernel<T, true, true><<<gr, 256, 0, s>>>(p);
     else if (!inter) qk_rows_kernel<T, 1, 8, false><<<gr, 256, 0, s>>>(p);
     else qk_rows_kernel<T, 1, 8, true><<<gr, 256, 0, s>>>(p);
     return launched("qk_rows launch");
@@ -287,13 +292,15 @@ int ojx_qk_norm_rope_backward(const ojx_qk_desc* d, const ojx_rows* gq, const oj
   QkParams p = make_qk(d);
   const int es = dtype_size(d->dtype);
   bool vec = qk_vector(d) && aligned16(dq) && aligned16(dk);
-  if (gq) p.gq = gq->data, p.gq_st = gq->stride_t, p.gq_sh = gq->stride_h, vec = vec && vector_rows(*gq, es);
-  if (gk) p.gk = gk->data, p.gk_st = gk->stride_t, p.gk_sh = gk->stride_h, vec = vec && vector_rows(*gk, es);
+  if (gq) p.gq_data = gq->data, p.gq_st = gq->stride_t, p.gq_sh = gq->stride_h, vec = vec && vector_rows(*gq, es);
+  if (gk) p.gk_data = gk->data, p.gk_st = gk->stride_t, p.gk_sh = gk->stride_h, vec = vec && vector_rows(*gk, es);
   p.dq = dq;
   p.dk = dk;
   const bool inter = d->interleaved != 0;
   p.npairs = p.D / (vec ? 16 : 2);
   p.lanes = std::min(32, pow2_at_least(p.npairs));
+  p.gq = (p.hq + 32 / p.lanes - 1) / (32 / p.lanes);
+  p.gk = (p.hk + 32 / p.lanes - 1) / (32 / p.lanes);
   // Blocks in proportion to each side's heads, at most one warp per token of it.
   const int64_t most = 3ll * current_props().sm_count;
   auto blocks_of = [&](int heads) -> int64_t {
@@ -308,14 +315,14 @@ int ojx_qk_norm_rope_backward(const ojx_qk_desc* d, const ojx_rows* gq, const oj
   const int smem = 8 * p.D * 4;
   st = for_dtype(d->dtype, [&](auto t) {
     using T = decltype(t);
-    if (vec && !inter) qk_grad_kernel<T, 8, 1, false><<<blocks, 256, smem, s>>>(p);
-    else if (vec) qk_grad_kernel<T, 8, 1, true><<<blocks, 256, smem, s>>>(p);
+    if (vec && !inter) qk_grad_fast_kernel<T, false><<<blocks, 256, smem, s>>>(p);
+    else if (vec) qk_grad_fast_kernel<T, true><<<blocks, 256, smem, s>>>(p);
     else if (!inter) qk_grad_kernel<T, 1, 8, false><<<blocks, 256, smem, s>>>(p);
     else qk_grad_kernel<T, 1, 8, true><<<blocks, 256, smem, s>>>(p);
     return launched("qk_grad launch");
   });
   if (st || (!dqw && !dkw)) return st;
-  qk_grad_weight_kernel<<<dim3((p.D + 31) / 32, 2), dim3(32, 8), 0, s>>>(p.partial, p.q_blocks, blocks, p.D, dqw,
+  qk_grad_weight_kernel<<<dim3((p.D + 31) / 32, 2), dim3(32, 32), 0, s>>>(p.partial, p.q_blocks, blocks, p.D, dqw,
                                                                         dkw, d->dtype_weight);
   return launched("qk_grad_weight launch");
 }
@@ -354,8 +361,8 @@ int ojx_kv_read(const ojx_kv_cache* cache, void* k_out, void* v_out, int32_t dty
   if (!k_out || !v_out || !slots) return set_error(OJX_ERR_INVALID, "ojx_kv_read: NULL pointer");
   if (!aligned16(k_out) || !aligned16(v_out))
     return set_error(OJX_ERR_INVALID, "ojx_kv_read: outputs must be 16-byte aligned");
-  const int64_t threads = 2 * n * cache->kv_heads * (cache->head_dim / 8);
-  const int64_t grid = (threads + 255) / 256;
+  const int64_t per_block = 2 * (256 / (cache->head_dim / 8));
+  const int64_t grid = (n * cache->kv_heads + per_block - 1) / per_block;
   if (grid > INT32_MAX) return set_error(OJX_ERR_INVALID, "ojx_kv_read: too many rows for one call");
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   return for_dtype(dtype, [&](auto t) {
