@@ -123,7 +123,7 @@ struct QkParams {
   int hq, hk, hv, blocks_per_token, iters;
   int gq, gk, gv;  // row groups (of 32 / lanes heads) of each side
   int dtype_w, pos64, slot64, k_to_cache;
-  float eps;
+  float eps, inv_dim;
   const void *q, *k, *v;
   int64_t q_st, q_sh, k_st, k_sh, v_st, v_sh;
   const void *qw, *kw;
@@ -585,13 +585,18 @@ __device__ __forceinline__ void load_weight(const void* w, int at, int dtype, bo
   for (int i = 0; i < 4; ++i) x[i] = f2_pair(v[2 * i], v[2 * i + 1]);
 }
 
+__device__ __forceinline__ bool table_aligned(const QkParams& p) {
+  return ((p.rotary & 7) | (reinterpret_cast<uintptr_t>(p.table) & 15)) == 0;
+}
+
 // The turn of a chunk pair (a, b), in pairs of elements.  Halves: (c, s) of elements 2 i,
 // 2 i + 1, the same for both chunks.  Interleaved: element pairs turn on themselves,
 // (c, c) and (-s, s), each chunk with its own four.
 template <bool INTER>
 struct Turn {
-  uint64_t c[INTER ? 8 : 4], s[INTER ? 8 : 4];
-  __device__ __forceinline__ void load(const QkParams& p, int64_t pos, bool known, bool turns, int a) {
+  uint64_t c[INTER ? 8 : 4], s[INTER ? 8 : 4], n[INTER ? 1 : 4];  // (n: -s)
+  // row: the position's cosines, its sines `half` further on.
+  __device__ __forceinline__ void load(const float* table_row, int half, bool aligned, bool known, bool turns, int a) {
     float cs[8], sn[8];
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
@@ -599,11 +604,11 @@ struct Turn {
       sn[e] = 0.0f;
     }
     if (turns && known) {
-      const float* row = p.table + pos * p.rotary + (INTER ? a / 2 : a);
-      if (((p.rotary & 7) | (reinterpret_cast<uintptr_t>(p.table) & 15)) == 0) {
+      const float* row = table_row + (INTER ? a / 2 : a);
+      if (aligned) {
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
-          const float4 x = reinterpret_cast<const float4*>(row)[h], y = reinterpret_cast<const float4*>(row + p.half)[h];
+          const float4 x = reinterpret_cast<const float4*>(row)[h], y = reinterpret_cast<const float4*>(row + half)[h];
           cs[4 * h] = x.x, cs[4 * h + 1] = x.y, cs[4 * h + 2] = x.z, cs[4 * h + 3] = x.w;
           sn[4 * h] = y.x, sn[4 * h + 1] = y.y, sn[4 * h + 2] = y.z, sn[4 * h + 3] = y.w;
         }
@@ -611,7 +616,7 @@ struct Turn {
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
           cs[e] = row[e];
-          sn[e] = row[p.half + e];
+          sn[e] = row[half + e];
         }
       }
     }
@@ -626,13 +631,14 @@ struct Turn {
       for (int i = 0; i < 4; ++i) {
         c[i] = f2_pair(cs[2 * i], cs[2 * i + 1]);
         s[i] = f2_pair(sn[2 * i], sn[2 * i + 1]);
+        n[i] = f2_pair(-sn[2 * i], -sn[2 * i + 1]);
       }
     }
   }
   // SIGN 1: by the angle, -1: back.
   template <int SIGN>
   __device__ __forceinline__ void apply(uint64_t (&a)[4], uint64_t (&b)[4]) const {
-    const uint64_t minus = f2_pair(-1.0f, -1.0f);
+    [[maybe_unused]] const uint64_t minus = f2_pair(-1.0f, -1.0f);
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       if constexpr (INTER) {
@@ -640,10 +646,9 @@ struct Turn {
         a[i] = f2_fma(f2_swap(a[i]), sa, f2_mul(a[i], c[i]));
         b[i] = f2_fma(f2_swap(b[i]), sb, f2_mul(b[i], c[4 + i]));
       } else {
-        const uint64_t n = f2_mul(s[i], minus);
         const uint64_t u = a[i], v = b[i];
-        a[i] = f2_fma(v, SIGN > 0 ? n : s[i], f2_mul(u, c[i]));
-        b[i] = f2_fma(u, SIGN > 0 ? s[i] : n, f2_mul(v, c[i]));
+        a[i] = f2_fma(v, SIGN > 0 ? n[i] : s[i], f2_mul(u, c[i]));
+        b[i] = f2_fma(u, SIGN > 0 ? s[i] : n[i], f2_mul(v, c[i]));
       }
     }
   }
@@ -654,12 +659,57 @@ __device__ __forceinline__ float f2_total(uint64_t v) {
   return a.x + a.y;
 }
 
+// What is done with a row pair of chunks once it is in registers.  out: where the row goes
+// if it is not cached; h: its head.
+template <typename T, bool INTER>
+__device__ __forceinline__ void norm_turn(const QkParams& p, const Turn<INTER>& turn, const uint64_t (&wa)[4], const uint64_t (&wb)[4],
+                                          uint64_t (&xa)[4], uint64_t (&xb)[4]) {
+  uint64_t ss = f2_mul(xa[0], xa[0]), tt = f2_mul(xb[0], xb[0]);
+#pragma unroll
+  for (int i = 1; i < 4; ++i) {
+    ss = f2_fma(xa[i], xa[i], ss);
+    tt = f2_fma(xb[i], xb[i], tt);
+  }
+  const float r = rsqrtf(fmaf(group_sum(f2_total(f2_add(ss, tt)), p.lanes), p.inv_dim, p.eps));
+  const uint64_t r2 = f2_pair(r, r);
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    xa[i] = f2_mul(f2_mul(xa[i], r2), wa[i]);
+    xb[i] = f2_mul(f2_mul(xb[i], r2), wb[i]);
+  }
+  turn.template apply<1>(xa, xb);
+}
+__device__ __forceinline__ void cache_row(const QkParams& p, int64_t slot, bool is_k, int h, bool valid, bool on, int j, int a, int b,
+                                          const uint64_t (&xa)[4], const uint64_t (&xb)[4]) {
+  float va[8], vb[8];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const float2 u = f2_split(xa[i]), v = f2_split(xb[i]);
+    va[2 * i] = u.x, va[2 * i + 1] = u.y, vb[2 * i] = v.x, vb[2 * i + 1] = v.y;
+  }
+  float step = 0.0f;
+  if (p.cache.format >= OJX_KV_INT8) {
+    float amax = 0.0f;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) amax = max_nan(amax, max_nan(fabsf(va[e]), fabsf(vb[e])));
+    for (int o = p.lanes >> 1; o > 0; o >>= 1) amax = max_nan(amax, __shfl_xor_sync(0xffffffffu, amax, o));
+    step = quantise_step(amax, p.cache.format);
+  }
+  const int64_t row = valid ? slot_row(p.cache, slot, h) : -1;
+  if (row >= 0 && on) {
+    void* base = is_k ? p.cache.k : p.cache.v;
+    if (p.cache.format >= OJX_KV_INT8 && j == 0) (is_k ? p.cache.k_scale : p.cache.v_scale)[row] = step;
+    store_cached<8>(base, row * p.D + a, p.cache.format, step, va);
+    store_cached<8>(base, row * p.D + b, p.cache.format, step, vb);
+  }
+}
+
 // Forward rows in 16-byte chunks.  A group is 32 / lanes heads of one side (queries, keys,
 // values) of a token; a warp runs p.iters groups of one token with the next two groups'
 // loads in flight: at 16 warps an SM that covers HBM's latency.  One group at a time took
 // 116 us for 16384 tokens of 40 bf16 heads of 128.
 template <typename T, bool INTER, bool NORM>
-__global__ void __launch_bounds__(256, NORM ? 2 : 3) qk_rows_fast_kernel(const QkParams p) {
+__global__ void __launch_bounds__(256, 2) qk_rows_fast_kernel(const QkParams p) {
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int sub = lane / p.lanes, j = lane % p.lanes, per_warp = 32 / p.lanes;
   const int64_t item = static_cast<int64_t>(blockIdx.x) * (blockDim.x >> 5) + warp;
@@ -695,7 +745,7 @@ __global__ void __launch_bounds__(256, NORM ? 2 : 3) qk_rows_fast_kernel(const Q
     const int64_t pos = load_index(p.positions, token, p.pos64);
     const bool known = pos >= 0 && pos < p.table_rows;
     if (!known && lane == 0) index_error();
-    turn.load(p, pos, known, turns, a);
+    turn.load(p.table + (known ? pos : 0) * p.rotary, p.half, table_aligned(p), known, turns, a);
   }
   const int64_t slot = p.slots ? load_index(p.slots, token, p.slot64) : -1;
   const bool wide_q = (reinterpret_cast<uintptr_t>(p.q_out) & 31) == 0, wide_k = (reinterpret_cast<uintptr_t>(p.k_out) & 31) == 0;
@@ -717,19 +767,7 @@ __global__ void __launch_bounds__(256, NORM ? 2 : 3) qk_rows_fast_kernel(const Q
         load_weight(is_q ? p.qw : p.kw, a, p.dtype_w, on, wa);
         load_weight(is_q ? p.qw : p.kw, b, p.dtype_w, on, wb);
       }
-      uint64_t ss = f2_mul(xa[0], xa[0]);
-#pragma unroll
-      for (int i = 1; i < 4; ++i) ss = f2_fma(xa[i], xa[i], ss);
-#pragma unroll
-      for (int i = 0; i < 4; ++i) ss = f2_fma(xb[i], xb[i], ss);
-      const float r = rsqrtf(group_sum(f2_total(ss), p.lanes) / p.D + p.eps);
-      const uint64_t r2 = f2_pair(r, r);
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        xa[i] = f2_mul(f2_mul(xa[i], r2), wa[i]);
-        xb[i] = f2_mul(f2_mul(xb[i], r2), wb[i]);
-      }
-      turn.template apply<1>(xa, xb);
+      norm_turn<T, INTER>(p, turn, wa, wb, xa, xb);
     }
     if (is_q || (is_k && !p.k_to_cache)) {
       if (valid && on) {
@@ -738,27 +776,67 @@ __global__ void __launch_bounds__(256, NORM ? 2 : 3) qk_rows_fast_kernel(const Q
         store_pairs<T>(out + b, xb, is_q ? wide_q : wide_k);
       }
     } else {
-      float va[8], vb[8], amax = 0.0f;
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const float2 u = f2_split(xa[i]), v = f2_split(xb[i]);
-        va[2 * i] = u.x, va[2 * i + 1] = u.y, vb[2 * i] = v.x, vb[2 * i + 1] = v.y;
-      }
-      float step = 0.0f;
-      if (p.cache.format >= OJX_KV_INT8) {
-#pragma unroll
-        for (int e = 0; e < 8; ++e) amax = max_nan(amax, max_nan(fabsf(va[e]), fabsf(vb[e])));
-        for (int o = p.lanes >> 1; o > 0; o >>= 1) amax = max_nan(amax, __shfl_xor_sync(0xffffffffu, amax, o));
-        step = quantise_step(amax, p.cache.format);
-      }
-      const int64_t row = valid ? slot_row(p.cache, slot, h) : -1;
-      if (row >= 0 && on) {
-        void* base = is_k ? p.cache.k : p.cache.v;
-        if (p.cache.format >= OJX_KV_INT8 && j == 0) (is_k ? p.cache.k_scale : p.cache.v_scale)[row] = step;
-        store_cached<8>(base, row * p.D + a, p.cache.format, step, va);
-        store_cached<8>(base, row * p.D + b, p.cache.format, step, vb);
-      }
+      cache_row(p, slot, is_k, h, valid, on, j, a, b, xa, xb);
     }
+  }
+}
+
+// A block's sum of dw: rows of a warp, then warps, in a fixed order.  sw: [warps][D].
+__device__ __forceinline__ void grad_weight_sums(const QkParams& p, float* sw, bool store, int a, int b, uint64_t (&da)[4],
+                                                 uint64_t (&db)[4]) {
+  const int warp = threadIdx.x >> 5, warps = blockDim.x >> 5;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    for (int o = p.lanes; o < 32; o <<= 1) {
+      da[i] = f2_add(da[i], __shfl_xor_sync(0xffffffffu, da[i], o));
+      db[i] = f2_add(db[i], __shfl_xor_sync(0xffffffffu, db[i], o));
+    }
+    if (store) {
+      *reinterpret_cast<float2*>(&sw[warp * p.D + a + 2 * i]) = f2_split(da[i]);
+      *reinterpret_cast<float2*>(&sw[warp * p.D + b + 2 * i]) = f2_split(db[i]);
+    }
+  }
+  __syncthreads();
+  for (int d = threadIdx.x; d < p.D; d += blockDim.x) {
+    float s = 0.0f;
+    for (int i = 0; i < warps; ++i) s += sw[i * p.D + d];
+    p.partial[static_cast<int64_t>(blockIdx.x) * p.D + d] = s;
+  }
+}
+
+template <typename T, bool INTER>
+__device__ __forceinline__ void grad_group(const QkParams& p, bool store, T* dx, int a, int b, bool wide, const Turn<INTER>& turn,
+                                           const uint64_t (&wa)[4], const uint64_t (&wb)[4], const uint64_t (&xa)[4],
+                                           const uint64_t (&xb)[4], uint64_t (&ga)[4], uint64_t (&gb)[4], uint64_t (&da)[4],
+                                           uint64_t (&db)[4]) {
+  turn.template apply<-1>(ga, gb);
+  uint64_t ss = 0, hx = 0;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    ss = f2_fma(xa[i], xa[i], ss);
+    ss = f2_fma(xb[i], xb[i], ss);
+    hx = f2_fma(f2_mul(ga[i], wa[i]), xa[i], hx);
+    hx = f2_fma(f2_mul(gb[i], wb[i]), xb[i], hx);
+  }
+  float s1 = f2_total(ss), s2 = f2_total(hx);
+  for (int o = p.lanes >> 1; o > 0; o >>= 1) {
+    s1 += __shfl_xor_sync(0xffffffffu, s1, o);
+    s2 += __shfl_xor_sync(0xffffffffu, s2, o);
+  }
+  const float r = rsqrtf(fmaf(s1, p.inv_dim, p.eps));
+  const float back = -(r * r * s2 * p.inv_dim);
+  const uint64_t r2 = f2_pair(r, r), back2 = f2_pair(back, back);
+  if (store) {
+    uint64_t oa[4], ob[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      oa[i] = f2_mul(f2_fma(xa[i], back2, f2_mul(ga[i], wa[i])), r2);
+      ob[i] = f2_mul(f2_fma(xb[i], back2, f2_mul(gb[i], wb[i])), r2);
+      da[i] = f2_fma(ga[i], f2_mul(xa[i], r2), da[i]);
+      db[i] = f2_fma(gb[i], f2_mul(xb[i], r2), db[i]);
+    }
+    store_pairs<T>(dx + a, oa, wide);
+    store_pairs<T>(dx + b, ob, wide);
   }
 }
 
@@ -812,7 +890,7 @@ __global__ void __launch_bounds__(256, 2) qk_grad_fast_kernel(const QkParams p) 
     const int64_t pos = load_index(p.positions, token, p.pos64);
     const bool known = pos >= 0 && pos < p.table_rows;
     if (!known && lane == 0) index_error();
-    turn.load(p, pos, known, turns, a);
+    turn.load(p.table + (known ? pos : 0) * p.rotary, p.half, table_aligned(p), known, turns, a);
     for (int rg = 0; rg < groups; ++rg) {
       const int h = rg * per_warp + sub;
       uint64_t xa[4], xb[4], ga[4], gb[4];
@@ -821,56 +899,281 @@ __global__ void __launch_bounds__(256, 2) qk_grad_fast_kernel(const QkParams p) 
       sa.pairs(ga);
       sb.pairs(gb);
       fetch();
-      turn.template apply<-1>(ga, gb);
-      uint64_t ss = 0, hx = 0;
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        ss = f2_fma(xa[i], xa[i], ss);
-        ss = f2_fma(xb[i], xb[i], ss);
-        hx = f2_fma(f2_mul(ga[i], wa[i]), xa[i], hx);
-        hx = f2_fma(f2_mul(gb[i], wb[i]), xb[i], hx);
-      }
-      float s1 = f2_total(ss), s2 = f2_total(hx);
-      for (int o = p.lanes >> 1; o > 0; o >>= 1) {
-        s1 += __shfl_xor_sync(0xffffffffu, s1, o);
-        s2 += __shfl_xor_sync(0xffffffffu, s2, o);
-      }
-      const float r = rsqrtf(s1 / p.D + p.eps);
-      const float back = -(r * r * s2 / p.D);
-      const uint64_t r2 = f2_pair(r, r), back2 = f2_pair(back, back);
-      if (h < heads && on) {
-        T* dx = dxs + (token * heads + h) * p.D;
-        uint64_t oa[4], ob[4];
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          oa[i] = f2_mul(f2_fma(xa[i], back2, f2_mul(ga[i], wa[i])), r2);
-          ob[i] = f2_mul(f2_fma(xb[i], back2, f2_mul(gb[i], wb[i])), r2);
-          da[i] = f2_fma(ga[i], f2_mul(xa[i], r2), da[i]);
-          db[i] = f2_fma(gb[i], f2_mul(xb[i], r2), db[i]);
-        }
-        store_pairs<T>(dx + a, oa, wide);
-        store_pairs<T>(dx + b, ob, wide);
-      }
+      grad_group<T, INTER>(p, h < heads && on, dxs + (token * heads + h) * p.D, a, b, wide, turn, wa, wb, xa, xb, ga, gb, da, db);
     }
   }
-  // rows of the warp, then warps of the block, in a fixed order
+  grad_weight_sums(p, sw, sub == 0 && on, a, b, da, db);
+}
+
+// ── rows streamed through shared memory ─────────────────────────────────────────
+// With many tokens whose heads lie side by side, a warp takes an equal run of all groups
+// and keeps a ring of them in flight: one bulk copy a group (its rows are one piece of
+// memory) into the warp's own ring, and with a token's first group the position's row of
+// the table.  A group is two rows a lane (float32: one): what is done once a group, the
+// wait, the next copy and the addresses, then weighs half as much, and instructions are
+// what bounds these kernels once the loads are ahead.
+template <typename T>
+inline constexpr int qk_rows_per_lane = sizeof(T) == 4 ? 1 : 2;
+constexpr int QK_RING = 4, QK_GRAD_RING = 2;
+
+struct StreamAt {  // the group that is issued, or used, next
+  int u, token, g;
+  __device__ __forceinline__ void begin(int first, int groups) {
+    u = first;
+    token = first / groups;
+    g = first - token * groups;
+  }
+  __device__ __forceinline__ bool next(int groups) {  // true: a new token
+    ++u;
+    if (++g < groups) return false;
+    g = 0;
+    ++token;
+    return true;
+  }
+};
+
+// Both weights as float32 in shared memory: [2][D].
+__device__ __forceinline__ void stage_weights(const QkParams& p, float* sw) {
+  for (int i = threadIdx.x; i < 2 * p.D; i += blockDim.x) {
+    const void* w = i < p.D ? p.qw : p.kw;
+    float v[1] = {1.0f};
+    if (w) load_chunk_as<1>(w, i < p.D ? i : i - p.D, p.dtype_w, v);
+    sw[i] = v[0];
+  }
+}
+__device__ __forceinline__ void staged_weight(const float* w, bool on, uint64_t (&x)[4]) {
+  if (!on) return;
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    for (int o = p.lanes; o < 32; o <<= 1) {
-      da[i] = f2_add(da[i], __shfl_xor_sync(0xffffffffu, da[i], o));
-      db[i] = f2_add(db[i], __shfl_xor_sync(0xffffffffu, db[i], o));
+  for (int h = 0; h < 2; ++h) {
+    const ulonglong2 v = reinterpret_cast<const ulonglong2*>(w)[h];
+    x[2 * h] = v.x;
+    x[2 * h + 1] = v.y;
+  }
+}
+
+template <typename T, bool INTER, bool NORM>
+__global__ void __launch_bounds__(256, 2) qk_rows_stream_kernel(const QkParams p, int slot_bytes, uint64_t budget) {
+  constexpr int RPL = qk_rows_per_lane<T>;
+  extern __shared__ __align__(128) uint8_t smem[];  // [8 warps][QK_RING][group | table row], then both weights
+  __shared__ __align__(8) uint64_t bars[8 * QK_RING];
+  __shared__ int s_known[8 * QK_RING], s_abort;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int sub = lane / p.lanes, j = lane % p.lanes, per_warp = 32 / p.lanes;
+  const int groups = p.gq + p.gk + p.gv;
+  const int group_bytes = RPL * per_warp * p.D * static_cast<int>(sizeof(T));
+  const uint32_t bar = smem_u32(&bars[warp * QK_RING]);
+  uint8_t* ring = smem + warp * QK_RING * slot_bytes;
+  const float* sw = reinterpret_cast<const float*>(smem + 8 * QK_RING * slot_bytes);
+  if (lane < QK_RING) mbar_init(bar + 8 * lane, 1);
+  if (threadIdx.x == 0) s_abort = 0;
+  if (NORM) stage_weights(p, reinterpret_cast<float*>(smem + 8 * QK_RING * slot_bytes));
+  fence_mbar_init();
+  __syncthreads();
+
+  const long long total = p.tokens * groups, warps = static_cast<long long>(gridDim.x) * 8, w = static_cast<long long>(blockIdx.x) * 8 + warp;
+  const int first = static_cast<int>(total * w / warps), end = static_cast<int>(total * (w + 1) / warps);
+  StreamAt in, at;
+  in.begin(first, groups);
+  at = in;
+  // (positions are read a token ahead of the copy that needs them)
+  int64_t pos = NORM && first < end ? load_index(p.positions, in.token, p.pos64) : 0;
+  int in_slot = 0;
+  auto issue = [&]() {
+    if (in.u >= end) return;
+    if (lane == 0) {
+      const bool is_q = in.g < p.gq, is_k = !is_q && in.g < p.gq + p.gk;
+      const int h = (in.g - (is_q ? 0 : is_k ? p.gq : p.gq + p.gk)) * (RPL * per_warp);
+      const int rows = min(RPL * per_warp, (is_q ? p.hq : is_k ? p.hk : p.hv) - h);
+      const bool fresh = NORM && (in.g == 0 || in.u == first), known = pos >= 0 && pos < p.table_rows;
+      const T* x = static_cast<const T*>(is_q ? p.q : is_k ? p.k : p.v) + in.token * (is_q ? p.q_st : is_k ? p.k_st : p.v_st);
+      const uint32_t dst = smem_u32(ring + in_slot * slot_bytes), full = bar + 8 * in_slot;
+      const uint32_t bytes = rows * p.D * sizeof(T), row = fresh && known ? p.rotary * 4 : 0;
+      mbar_arrive_expect_tx(full, bytes + row);
+      bulk_load_g2s(dst, x + h * p.D, bytes, full);
+      if (fresh) {
+        if (!known) index_error();
+        s_known[warp * QK_RING + in_slot] = known;
+        if (row) bulk_load_g2s(dst + group_bytes, p.table + pos * p.rotary, row, full);
+      }
     }
-    if (sub == 0 && on) {
-      *reinterpret_cast<float2*>(&sw[warp * p.D + a + 2 * i]) = f2_split(da[i]);
-      *reinterpret_cast<float2*>(&sw[warp * p.D + b + 2 * i]) = f2_split(db[i]);
+    if (in.next(groups) && NORM && in.u < end) pos = load_index(p.positions, in.token, p.pos64);
+    in_slot = in_slot + 1 == QK_RING ? 0 : in_slot + 1;
+  };
+#pragma unroll 1
+  for (int i = 0; i < QK_RING; ++i) issue();
+
+  const bool on = j < p.npairs;
+  int a = 0, b = 0;
+  const bool turns = on && pair_at<8, INTER>(p, j, a, b);
+  const bool wide_q = (reinterpret_cast<uintptr_t>(p.q_out) & 31) == 0, wide_k = (reinterpret_cast<uintptr_t>(p.k_out) & 31) == 0;
+  Turn<INTER> turn;
+  uint64_t wa[4] = {0, 0, 0, 0}, wb[4] = {0, 0, 0, 0};
+  int slot_at = 0;
+  uint32_t phase = 0;
+  int64_t slot = -1;
+  while (at.u < end) {
+    const bool is_q = at.g < p.gq, is_k = !is_q && at.g < p.gq + p.gk, fresh = at.g == 0 || at.u == first;
+    const int h0 = (at.g - (is_q ? 0 : is_k ? p.gq : p.gq + p.gk)) * (RPL * per_warp) + sub, heads = is_q ? p.hq : is_k ? p.hk : p.hv;
+    if (fresh && p.slots) slot = load_index(p.slots, at.token, p.slot64);
+    if (NORM && (fresh || at.g == p.gq)) {  // the side changes
+      staged_weight(sw + (is_q ? a : p.D + a), on, wa);
+      staged_weight(sw + (is_q ? b : p.D + b), on, wb);
     }
+    if (!__all_sync(0xffffffffu, mbar_wait(bar + 8 * slot_at, phase, budget, &s_abort))) break;
+    const uint8_t* src = ring + slot_at * slot_bytes;
+    if (NORM && fresh)
+      turn.load(reinterpret_cast<const float*>(src + group_bytes), p.half, (p.rotary & 7) == 0, s_known[warp * QK_RING + slot_at] != 0, turns, a);
+    Eight<T> ra[RPL], rb[RPL];
+#pragma unroll
+    for (int r = 0; r < RPL; ++r) {
+      ra[r].clear();
+      rb[r].clear();
+      if (h0 + r * per_warp < heads && on) {
+        const T* x = reinterpret_cast<const T*>(src) + (sub + r * per_warp) * p.D;
+        ra[r].load(x + a);
+        rb[r].load(x + b);
+      }
+    }
+    uint64_t xa[RPL][4], xb[RPL][4];
+#pragma unroll
+    for (int r = 0; r < RPL; ++r) {
+      ra[r].pairs(xa[r]);
+      rb[r].pairs(xb[r]);
+    }
+    __syncwarp();  // the slot is read
+    issue();
+    if (is_q || (is_k && !p.k_to_cache)) {
+      T* out = static_cast<T*>(is_q ? p.q_out : p.k_out) + static_cast<int64_t>(at.token) * (heads * p.D) + h0 * p.D;
+#pragma unroll
+      for (int r = 0; r < RPL; ++r) {
+        if (NORM) norm_turn<T, INTER>(p, turn, wa, wb, xa[r], xb[r]);
+        if (h0 + r * per_warp < heads && on) {
+          store_pairs<T>(out + r * per_warp * p.D + a, xa[r], is_q ? wide_q : wide_k);
+          store_pairs<T>(out + r * per_warp * p.D + b, xb[r], is_q ? wide_q : wide_k);
+        }
+      }
+    } else {
+#pragma unroll
+      for (int r = 0; r < RPL; ++r) {
+        if (NORM && is_k) norm_turn<T, INTER>(p, turn, wa, wb, xa[r], xb[r]);
+        cache_row(p, slot, is_k, h0 + r * per_warp, h0 + r * per_warp < heads, on, j, a, b, xa[r], xb[r]);
+      }
+    }
+    at.next(groups);
+    if (++slot_at == QK_RING) slot_at = 0, phase ^= 1;
+  }
+  // (after a wait that ran out: let the copies in flight land before the block may exit)
+  for (; at.u < in.u; at.next(groups)) {
+    mbar_wait_drain(bar + 8 * slot_at, phase, budget);
+    if (++slot_at == QK_RING) slot_at = 0, phase ^= 1;
+  }
+}
+
+template <typename T, bool INTER>
+__global__ void __launch_bounds__(256, 2) qk_grad_stream_kernel(const QkParams p, int slot_bytes, uint64_t budget) {
+  constexpr int RPL = qk_rows_per_lane<T>, RING = QK_GRAD_RING;
+  extern __shared__ __align__(128) uint8_t smem[];  // [8 warps][RING][rows | gradients | table row]; at the end [8][D] sums
+  __shared__ __align__(8) uint64_t bars[8 * RING];
+  __shared__ int s_known[8 * RING], s_abort;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int sub = lane / p.lanes, j = lane % p.lanes, per_warp = 32 / p.lanes;
+  const bool is_q = blockIdx.x < p.q_blocks;
+  const int block = is_q ? blockIdx.x : blockIdx.x - p.q_blocks;
+  const int blocks = is_q ? p.q_blocks : gridDim.x - p.q_blocks;
+  const int heads = is_q ? p.hq : p.hk, groups = is_q ? p.gq : p.gk;
+  const T* xs = static_cast<const T*>(is_q ? p.q : p.k);
+  const T* gs = static_cast<const T*>(is_q ? p.gq_data : p.gk_data);
+  T* dxs = static_cast<T*>(is_q ? p.dq : p.dk);
+  const int64_t x_st = is_q ? p.q_st : p.k_st, g_st = is_q ? p.gq_st : p.gk_st;
+  const int group_bytes = RPL * per_warp * p.D * static_cast<int>(sizeof(T));
+  const uint32_t bar = smem_u32(&bars[warp * RING]);
+  uint8_t* ring = smem + warp * RING * slot_bytes;
+  if (lane < RING) mbar_init(bar + 8 * lane, 1);
+  if (threadIdx.x == 0) s_abort = 0;
+  fence_mbar_init();
+  __syncthreads();
+
+  const long long total = p.tokens * groups, warps = static_cast<long long>(blocks) * 8, w = static_cast<long long>(block) * 8 + warp;
+  const int first = static_cast<int>(total * w / warps), end = static_cast<int>(total * (w + 1) / warps);
+  StreamAt in, at;
+  in.begin(first, groups);
+  at = in;
+  int64_t pos = first < end ? load_index(p.positions, in.token, p.pos64) : 0;
+  int in_slot = 0;
+  auto issue = [&]() {
+    if (in.u >= end) return;
+    if (lane == 0) {
+      const int h = in.g * (RPL * per_warp), rows = min(RPL * per_warp, heads - h);
+      const bool fresh = in.g == 0 || in.u == first, known = pos >= 0 && pos < p.table_rows;
+      const uint32_t dst = smem_u32(ring + in_slot * slot_bytes), full = bar + 8 * in_slot;
+      const uint32_t bytes = rows * p.D * sizeof(T), row = fresh && known ? p.rotary * 4 : 0;
+      mbar_arrive_expect_tx(full, 2 * bytes + row);
+      bulk_load_g2s(dst, xs + in.token * x_st + h * p.D, bytes, full);
+      bulk_load_g2s(dst + group_bytes, gs + in.token * g_st + h * p.D, bytes, full);
+      if (fresh) {
+        if (!known) index_error();
+        s_known[warp * RING + in_slot] = known;
+        if (row) bulk_load_g2s(dst + 2 * group_bytes, p.table + pos * p.rotary, row, full);
+      }
+    }
+    if (in.next(groups) && in.u < end) pos = load_index(p.positions, in.token, p.pos64);
+    in_slot = in_slot + 1 == RING ? 0 : in_slot + 1;
+  };
+#pragma unroll 1
+  for (int i = 0; i < RING; ++i) issue();
+
+  const bool wide = (reinterpret_cast<uintptr_t>(dxs) & 31) == 0;
+  const bool on = j < p.npairs;
+  int a = 0, b = 0;
+  const bool turns = on && pair_at<8, INTER>(p, j, a, b);
+  uint64_t wa[4], wb[4], da[4], db[4];
+  load_weight(is_q ? p.qw : p.kw, a, p.dtype_w, on, wa);
+  load_weight(is_q ? p.qw : p.kw, b, p.dtype_w, on, wb);
+#pragma unroll
+  for (int i = 0; i < 4; ++i) da[i] = db[i] = 0;
+  Turn<INTER> turn;
+  int slot_at = 0;
+  uint32_t phase = 0;
+  while (at.u < end) {
+    const int h0 = at.g * (RPL * per_warp) + sub;
+    if (!__all_sync(0xffffffffu, mbar_wait(bar + 8 * slot_at, phase, budget, &s_abort))) break;
+    const uint8_t* src = ring + slot_at * slot_bytes;
+    if (at.g == 0 || at.u == first)
+      turn.load(reinterpret_cast<const float*>(src + 2 * group_bytes), p.half, (p.rotary & 7) == 0, s_known[warp * RING + slot_at] != 0, turns, a);
+    T* dx = dxs + static_cast<int64_t>(at.token) * (heads * p.D) + h0 * p.D;
+#pragma unroll
+    for (int r = 0; r < RPL; ++r) {
+      const bool mine = h0 + r * per_warp < heads && on;
+      Eight<T> ra, rb, ga_, gb_;
+      ra.clear(), rb.clear(), ga_.clear(), gb_.clear();
+      if (mine) {
+        const T* x = reinterpret_cast<const T*>(src) + (sub + r * per_warp) * p.D;
+        const T* g = reinterpret_cast<const T*>(src + group_bytes) + (sub + r * per_warp) * p.D;
+        ra.load(x + a);
+        rb.load(x + b);
+        ga_.load(g + a);
+        gb_.load(g + b);
+      }
+      uint64_t xa[4], xb[4], ga[4], gb[4];
+      ra.pairs(xa);
+      rb.pairs(xb);
+      ga_.pairs(ga);
+      gb_.pairs(gb);
+      if (r == RPL - 1) {
+        __syncwarp();  // the slot is read
+        issue();
+      }
+      grad_group<T, INTER>(p, mine, dx + r * per_warp * p.D, a, b, wide, turn, wa, wb, xa, xb, ga, gb, da, db);
+    }
+    at.next(groups);
+    if (++slot_at == RING) slot_at = 0, phase ^= 1;
+  }
+  for (; at.u < in.u; at.next(groups)) {
+    mbar_wait_drain(bar + 8 * slot_at, phase, budget);
+    if (++slot_at == RING) slot_at = 0, phase ^= 1;
   }
   __syncthreads();
-  for (int d = threadIdx.x; d < p.D; d += blockDim.x) {
-    float s = 0.0f;
-    for (int i = 0; i < warps; ++i) s += sw[i * p.D + d];
-    p.partial[static_cast<int64_t>(blockIdx.x) * p.D + d] = s;
-  }
+  grad_weight_sums(p, reinterpret_cast<float*>(smem), sub == 0 && on, a, b, da, db);
 }
 
 __device__ __forceinline__ void store_as(void* p, int64_t at, int dtype, float v) {

@@ -71,6 +71,9 @@ static int for_dtype(int dtype, F f) {
   return f(__half{});
 }
 
+// Whether a token's heads lie side by side, so that a group of rows is one copy.
+static bool side_by_side(int64_t stride_h, int D, int heads) { return heads <= 1 || stride_h == D; }
+
 static int launch_rows(QkParams& p, int dtype, bool vec, bool inter, cudaStream_t s) {
   if (p.tokens == 0) return OJX_OK;
   const int CH = vec ? 8 : 1;
@@ -89,6 +92,31 @@ static int launch_rows(QkParams& p, int dtype, bool vec, bool inter, cudaStream_
   split = std::min(split, groups);
   p.iters = (groups + split - 1) / split;
   p.blocks_per_token = (groups + p.iters - 1) / p.iters;
+  // Streaming wants every warp to have a ring's worth of groups several times over: from 4
+  // tokens a warp it is the faster form (prefetching in registers: the other).
+  const int sms = current_props().sm_count;
+  const bool table_ok = !p.norm || (aligned16(p.table) && p.rotary % 4 == 0);
+  if (vec && table_ok && p.tokens >= 16ll * sms && side_by_side(p.q_sh, p.D, p.hq) && side_by_side(p.k_sh, p.D, p.hk) &&
+      side_by_side(p.v_sh, p.D, p.hv)) {
+    const int rpl = dtype == OJX_F32 ? 1 : 2, heads_each = rpl * per_warp;
+    p.gq = (p.hq + heads_each - 1) / heads_each;
+    p.gk = (p.hk + heads_each - 1) / heads_each;
+    p.gv = (p.hv + heads_each - 1) / heads_each;
+    if (p.tokens * (p.gq + p.gk + p.gv) > INT32_MAX) return set_error(OJX_ERR_INVALID, "too many rows for one call");
+    const int slot = heads_each * p.D * dtype_size(dtype) + (p.norm ? p.rotary * 4 : 0);
+    const int smem = 8 * QK_RING * slot + (p.norm ? 2 * p.D * 4 : 0);
+    return for_dtype(dtype, [&](auto t) {
+      using T = decltype(t);
+      auto go = [&](auto kern) {
+        int st = ensure_smem_attr(reinterpret_cast<const void*>(kern), smem);
+        if (st) return st;
+        kern<<<2 * sms, 256, smem, s>>>(p, slot, g_wait_budget.load());
+        return launched("qk_rows_stream launch");
+      };
+      if (!p.norm) return go(qk_rows_stream_kernel<T, false, false>);
+      return inter ? go(qk_rows_stream_kernel<T, true, true>) : go(qk_rows_stream_kernel<T, false, true>);
+    });
+  }
   const int64_t warps = p.tokens * p.blocks_per_token;
   const int64_t grid = (warps + 7) / 8;
   if (grid > INT32_MAX) return set_error(OJX_ERR_INVALID, "too many rows for one call");
@@ -133,6 +161,7 @@ static QkParams make_qk(const ojx_qk_desc* d) {
   p.dtype_w = d->dtype_weight;
   p.pos64 = d->positions_int64;
   p.eps = d->eps;
+  p.inv_dim = 1.0f / d->head_dim;
   p.q = d->q.data, p.q_st = d->q.stride_t, p.q_sh = d->q.stride_h;
   p.k = d->k.data, p.k_st = d->k.stride_t, p.k_sh = d->k.stride_h;
   p.qw = d->q_weight;
@@ -302,7 +331,7 @@ int ojx_qk_norm_rope_backward(const ojx_qk_desc* d, const ojx_rows* gq, const oj
   p.gq = (p.hq + 32 / p.lanes - 1) / (32 / p.lanes);
   p.gk = (p.hk + 32 / p.lanes - 1) / (32 / p.lanes);
   // Blocks in proportion to each side's heads, at most one warp per token of it.
-  const int64_t most = 3ll * current_props().sm_count;
+  const int64_t most = 2ll * current_props().sm_count;  // two blocks an SM
   auto blocks_of = [&](int heads) -> int64_t {
     if (heads == 0) return 0;
     const int64_t share = std::max<int64_t>(1, most * heads / (d->q_heads + d->kv_heads));
@@ -312,9 +341,30 @@ int ojx_qk_norm_rope_backward(const ojx_qk_desc* d, const ojx_rows* gq, const oj
   const int blocks = p.q_blocks + static_cast<int>(blocks_of(d->kv_heads));
   p.partial = static_cast<float*>(stream_workspace(s, static_cast<size_t>(blocks) * p.D * 4, 9, false));
   if (!p.partial) return workspace_error();
-  const int smem = 8 * p.D * 4;
+  int smem = 8 * p.D * 4;
+  const int sms = current_props().sm_count, per_warp = 32 / p.lanes;
+  const bool stream_rows = vec && p.tokens >= 16ll * sms && aligned16(p.table) && p.rotary % 4 == 0 &&
+                           side_by_side(p.q_sh, p.D, p.hq) && side_by_side(p.k_sh, p.D, p.hk) && side_by_side(p.gq_sh, p.D, p.hq) &&
+                           side_by_side(p.gk_sh, p.D, p.hk);
+  const int heads_each = per_warp * (es == 4 ? 1 : 2);
+  const int slot = 2 * heads_each * p.D * es + p.rotary * 4;
+  if (stream_rows) {
+    p.gq = (p.hq + heads_each - 1) / heads_each;
+    p.gk = (p.hk + heads_each - 1) / heads_each;
+    if (p.tokens * std::max(p.gq, p.gk) > INT32_MAX) return set_error(OJX_ERR_INVALID, "too many rows for one call");
+    smem = std::max(smem, 8 * QK_GRAD_RING * slot);
+  }
   st = for_dtype(d->dtype, [&](auto t) {
     using T = decltype(t);
+    if (stream_rows) {
+      auto go = [&](auto kern) {
+        int r = ensure_smem_attr(reinterpret_cast<const void*>(kern), smem);
+        if (r) return r;
+        kern<<<blocks, 256, smem, s>>>(p, slot, g_wait_budget.load());
+        return launched("qk_grad_stream launch");
+      };
+      return inter ? go(qk_grad_stream_kernel<T, true>) : go(qk_grad_stream_kernel<T, false>);
+    }
     if (vec && !inter) qk_grad_fast_kernel<T, false><<<blocks, 256, smem, s>>>(p);
     else if (vec) qk_grad_fast_kernel<T, true><<<blocks, 256, smem, s>>>(p);
     else if (!inter) qk_grad_kernel<T, 1, 8, false><<<blocks, 256, smem, s>>>(p);

@@ -591,3 +591,58 @@ def test_graph_capture_of_a_decoding_step(S):
     g.replay()
     torchcl.synchronize()
     assert all(torch.equal(torchcl.to_cpu(a), b) for a, b in zip(out, want))
+
+
+# ── long calls: the forms that stream rows ─────────────────────────────────────────
+
+@pytest.mark.parametrize("tokens,hq,hk,dim,rotary,inter,dtype", [
+    (2400, 8, 2, 128, 128, False, "bf16"), (2371, 7, 1, 96, 48, False, "f32"), (5003, 3, 3, 64, 64, True, "f16"),
+    (2999, 2, 1, 256, 128, False, "bf16"), (2500, 1, 1, 512, 512, False, "f32"), (2400, 5, 3, 32, 16, False, "bf16")])
+def test_qk_many_tokens(S, tokens, hq, hk, dim, rotary, inter, dtype):
+    q, k, qw, kw, table, pos = qk_inputs(tokens, hq, hk, dim, rotary, dtype)
+    gq, gk = rnd(8, *q.shape, dtype=q.dtype), rnd(9, *k.shape, dtype=q.dtype)
+    d = [t.cuda().requires_grad_(True) for t in (q, k, qw, kw)]
+    out = S.qk_norm_rope(*d, table.cuda(), pos.cuda(), interleaved=inter)
+    got = torch.autograd.grad(out, d, [gq.cuda(), gk.cuda()])
+    for x, w, g, y, dx, dw in ((q, qw, gq, out[0].detach(), got[0], got[2]), (k, kw, gk, out[1].detach(), got[1], got[3])):
+        u = ROUND[x.dtype] if x.dtype != torch.float32 else 0.0
+        tiny = 6e-8 if dtype == "f16" else 0.0
+        want, size = ref.norm_rope(x, w, table, pos, interleaved=inter)
+        within(y, want, u * want.abs() + 32 * F32 * size + tiny)
+        want, dwant, size, dsize = ref.norm_rope_grad(x, w, g, table, pos, interleaved=inter)
+        within(dx, want, u * want.abs() + 64 * F32 * size + tiny)
+        # runs in a register, warps of a block, blocks: at most a few hundred roundings deep
+        within(dw, dwant, u * dwant.abs() + 1024 * F32 * dsize)
+
+
+def test_many_tokens_bad_positions_and_slots(S):
+    import torchcl
+    n = 2500
+    q, k, qw, kw, table, pos = qk_inputs(n, 4, 2, 128, 128, "bf16")
+    pos[7], pos[2000] = 5000, -3
+    slots = torch.randperm(n + 100, generator=torch.Generator().manual_seed(1))[:n]
+    slots[11], slots[12] = -1, 10 ** 9
+    fused = torch.cat([q, k, k], 1).cuda()
+    cache = S.KVCache.from_pages(*pages_for("int8", (n + 100) // 4, 2, 4, 128))
+    got = S.qkv_to_cache(fused[:, :4], fused[:, 4:6], fused[:, 6:], qw.cuda(), kw.cuda(), table.cuda(), pos.cuda(), cache, slots.cuda())
+    with pytest.raises(ValueError, match="out of range"):
+        torchcl.synchronize()
+    assert torch.isnan(got[[7, 2000]]).all() and int(torch.isnan(got).any(-1).any(-1).sum()) == 2
+    keep = torch.ones(n, dtype=torch.bool)
+    keep[[11, 12]] = False
+    kk, v = cache.read(slots[keep].cuda(), dtype=torch.float32)
+    assert torch.equal(v.cpu(), ref.stored(k[keep], "int8")[0])
+    bad = torch.isnan(kk).any(-1).any(-1).cpu()
+    assert torch.equal(bad, ((pos < 0) | (pos >= 5000))[keep])
+
+
+@pytest.mark.parametrize("fmt", FORMATS)
+@pytest.mark.parametrize("dtype", ["f32", "f16"])
+def test_cache_many_tokens_is_exact(S, fmt, dtype):
+    n, heads, dim, size = 3001, 3, 96, 16
+    k, v = rnd(1, n, heads, dim, dtype=DT[dtype], scale=7.0), rnd(2, n, heads, dim, dtype=DT[dtype], scale=1e-3)
+    cache = S.KVCache.from_pages(*pages_for(fmt, n // size + 2, heads, size, dim))
+    slots = torch.randperm(n, generator=torch.Generator().manual_seed(3)).cuda()
+    cache.append(k.cuda(), v.cuda(), slots)
+    for x, y in zip((k, v), cache.read(slots, dtype=torch.float32)):
+        assert torch.equal(y.cpu(), ref.stored(x, fmt)[0])
