@@ -224,15 +224,8 @@ __device__ __forceinline__ void store_cached(void* base, int64_t at, int format,
 #pragma unroll
     for (int e = 0; e < CH; ++e) q[e] = quantise_one(v[e], step, format);
     uint8_t* dst = static_cast<uint8_t*>(base) + at;
-    if constexpr (CH == 8) {
-      uint2 w;
-      w.x = q[0] | (q[1] << 8) | (q[2] << 16) | (static_cast<uint32_t>(q[3]) << 24);
-      w.y = q[4] | (q[5] << 8) | (q[6] << 16) | (static_cast<uint32_t>(q[7]) << 24);
-      *reinterpret_cast<uint2*>(dst) = w;
-    } else {
 #pragma unroll
-      for (int e = 0; e < CH; ++e) dst[e] = q[e];
-    }
+    for (int e = 0; e < CH; ++e) dst[e] = q[e];
   }
 }
 
@@ -679,28 +672,72 @@ __device__ __forceinline__ void norm_turn(const QkParams& p, const Turn<INTER>& 
   }
   turn.template apply<1>(xa, xb);
 }
+// x / step of two elements, correctly rounded, from inv = 1 / step rounded: an estimate
+// x * inv and two corrections by its exact remainder (P. Markstein, "Computation of
+// elementary functions on the IBM RISC System/6000 processor", 1990: the second correction
+// of a quotient within one ulp rounds it correctly).  Needs steps far from under- and
+// overflow.  The compiler's division took 40 % of the instructions of an append.
+__device__ __forceinline__ uint64_t quotient2(uint64_t x, uint64_t minus_step, uint64_t inv) {
+  uint64_t q = f2_mul(x, inv);
+  q = f2_fma(f2_fma(q, minus_step, x), inv, q);
+  return f2_fma(f2_fma(q, minus_step, x), inv, q);
+}
+// Eight elements of a row of this step as the cache's bytes.
+__device__ __forceinline__ uint2 quantise_eight(const uint64_t (&x)[4], float step, int format) {
+  uint32_t w[2] = {0, 0};
+  if (step >= 8.67361738e-19f && step <= 1.15292150e18f) {  // 2^-60 .. 2^60
+    const float inv = __frcp_rn(step);
+    const uint64_t inv2 = f2_pair(inv, inv), minus = f2_pair(-step, -step);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const float2 q = f2_split(quotient2(x[i], minus, inv2));
+      uint32_t two;
+      if (format == OJX_KV_INT8) {
+        // rounding to whole by adding 1.5 * 2^23: the low byte is the two's complement
+        const float u = fminf(fmaxf(q.x, -127.0f), 127.0f) + 12582912.0f, v = fminf(fmaxf(q.y, -127.0f), 127.0f) + 12582912.0f;
+        two = __byte_perm(__float_as_uint(u), __float_as_uint(v), 0x0040);
+      } else {
+        two = __nv_cvt_float2_to_fp8x2(q, __NV_SATFINITE, __NV_E4M3);
+      }
+      w[i >> 1] |= (two & 0xffffu) << (16 * (i & 1));
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const float2 v = f2_split(x[i]);
+      w[i >> 1] |= (quantise_one(v.x, step, format) | (static_cast<uint32_t>(quantise_one(v.y, step, format)) << 8)) << (16 * (i & 1));
+    }
+  }
+  return make_uint2(w[0], w[1]);
+}
+
+// A row pair of chunks into the cache.
 __device__ __forceinline__ void cache_row(const QkParams& p, int64_t slot, bool is_k, int h, bool valid, bool on, int j, int a, int b,
                                           const uint64_t (&xa)[4], const uint64_t (&xb)[4]) {
-  float va[8], vb[8];
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const float2 u = f2_split(xa[i]), v = f2_split(xb[i]);
-    va[2 * i] = u.x, va[2 * i + 1] = u.y, vb[2 * i] = v.x, vb[2 * i + 1] = v.y;
-  }
-  float step = 0.0f;
+  void* base = is_k ? p.cache.k : p.cache.v;
+  const int64_t row = valid ? slot_row(p.cache, slot, h) : -1;
   if (p.cache.format >= OJX_KV_INT8) {
     float amax = 0.0f;
 #pragma unroll
-    for (int e = 0; e < 8; ++e) amax = max_nan(amax, max_nan(fabsf(va[e]), fabsf(vb[e])));
+    for (int i = 0; i < 4; ++i) {
+      const float2 u = f2_split(xa[i]), v = f2_split(xb[i]);
+      amax = max_nan(amax, max_nan(max_nan(fabsf(u.x), fabsf(u.y)), max_nan(fabsf(v.x), fabsf(v.y))));
+    }
     for (int o = p.lanes >> 1; o > 0; o >>= 1) amax = max_nan(amax, __shfl_xor_sync(0xffffffffu, amax, o));
-    step = quantise_step(amax, p.cache.format);
-  }
-  const int64_t row = valid ? slot_row(p.cache, slot, h) : -1;
-  if (row >= 0 && on) {
-    void* base = is_k ? p.cache.k : p.cache.v;
-    if (p.cache.format >= OJX_KV_INT8 && j == 0) (is_k ? p.cache.k_scale : p.cache.v_scale)[row] = step;
-    store_cached<8>(base, row * p.D + a, p.cache.format, step, va);
-    store_cached<8>(base, row * p.D + b, p.cache.format, step, vb);
+    const float step = quantise_step(amax, p.cache.format);
+    if (row < 0 || !on) return;
+    if (j == 0) (is_k ? p.cache.k_scale : p.cache.v_scale)[row] = step;
+    uint8_t* dst = static_cast<uint8_t*>(base) + row * p.D;
+    *reinterpret_cast<uint2*>(dst + a) = quantise_eight(xa, step, p.cache.format);
+    *reinterpret_cast<uint2*>(dst + b) = quantise_eight(xb, step, p.cache.format);
+  } else if (row >= 0 && on) {
+    if (p.cache.format == OJX_KV_BF16) {
+      store_pairs<__nv_bfloat16>(static_cast<__nv_bfloat16*>(base) + row * p.D + a, xa, false);
+      store_pairs<__nv_bfloat16>(static_cast<__nv_bfloat16*>(base) + row * p.D + b, xb, false);
+    } else {
+      store_pairs<__half>(static_cast<__half*>(base) + row * p.D + a, xa, false);
+      store_pairs<__half>(static_cast<__half*>(base) + row * p.D + b, xb, false);
+    }
   }
 }
 

@@ -646,3 +646,18 @@ def test_cache_many_tokens_is_exact(S, fmt, dtype):
     cache.append(k.cuda(), v.cuda(), slots)
     for x, y in zip((k, v), cache.read(slots, dtype=torch.float32)):
         assert torch.equal(y.cpu(), ref.stored(x, fmt)[0])
+
+
+@pytest.mark.parametrize("fmt", ["int8", "float8"])
+def test_cache_quotients_are_those_of_division(S, fmt):
+    """Four million quotients, steps over 60 powers of ten, ties among them: every stored
+    value is that of a correctly rounded division."""
+    n, dim = 32768, 128
+    gen = torch.Generator().manual_seed(5)
+    x = torch.randn(n, 1, dim, generator=gen) * 10.0 ** (torch.rand(n, 1, 1, generator=gen) * 60 - 30)
+    x[:, :, 64:] = (torch.randint(-254, 255, (n, 1, 64), generator=gen) * 0.5) / 127 * x.abs().amax(-1, keepdim=True)
+    cache = S.KVCache.from_pages(*pages_for(fmt, n // 16, 1, 16, dim))
+    slots = torch.arange(n).cuda()
+    cache.append(x.cuda(), x.flip(0).cuda(), slots)
+    for a, b in zip((x, x.flip(0)), cache.read(slots, dtype=torch.float32)):
+        assert torch.equal(b.cpu(), ref.stored(a, fmt)[0])
