@@ -178,36 +178,41 @@ static bool qk_vector(const ojx_qk_desc* d) {
          vector_rows(d->k, es) && aligned16(d->q_weight) && aligned16(d->k_weight);
 }
 
-template <int FMT, int D, int MT>
-static int launch_tree(TaParams& p, cudaStream_t s) {
-  using L = TaLayout<FMT, D, MT>;
-  auto kern = tree_attention_kernel<FMT, D, MT>;
-  int st = ensure_smem_attr(reinterpret_cast<const void*>(kern), L::SMEM);
-  if (st) return st;
+// CTAs of a call (an equal share of its key tiles each, an SM each) and their workspace.
+static int plan_tree(TaParams& p, int tile_rows, int unit, int D, cudaStream_t s, int* ctas) {
   const int rows = p.tokens * p.group;
-  p.row_tiles = (rows + L::ROWS - 1) / L::ROWS;
-  const int64_t segments = static_cast<int64_t>(p.batch) * p.cache.kv_heads * p.row_tiles;
-  const int64_t most_keys = static_cast<int64_t>(p.width) * p.cache.page_size;
-  const int64_t steps = (most_keys + L::NW * L::KB - 1) / (L::NW * L::KB);
-  const int sms = current_props().sm_count;
-  int64_t splits = std::max<int64_t>(1, std::min((sms + segments - 1) / segments, steps));
-  p.splits = static_cast<int>(splits);
-  if (segments * splits > INT32_MAX) return set_error(OJX_ERR_INVALID, "ojx_tree_attention: too many rows");
-  if (splits > 1) {
-    const size_t slots = static_cast<size_t>(segments) * splits * L::ROWS;
-    char* ws = static_cast<char*>(stream_workspace(s, slots * (D * 4 + 8), 8, false));
-    if (!ws) return workspace_error();
-    p.part_o = reinterpret_cast<float*>(ws);
-    p.part_ml = reinterpret_cast<float2*>(ws + slots * D * 4);
-  }
-  kern<<<static_cast<unsigned>(segments * splits), L::NW * 32, L::SMEM, s>>>(p);
-  if ((st = launched("tree_attention launch"))) return st;
-  if (splits > 1) {
-    const int64_t all = static_cast<int64_t>(p.batch) * p.cache.kv_heads * rows;
-    tree_attention_join_kernel<D><<<static_cast<unsigned>((all + 3) / 4), 128, 0, s>>>(p, L::ROWS);
-    st = launched("tree_attention join launch");
-  }
-  return st;
+  p.row_tiles = (rows + tile_rows - 1) / tile_rows;
+  const int64_t per_seq = static_cast<int64_t>(p.cache.kv_heads) * p.row_tiles;
+  const int64_t most = p.batch * per_seq * ((static_cast<int64_t>(p.width) * p.cache.page_size + unit - 1) / unit);
+  if (per_seq > INT32_MAX || most > INT32_MAX) return set_error(OJX_ERR_INVALID, "ojx_tree_attention: too large");
+  *ctas = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(most, current_props().sm_count)));
+  const size_t slots = static_cast<size_t>(*ctas) * 2 * tile_rows;
+  char* ws = static_cast<char*>(stream_workspace(s, slots * (D * 4 + 8), 8, false));
+  if (!ws) return workspace_error();
+  p.part_o = reinterpret_cast<float*>(ws);
+  p.part_ml = reinterpret_cast<float2*>(ws + slots * D * 4);
+  return OJX_OK;
+}
+template <int D>
+static int join_tree(const TaParams& p, int tile_rows, int unit, int ctas, cudaStream_t s) {
+  const int64_t all = static_cast<int64_t>(p.batch) * p.cache.kv_heads * p.tokens * p.group;
+  tree_attention_parts_kernel<D><<<static_cast<unsigned>((all + 3) / 4), 128, 0, s>>>(p, tile_rows, unit, ctas);
+  return launched("tree_attention parts launch");
+}
+
+template <int FMT, int D>
+static int launch_tree(TaParams& p, cudaStream_t s) {
+  using L = TaLayout<FMT, D>;
+  int ctas = 0, st = plan_tree(p, 16, L::UNIT, D, s, &ctas);
+  if (st) return st;
+  auto go = [&](auto kern) {
+    int r = ensure_smem_attr(reinterpret_cast<const void*>(kern), L::SMEM);
+    if (r) return r;
+    kern<<<ctas, L::NW * 32, L::SMEM, s>>>(p, g_wait_budget.load());
+    return launched("tree_attention launch");
+  };
+  st = p.tokens * p.group <= 8 ? go(tree_attention_kernel<FMT, D, true>) : go(tree_attention_kernel<FMT, D, false>);
+  return st ? st : join_tree<D>(p, 16, L::UNIT, ctas, s);
 }
 
 template <int FMT, int D, int QT>
@@ -216,17 +221,8 @@ static int launch_tree_tc(TaParams& p, cudaStream_t s) {
   auto kern = tree_attention_tc_kernel<FMT, D, QT>;
   int st = ensure_smem_attr(reinterpret_cast<const void*>(kern), L::SMEM);
   if (st) return st;
-  const int rows = p.tokens * p.group, tile_rows = QT * TC_BN;
-  p.row_tiles = (rows + tile_rows - 1) / tile_rows;
-  const int64_t per_seq = static_cast<int64_t>(p.cache.kv_heads) * p.row_tiles;
-  const int64_t most = p.batch * per_seq * ((static_cast<int64_t>(p.width) * p.cache.page_size + TC_BN - 1) / TC_BN);
-  if (per_seq > INT32_MAX || most > INT32_MAX) return set_error(OJX_ERR_INVALID, "ojx_tree_attention: too large");
-  const int ctas = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(most, current_props().sm_count)));
-  const size_t slots = static_cast<size_t>(ctas) * 2 * tile_rows;
-  char* ws = static_cast<char*>(stream_workspace(s, slots * (D * 4 + 8), 8, false));
-  if (!ws) return workspace_error();
-  p.part_o = reinterpret_cast<float*>(ws);
-  p.part_ml = reinterpret_cast<float2*>(ws + slots * D * 4);
+  int ctas = 0;
+  if ((st = plan_tree(p, QT * TC_BN, TC_BN, D, s, &ctas))) return st;
   // A TMA box holds rows of one page, so the page size decides its rows; the swizzle's
   // pattern spans eight.
   CUtensorMap tk{}, tv{};
@@ -242,22 +238,18 @@ static int launch_tree_tc(TaParams& p, cudaStream_t s) {
   }
   kern<<<ctas, TC_THREADS, L::SMEM, s>>>(tk, tv, p, g_wait_budget.load());
   if ((st = launched("tree_attention_tc launch"))) return st;
-  const int64_t all = static_cast<int64_t>(p.batch) * p.cache.kv_heads * rows;
-  tree_attention_parts_kernel<D><<<static_cast<unsigned>((all + 3) / 4), 128, 0, s>>>(p, tile_rows, TC_BN, ctas);
-  return launched("tree_attention parts launch");
+  return join_tree<D>(p, QT * TC_BN, TC_BN, ctas, s);
 }
 
 template <int FMT>
 static int launch_tree_fmt(TaParams& p, cudaStream_t s) {
   const int rows = p.tokens * p.group;
-  if (rows > 32) {
+  if (rows > 16) {
     const bool two = rows > 128;
     if (p.cache.head_dim == 64) return two ? launch_tree_tc<FMT, 64, 2>(p, s) : launch_tree_tc<FMT, 64, 1>(p, s);
     return two ? launch_tree_tc<FMT, 128, 2>(p, s) : launch_tree_tc<FMT, 128, 1>(p, s);
   }
-  const bool wide = p.tokens * p.group > 16;  // more than one 16-row tile
-  if (p.cache.head_dim == 64) return wide ? launch_tree<FMT, 64, 2>(p, s) : launch_tree<FMT, 64, 1>(p, s);
-  return wide ? launch_tree<FMT, 128, 2>(p, s) : launch_tree<FMT, 128, 1>(p, s);
+  return p.cache.head_dim == 64 ? launch_tree<FMT, 64>(p, s) : launch_tree<FMT, 128>(p, s);
 }
 
 }  // namespace ojx

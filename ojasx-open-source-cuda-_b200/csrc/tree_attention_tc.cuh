@@ -62,146 +62,6 @@ struct TcLayout {
   static_assert(SMEM <= 227 * 1024, "shared memory");
 };
 
-// ── the division of a call's key tiles over CTAs ──────────────────────────────────
-// Sequence b has tiles(b) key tiles in each of its `per_seq` segments; tiles are counted
-// sequence by sequence, segment by segment.  CTA c of G takes tiles [c U / G, (c+1) U / G).
-// A segment's part that is not the whole segment goes to slot 0 of its CTA when it is the
-// CTA's first, else to slot 1; the join kernel finds the parts from the same numbers.
-struct TaLens {
-  int ctx, drafts;
-};
-__device__ __forceinline__ TaLens ta_lens(const TaParams& p, int b, bool report) {
-  int ctx = max(p.contexts[b], 0);
-  int drafts = p.drafts ? min(max(p.drafts[b], 0), p.tokens) : p.tokens;
-  const int64_t room = static_cast<int64_t>(p.width) * p.cache.page_size;
-  if (static_cast<int64_t>(ctx) + drafts > room) {  // more keys than the page table holds
-    if (report) index_error();
-    ctx = static_cast<int>(min(static_cast<int64_t>(ctx), room));
-    drafts = static_cast<int>(min(static_cast<int64_t>(drafts), room - ctx));
-  }
-  return {ctx, drafts};
-}
-__device__ __forceinline__ int ta_tiles(const TaParams& p, int b, int unit) {
-  const TaLens l = ta_lens(p, b, false);
-  return (l.ctx + l.drafts + unit - 1) / unit;
-}
-
-// Where a CTA's share begins: sequence, tiles before that sequence, first and last tile.
-// (A call has fewer than 2^31 tiles.)
-struct TaShare {
-  int b, base, u, end;
-};
-// By one warp; the lanes take equal strips of sequences.
-__device__ __forceinline__ TaShare ta_share_of(const TaParams& p, int per_seq, int unit, int cta, int ctas) {
-  const int lane = threadIdx.x & 31;
-  const int strip = (p.batch + 31) / 32;
-  const int b0 = min(p.batch, lane * strip), b1 = min(p.batch, b0 + strip);
-  long long mine = 0;
-  for (int b = b0; b < b1; ++b) {
-    const TaLens l = ta_lens(p, b, cta == 0);
-    mine += (l.ctx + l.drafts + unit - 1) / unit;
-  }
-  long long run = mine;
-  for (int o = 1; o < 32; o <<= 1) {
-    const long long up = __shfl_up_sync(0xffffffffu, run, o);
-    if (lane >= o) run += up;
-  }
-  const long long total = __shfl_sync(0xffffffffu, run, 31) * per_seq;
-  TaShare s;
-  s.u = static_cast<int>(total * cta / ctas);
-  s.end = static_cast<int>(total * (cta + 1) / ctas);
-  s.b = 0;
-  s.base = 0;
-  const bool here = s.u < s.end && (run - mine) * per_seq <= s.u && s.u < run * per_seq;
-  if (here) {
-    long long base = (run - mine) * per_seq;
-    int b = b0;
-    for (; b < b1; ++b) {
-      const long long n = static_cast<long long>(ta_tiles(p, b, unit)) * per_seq;
-      if (s.u < base + n) break;
-      base += n;
-    }
-    s.b = b;
-    s.base = static_cast<int>(base);
-  }
-  const unsigned who = __ballot_sync(0xffffffffu, here);
-  const int src = who ? __ffs(who) - 1 : 0;
-  s.b = __shfl_sync(0xffffffffu, s.b, src);
-  s.base = __shfl_sync(0xffffffffu, s.base, src);
-  return s;
-}
-
-// One segment's part of a CTA's share.
-struct TaPart {
-  int b, seg, t0, n, tiles;  // sequence, segment in it, first tile, tiles here, tiles in all
-  int kvh;                   // the segment's key head
-  int ctx, drafts;
-  bool first;                // first part of this CTA
-};
-struct TaWalk {
-  TaShare s;
-  int tiles, ctx, drafts;
-  bool first;
-  __device__ __forceinline__ void begin(const TaParams& p, const TaShare& share, int unit) {
-    s = share;
-    first = true;
-    if (s.u < s.end) load(p, unit);
-  }
-  __device__ __forceinline__ void load(const TaParams& p, int unit) {
-    const TaLens l = ta_lens(p, s.b, false);
-    ctx = l.ctx;
-    drafts = l.drafts;
-    tiles = (ctx + drafts + unit - 1) / unit;
-  }
-  __device__ __forceinline__ bool next(const TaParams& p, int per_seq, int unit, TaPart& o) {
-    if (s.u >= s.end) return false;
-    while (s.u >= s.base + tiles * per_seq) {  // (ends: u < end <= all tiles)
-      s.base += tiles * per_seq;
-      ++s.b;
-      load(p, unit);
-    }
-    const int at = s.u - s.base;
-    o.b = s.b;
-    o.seg = at / tiles;
-    o.t0 = at - o.seg * tiles;
-    o.kvh = o.seg / p.row_tiles;
-    o.tiles = tiles;
-    o.n = min(tiles - o.t0, s.end - s.u);
-    o.ctx = ctx;
-    o.drafts = drafts;
-    o.first = first;
-    first = false;
-    s.u += o.n;
-    return true;
-  }
-};
-
-// Bits of keys k0 .. k0 + 31 that row `token` of sequence b sees (keys end at `hi`).
-__device__ __forceinline__ uint32_t ta_visible(const TaParams& p, int b, int token, int k0, int ctx, int hi) {
-  if (token < 0 || k0 >= hi) return 0;
-  uint32_t bits = 0;
-  const int d0 = k0 - ctx;
-  if (d0 <= -32) {
-    bits = 0xffffffffu;
-  } else {
-    const int from = max(d0, 0), lead = from - d0;  // first draft of the window, context keys before it
-    uint32_t m;
-    if (p.mask) {
-      const int64_t* row = p.mask + b * p.mask_sb + static_cast<int64_t>(token) * p.words;
-      const int w = from >> 6, sh = from & 63;
-      uint64_t x = w < p.words ? static_cast<uint64_t>(row[w]) >> sh : 0;
-      if (sh > 32 && w + 1 < p.words) x |= static_cast<uint64_t>(row[w + 1]) << (64 - sh);
-      m = static_cast<uint32_t>(x);
-    } else {
-      const int n = token - from + 1;  // causal: drafts up to the row's own
-      m = n >= 32 ? 0xffffffffu : n <= 0 ? 0u : (1u << n) - 1u;
-    }
-    bits = lead == 0 ? m : (m << lead) | ((1u << lead) - 1u);
-  }
-  const int n = hi - k0;
-  return n >= 32 ? bits : bits & ((1u << n) - 1u);
-}
-
 __device__ __forceinline__ void tc_sts128(uint32_t a, uint32_t x, uint32_t y, uint32_t z, uint32_t w) {
   asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(a), "r"(x), "r"(y), "r"(z), "r"(w) : "memory");
 }
@@ -298,11 +158,6 @@ struct TcCursor {
   // Number (as K tile) of the V tile at the cursor: i - lead of the min(i, n) before it here.
   __device__ __forceinline__ uint32_t k_number() const { return kc - static_cast<uint32_t>(min(i, part.n) - (i - lead)); }
 };
-
-// Asynchronous copies of this thread so far arrive on `bar` when they have landed.
-__device__ __forceinline__ void tc_copies_arrive(uint32_t bar) {
-  asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(bar) : "memory");
-}
 
 template <int FMT, int D, int QT>
 __global__ void __launch_bounds__(TC_THREADS, 1) tree_attention_tc_kernel(const __grid_constant__ CUtensorMap tmK,
@@ -1126,73 +981,6 @@ __global__ void __launch_bounds__(TC_THREADS, 1) tree_attention_tc_kernel(const 
     tc_fence_after();
     tmem_dealloc(tmem, 512);
   }
-}
-
-// Joins the parts of segments that more than one CTA took, and writes the zeros of
-// sequences without keys.  One warp per row; the parts' factors sit in the lanes, so the
-// loads of a pass over 32 parts do not wait for one another.
-template <int D>
-__global__ void __launch_bounds__(128) tree_attention_parts_kernel(const TaParams p, int tile_rows, int unit, int ctas) {
-  const int lane = threadIdx.x & 31;
-  const int rows = p.tokens * p.group;
-  const int64_t w = static_cast<int64_t>(blockIdx.x) * 4 + (threadIdx.x >> 5);
-  if (w >= static_cast<int64_t>(p.batch) * p.cache.kv_heads * rows) return;
-  const int r = static_cast<int>(w % rows);
-  const int64_t bh = w / rows;
-  const int b = static_cast<int>(bh / p.cache.kv_heads), kvh = static_cast<int>(bh % p.cache.kv_heads);
-  const int per_seq = p.cache.kv_heads * p.row_tiles;
-  long long before = 0, total = 0;
-  for (int i = lane; i < p.batch; i += 32) {
-    const int n = ta_tiles(p, i, unit);
-    total += n;
-    if (i < b) before += n;
-  }
-  for (int o = 16; o > 0; o >>= 1) {
-    before += __shfl_xor_sync(0xffffffffu, before, o);
-    total += __shfl_xor_sync(0xffffffffu, total, o);
-  }
-  const int tiles = ta_tiles(p, b, unit);
-  const int64_t at = ((static_cast<int64_t>(b) * p.tokens + r / p.group) * p.q_heads + kvh * p.group + r % p.group) * D;
-  if (tiles == 0) {
-    for (int i = 0; i < D / 32; ++i) store_as(p.out, at + lane + 32 * i, p.dtype, 0.0f);
-    return;
-  }
-  total *= per_seq;
-  const long long u0 = before * per_seq + static_cast<long long>(kvh * p.row_tiles + r / tile_rows) * tiles;
-  auto owner = [&](long long u) { return static_cast<int>(((u + 1) * ctas - 1) / total); };
-  const int c0 = owner(u0), c1 = owner(u0 + tiles - 1);
-  if (c0 == c1) return;  // written by its CTA
-  const bool first0 = total * c0 / ctas == u0;
-  auto slot_of = [&](int c) {
-    return (static_cast<int64_t>(c) * 2 + (c > c0 || first0 ? 0 : 1)) * tile_rows + r % tile_rows;
-  };
-  float ref = -INFINITY, acc[D / 32], l = 0.0f;
-#pragma unroll
-  for (int i = 0; i < D / 32; ++i) acc[i] = 0.0f;
-  for (int c = c0; c <= c1; c += 32) {
-    const int mine = c + lane;
-    float2 ml = make_float2(-INFINITY, 0.0f);
-    if (mine <= c1 && total * mine / ctas < total * (mine + 1) / ctas) ml = p.part_ml[slot_of(mine)];  // (or no tiles)
-    float top = fmaxf(ref, ml.x);
-    for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-    const float keep = ta_share(ref, l, top), f = ta_share(ml.x, ml.y, top);
-    float part = f != 0.0f ? f * ml.y : 0.0f;
-    for (int o = 16; o > 0; o >>= 1) part += __shfl_xor_sync(0xffffffffu, part, o);
-    l = (keep != 0.0f ? l * keep : 0.0f) + part;
-#pragma unroll
-    for (int i = 0; i < D / 32; ++i) acc[i] = keep != 0.0f ? acc[i] * keep : 0.0f;
-    ref = top;
-    const int n = min(32, c1 - c + 1);
-#pragma unroll 8
-    for (int k = 0; k < n; ++k) {
-      const float g = __shfl_sync(0xffffffffu, f, k);
-      const float* o = p.part_o + slot_of(c + k) * D + lane;
-#pragma unroll
-      for (int i = 0; i < D / 32; ++i) acc[i] += g != 0.0f ? g * o[32 * i] : 0.0f;
-    }
-  }
-#pragma unroll
-  for (int i = 0; i < D / 32; ++i) store_as(p.out, at + lane + 32 * i, p.dtype, l == 0.0f ? 0.0f : acc[i] / l);
 }
 
 }  // namespace ojx
