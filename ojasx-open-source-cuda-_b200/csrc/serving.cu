@@ -200,18 +200,15 @@ static int join_tree(const TaParams& p, int tile_rows, int unit, int ctas, cudaS
   return launched("tree_attention parts launch");
 }
 
-template <int FMT, int D>
+template <int FMT, int D, bool FEW>
 static int launch_tree(TaParams& p, cudaStream_t s) {
-  using L = TaLayout<FMT, D>;
+  using L = TaLayout<FMT, D, FEW>;
   int ctas = 0, st = plan_tree(p, 16, L::UNIT, D, s, &ctas);
   if (st) return st;
-  auto go = [&](auto kern) {
-    int r = ensure_smem_attr(reinterpret_cast<const void*>(kern), L::SMEM);
-    if (r) return r;
-    kern<<<ctas, L::NW * 32, L::SMEM, s>>>(p, g_wait_budget.load());
-    return launched("tree_attention launch");
-  };
-  st = p.tokens * p.group <= 8 ? go(tree_attention_kernel<FMT, D, true>) : go(tree_attention_kernel<FMT, D, false>);
+  auto kern = tree_attention_kernel<FMT, D, FEW>;
+  if ((st = ensure_smem_attr(reinterpret_cast<const void*>(kern), L::SMEM))) return st;
+  kern<<<ctas, L::NW * 32, L::SMEM, s>>>(p, g_wait_budget.load());
+  st = launched("tree_attention launch");
   return st ? st : join_tree<D>(p, 16, L::UNIT, ctas, s);
 }
 
@@ -249,7 +246,9 @@ static int launch_tree_fmt(TaParams& p, cudaStream_t s) {
     if (p.cache.head_dim == 64) return two ? launch_tree_tc<FMT, 64, 2>(p, s) : launch_tree_tc<FMT, 64, 1>(p, s);
     return two ? launch_tree_tc<FMT, 128, 2>(p, s) : launch_tree_tc<FMT, 128, 1>(p, s);
   }
-  return p.cache.head_dim == 64 ? launch_tree<FMT, 64>(p, s) : launch_tree<FMT, 128>(p, s);
+  const bool few = rows <= 8;
+  if (p.cache.head_dim == 64) return few ? launch_tree<FMT, 64, true>(p, s) : launch_tree<FMT, 64, false>(p, s);
+  return few ? launch_tree<FMT, 128, true>(p, s) : launch_tree<FMT, 128, false>(p, s);
 }
 
 }  // namespace ojx

@@ -281,7 +281,7 @@ __device__ __forceinline__ void tc_copies_arrive(uint32_t bar) {
 // for each run of a page (a warp's block in one piece, unswizzled: reading it meets a bank
 // two to four times, which costs less than permuting copies, about a hundred instructions
 // a block), widened to f16 in registers.  mma.sync m16n8k16 with the queries as the 16 rows.
-template <int FMT, int D>
+template <int FMT, int D, bool FEW>
 struct TaLayout {
   static constexpr bool QUANT = FMT >= TA_INT8;
   static constexpr int ES = QUANT ? 1 : 2;
@@ -289,9 +289,9 @@ struct TaLayout {
   static constexpr int CPR = D * ES / 16;               // 16-byte chunks per row
   static constexpr int TILE = KB * D * ES;              // K (or V) bytes per block
   static constexpr int STAGE = 2 * TILE + (QUANT ? KB * 8 : 0);  // 8 bits: (key step, value step) a key
-  static constexpr int NW = QUANT ? 12 : 8;             // warps per CTA
+  static constexpr int NW = QUANT && FEW ? 12 : 8;      // warps per CTA
   static constexpr int UNIT = NW * KB;
-  static constexpr int ST = D == 128 ? (QUANT ? 2 : 3) : 4;  // ring depth
+  static constexpr int ST = D == 128 ? (NW == 12 ? 2 : 3) : 4;  // ring depth
   static constexpr int RING = NW * ST * STAGE;
   static constexpr int MERGE = NW * 4 * (D * 4 + 8);    // four rows of every warp's result at a time
   static constexpr int SMEM = RING + MERGE;
@@ -307,8 +307,8 @@ __device__ __forceinline__ uint32_t ta_chunk(int r, int c) {
 
 // FEW: at most eight rows, so the fragments' rows 8-15 are empty and their softmax is left out.
 template <int FMT, int D, bool FEW>
-__global__ void __launch_bounds__(TaLayout<FMT, D>::NW * 32, 1) tree_attention_kernel(const TaParams p, uint64_t budget) {
-  using L = TaLayout<FMT, D>;
+__global__ void __launch_bounds__(TaLayout<FMT, D, FEW>::NW * 32, 1) tree_attention_kernel(const TaParams p, uint64_t budget) {
+  using L = TaLayout<FMT, D, FEW>;
   constexpr bool QUANT = L::QUANT, BF = FMT == TA_BF16;
   constexpr int KB = L::KB, NT = KB / 8, DT = D / 8, KS = D / 16, H = FEW ? 1 : 2, NW = L::NW;
   extern __shared__ __align__(128) uint8_t smem[];

@@ -159,6 +159,39 @@ struct TcCursor {
   __device__ __forceinline__ uint32_t k_number() const { return kc - static_cast<uint32_t>(min(i, part.n) - (i - lead)); }
 };
 
+// MMAs and commits issued by the lane with `lead`, in a warp that runs together.  Shared-memory
+// descriptors (128-byte swizzle): their constant parts for K and Q tiles and for V tiles; the
+// address, in 16-byte units, joins the low word.
+constexpr uint64_t tc_desc(uint32_t lbo, uint32_t sbo) {
+  return (static_cast<uint64_t>(lbo >> 4) << 16) | (static_cast<uint64_t>(sbo >> 4) << 32) | (1ull << 46) | (2ull << 61);
+}
+constexpr uint64_t SW128_K = tc_desc(16, 1024), SW128_V = tc_desc(8192, 1024);
+__device__ __forceinline__ void tc_mma_ss(uint32_t d, uint32_t a_lo, uint32_t b_lo, uint32_t hi, uint32_t idesc, bool add, bool lead) {
+  asm volatile(
+      "{\n\t.reg .pred p, q;\n\t.reg .b64 a, b;\n\t"
+      "setp.ne.b32 p, %5, 0;\n\tsetp.ne.b32 q, %6, 0;\n\t"
+      "mov.b64 a, {%1, %3};\n\tmov.b64 b, {%2, %3};\n\t"
+      "@q tcgen05.mma.cta_group::1.kind::f16 [%0], a, b, %4, p;\n\t}" ::"r"(d),
+      "r"(a_lo), "r"(b_lo), "r"(hi), "r"(idesc), "r"(static_cast<uint32_t>(add)), "r"(static_cast<uint32_t>(lead))
+      : "memory");
+}
+__device__ __forceinline__ void tc_mma_ts(uint32_t d, uint32_t a_tmem, uint32_t b_lo, uint32_t hi, uint32_t idesc, bool add, bool lead) {
+  asm volatile(
+      "{\n\t.reg .pred p, q;\n\t.reg .b64 b;\n\t"
+      "setp.ne.b32 p, %5, 0;\n\tsetp.ne.b32 q, %6, 0;\n\t"
+      "mov.b64 b, {%2, %3};\n\t"
+      "@q tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], b, %4, p;\n\t}" ::"r"(d),
+      "r"(a_tmem), "r"(b_lo), "r"(hi), "r"(idesc), "r"(static_cast<uint32_t>(add)), "r"(static_cast<uint32_t>(lead))
+      : "memory");
+}
+__device__ __forceinline__ void tc_commit(uint32_t bar, bool lead) {
+  asm volatile(
+      "{\n\t.reg .pred q;\n\tsetp.ne.b32 q, %1, 0;\n\t"
+      "@q tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n\t}" ::"r"(bar),
+      "r"(static_cast<uint32_t>(lead))
+      : "memory");
+}
+
 template <int FMT, int D, int QT>
 __global__ void __launch_bounds__(TC_THREADS, 1) tree_attention_tc_kernel(const __grid_constant__ CUtensorMap tmK,
                                                                           const __grid_constant__ CUtensorMap tmV,
@@ -451,57 +484,65 @@ __global__ void __launch_bounds__(TC_THREADS, 1) tree_attention_tc_kernel(const 
   } else if (warp >= 12) {
     // ── MMA issuer (warps 13-15 only give up registers) ────────────────────────
     asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
-    if (warp == 12 && lane == 0) {
+    if (warp == 12) {
+      // The whole warp runs the loop, with addresses from lane 0, and one lane issues: so the
+      // descriptors stay in uniform registers.  (Issued from a branch of one lane, an MMA of
+      // 32 cycles took a hundred.)
       constexpr uint32_t IDESC_S = make_idesc(MFMT, 0, 0, TC_BN, TC_BN);
       constexpr uint32_t IDESC_PV = make_idesc(MFMT, 0, 1, TC_BN, D);
+      constexpr uint32_t HI_KV = static_cast<uint32_t>(SW128_K >> 32), LO_K = static_cast<uint32_t>(SW128_K);
+      constexpr uint32_t HI_V = static_cast<uint32_t>(SW128_V >> 32), LO_V = static_cast<uint32_t>(SW128_V);
+      const bool lead = lane == 0;
+      auto uniform = [](uint32_t v) { return __shfl_sync(0xffffffffu, v, 0); };
+      const uint32_t uK = uniform(sK0 >> 4), uV = uniform(sV0 >> 4), uQ = uniform(sQ >> 4), uT = uniform(tmem);
       uint32_t kn = 0, pn[2] = {0, 0}, parts = 0;
       bool ok = true;
       TaWalk walk;
       walk.begin(p, *s_share, TC_BN);
       TaPart part;
       while (ok && walk.next(p, per_seq, TC_BN, part)) {
-        const int steps = QT * part.n;
-        ok = mbar_wait(q_full, parts & 1u, budget, s_abort);
+        const int n_tiles = static_cast<int>(uniform(part.n)), steps = QT * n_tiles;
+        ok = __all_sync(0xffffffffu, mbar_wait(q_full, parts & 1u, budget, s_abort));
         ++parts;
         // (from -2: the first scores of both units; S_t of step i + 2 lies over P_t of step i,
         // and the MMAs run in order)
         for (int i = -2; i < steps && ok; ++i) {
           const int t = i & 1;
           if (i >= 0) {
-            const uint32_t j = kn + (QT == 1 ? i : i >> 1);
-            if ((QT == 1 || t == 0) && !(ok = mbar_wait(v_full(j % VST), (j / VST) & 1u, budget, s_abort))) break;
-            if (!(ok = mbar_wait(p_full(t), pn[t] & 1u, budget, s_abort))) break;
+            const uint32_t j = kn + (QT == 1 ? i : i >> 1), st = j % VST;
+            if (QT == 1 || t == 0) ok = mbar_wait(v_full(st), (j / VST) & 1u, budget, s_abort);
+            ok = ok && mbar_wait(p_full(t), pn[t] & 1u, budget, s_abort);
+            if (!(ok = __all_sync(0xffffffffu, ok))) break;
             tc_fence_after();
-            const uint64_t bd = make_sw128_desc(sV0 + (j % VST) * L::TILE, 8192, 1024);
-            const uint32_t dO = tmem + 2 * TC_BN + t * D, aP = tmem + t * TC_BN;
+            const uint32_t b = LO_V | (uV + st * (L::TILE >> 4)), dO = uT + 2 * TC_BN + t * D, aP = uT + t * TC_BN;
 #pragma unroll
             for (int ks = 0; ks < TC_BN / 16; ++ks) {
-              const uint64_t b = bd + (((ks >> 2) * (L::DB * 8192) + (ks & 3) * 2048) >> 4);
-              mma_f16_ts(dO, aP + (ks >> 1) * 32 + (ks & 1) * 8, b, IDESC_PV, (i > 1 || ks > 0) ? 1u : 0u);
-              if constexpr (BF) mma_f16_ts(dO, aP + (ks >> 1) * 32 + (ks & 1) * 8 + 16, b, IDESC_PV, 1u);
+              const uint32_t at = b + (((ks >> 2) * (L::DB * 8192) + (ks & 3) * 2048) >> 4);
+              tc_mma_ts(dO, aP + (ks >> 1) * 32 + (ks & 1) * 8, at, HI_V, IDESC_PV, i > 1 || ks > 0, lead);
+              if constexpr (BF) tc_mma_ts(dO, aP + (ks >> 1) * 32 + (ks & 1) * 8 + 16, at, HI_V, IDESC_PV, true, lead);
             }
             ++pn[t];
-            if (QT == 1 || t == 1) mma_commit(v_empty(j % VST));
-            if (i + 2 >= steps) mma_commit(pv_done(t));
+            if (QT == 1 || t == 1) tc_commit(v_empty(st), lead);
+            if (i + 2 >= steps) tc_commit(pv_done(t), lead);
           }
           if (i + 2 < steps) {
-            const uint32_t j = kn + (QT == 1 ? i + 2 : (i + 2) >> 1);
-            if ((QT == 1 || t == 0) && !(ok = mbar_wait(k_full(j % KST), (j / KST) & 1u, budget, s_abort))) break;
+            const uint32_t j = kn + (QT == 1 ? i + 2 : (i + 2) >> 1), st = j % KST;
+            if (QT == 1 || t == 0) ok = mbar_wait(k_full(st), (j / KST) & 1u, budget, s_abort);
+            if (!(ok = __all_sync(0xffffffffu, ok))) break;
             tc_fence_after();
-            const uint64_t ad = make_sw128_desc(sQ + (QT == 1 ? 0 : t) * L::TILE, 16, 1024);
-            const uint64_t bd = make_sw128_desc(sK0 + (j % KST) * L::TILE, 16, 1024);
+            const uint32_t a = LO_K | (uQ + (QT == 1 ? 0 : t) * (L::TILE >> 4)), b = LO_K | (uK + st * (L::TILE >> 4));
 #pragma unroll
             for (int ks = 0; ks < D / 16; ++ks) {
               const uint32_t off = ((ks >> 2) * 16384 + (ks & 3) * 32) >> 4;
-              mma_f16(tmem + t * TC_BN, ad + off, bd + off, IDESC_S, ks > 0 ? 1u : 0u);
+              tc_mma_ss(uT + t * TC_BN, a + off, b + off, HI_KV, IDESC_S, ks > 0, lead);
             }
-            mma_commit(s_full(t));
-            if (QT == 1 || t == 1) mma_commit(k_empty(j % KST));
+            tc_commit(s_full(t), lead);
+            if (QT == 1 || t == 1) tc_commit(k_empty(st), lead);
           }
         }
-        kn += part.n;
+        kn += n_tiles;
       }
-      mma_commit(done_bar);  // every MMA must complete before TMEM is released
+      tc_commit(done_bar, lead);  // every MMA must complete before TMEM is released
       mbar_wait_drain(done_bar, 0, budget);
     } else if (warp == 13 && (QUANT || tma)) {
       // ── loader ─────────────────────────────────────────────────────────
