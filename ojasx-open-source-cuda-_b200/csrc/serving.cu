@@ -196,8 +196,18 @@ static int plan_tree(TaParams& p, int tile_rows, int unit, int D, cudaStream_t s
 template <int D>
 static int join_tree(const TaParams& p, int tile_rows, int unit, int ctas, cudaStream_t s) {
   const int64_t all = static_cast<int64_t>(p.batch) * p.cache.kv_heads * p.tokens * p.group;
-  tree_attention_parts_kernel<D><<<static_cast<unsigned>((all + 3) / 4), 128, 0, s>>>(p, tile_rows, unit, ctas);
-  return launched("tree_attention parts launch");
+  // (launched while the attention kernel ends: what it reads of the call's inputs overlaps)
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3(static_cast<unsigned>((all + 3) / 4));
+  cfg.blockDim = dim3(128);
+  cfg.stream = s;
+  cudaLaunchAttribute attr{};
+  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr.val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = &attr;
+  cfg.numAttrs = 1;
+  const int st = cuda_status(cudaLaunchKernelEx(&cfg, tree_attention_parts_kernel<D>, p, tile_rows, unit, ctas), "tree_attention parts launch");
+  return st ? st : launched("tree_attention parts launch");
 }
 
 template <int FMT, int D, bool FEW>
@@ -233,7 +243,7 @@ static int launch_tree_tc(TaParams& p, cudaStream_t s) {
     if ((st = make_tmap_2d_sw128(&tv, dt, 2, p.cache.v, D, all, D * 2, 64, r))) return st;
     p.box_rows = r;
   }
-  kern<<<ctas, TC_THREADS, L::SMEM, s>>>(tk, tv, p, g_wait_budget.load());
+  kern<<<ctas, L::THREADS, L::SMEM, s>>>(tk, tv, p, g_wait_budget.load());
   if ((st = launched("tree_attention_tc launch"))) return st;
   return join_tree<D>(p, QT * TC_BN, TC_BN, ctas, s);
 }

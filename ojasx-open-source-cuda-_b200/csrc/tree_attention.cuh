@@ -748,6 +748,7 @@ __global__ void __launch_bounds__(TaLayout<FMT, D, FEW>::NW * 32, 1) tree_attent
       __syncthreads();
     }
   }
+  grid_dep_launch_dependents();  // the join kernel may start; it waits for this grid's end
   if constexpr (QUANT) {
     // (after a wait that ran out: let the copies in flight land before the CTA may exit)
     for (; used < issued; ++used) {
@@ -764,6 +765,7 @@ __global__ void __launch_bounds__(TaLayout<FMT, D, FEW>::NW * 32, 1) tree_attent
 // loads of a pass over 32 parts do not wait for one another.
 template <int D>
 __global__ void __launch_bounds__(128) tree_attention_parts_kernel(const TaParams p, int tile_rows, int unit, int ctas) {
+  constexpr int E = D / 32;  // values a lane
   const int lane = threadIdx.x & 31;
   const int rows = p.tokens * p.group;
   const int64_t w = static_cast<int64_t>(blockIdx.x) * 4 + (threadIdx.x >> 5);
@@ -783,27 +785,36 @@ __global__ void __launch_bounds__(128) tree_attention_parts_kernel(const TaParam
     total += __shfl_xor_sync(0xffffffffu, total, o);
   }
   const int tiles = ta_tiles(p, b, unit);
+  grid_dep_wait();  // the parts are written (all above reads the call's inputs only)
   const int64_t at = ((static_cast<int64_t>(b) * p.tokens + r / p.group) * p.q_heads + kvh * p.group + r % p.group) * D;
   if (tiles == 0) {
-    for (int i = 0; i < D / 32; ++i) store_as(p.out, at + lane + 32 * i, p.dtype, 0.0f);
+    for (int i = 0; i < E; ++i) store_as(p.out, at + lane * E + i, p.dtype, 0.0f);
     return;
   }
-  total *= per_seq;
-  const long long u0 = before * per_seq + static_cast<long long>(kvh * p.row_tiles + r / tile_rows) * tiles;
-  auto owner = [&](long long u) { return static_cast<int>(((u + 1) * ctas - 1) / total); };
+  // CTA c's first tile, total * c / ctas, with one long division for all; and the CTA that has tile u.
+  const long long all = total * per_seq, each = all / ctas;
+  const int rest = static_cast<int>(all - each * ctas);
+  auto first_of = [&](int c) { return each * c + rest * c / ctas; };
+  auto owner = [&](long long u) {
+    int c = min(static_cast<int>(static_cast<float>(u) * (static_cast<float>(ctas) / static_cast<float>(all))), ctas - 1);
+    while (first_of(c) > u) --c;
+    while (c + 1 < ctas && first_of(c + 1) <= u) ++c;
+    return c;
+  };
+  const long long u0 = before * per_seq + (kvh * p.row_tiles + r / tile_rows) * tiles;
   const int c0 = owner(u0), c1 = owner(u0 + tiles - 1);
   if (c0 == c1) return;  // written by its CTA
-  const bool first0 = total * c0 / ctas == u0;
+  const bool first0 = first_of(c0) == u0;
   auto slot_of = [&](int c) {
     return (static_cast<int64_t>(c) * 2 + (c > c0 || first0 ? 0 : 1)) * tile_rows + r % tile_rows;
   };
-  float ref = -INFINITY, acc[D / 32], l = 0.0f;
+  float ref = -INFINITY, acc[E], l = 0.0f;
 #pragma unroll
-  for (int i = 0; i < D / 32; ++i) acc[i] = 0.0f;
+  for (int i = 0; i < E; ++i) acc[i] = 0.0f;
   for (int c = c0; c <= c1; c += 32) {
     const int mine = c + lane;
     float2 ml = make_float2(-INFINITY, 0.0f);
-    if (mine <= c1 && total * mine / ctas < total * (mine + 1) / ctas) ml = p.part_ml[slot_of(mine)];  // (or no tiles)
+    if (mine <= c1 && first_of(mine) < first_of(mine + 1)) ml = p.part_ml[slot_of(mine)];  // (or no tiles)
     float top = fmaxf(ref, ml.x);
     for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
     const float keep = ta_share(ref, l, top), f = ta_share(ml.x, ml.y, top);
@@ -811,19 +822,24 @@ __global__ void __launch_bounds__(128) tree_attention_parts_kernel(const TaParam
     for (int o = 16; o > 0; o >>= 1) part += __shfl_xor_sync(0xffffffffu, part, o);
     l = (keep != 0.0f ? l * keep : 0.0f) + part;
 #pragma unroll
-    for (int i = 0; i < D / 32; ++i) acc[i] = keep != 0.0f ? acc[i] * keep : 0.0f;
+    for (int i = 0; i < E; ++i) acc[i] = keep != 0.0f ? acc[i] * keep : 0.0f;
     ref = top;
     const int n = min(32, c1 - c + 1);
 #pragma unroll 8
     for (int k = 0; k < n; ++k) {
       const float g = __shfl_sync(0xffffffffu, f, k);
-      const float* o = p.part_o + slot_of(c + k) * D + lane;
+      float o[E];
+      if constexpr (E == 4) {
+        *reinterpret_cast<float4*>(o) = *reinterpret_cast<const float4*>(p.part_o + slot_of(c + k) * D + lane * E);
+      } else {
+        *reinterpret_cast<float2*>(o) = *reinterpret_cast<const float2*>(p.part_o + slot_of(c + k) * D + lane * E);
+      }
 #pragma unroll
-      for (int i = 0; i < D / 32; ++i) acc[i] += g != 0.0f ? g * o[32 * i] : 0.0f;
+      for (int i = 0; i < E; ++i) acc[i] += g != 0.0f ? g * o[i] : 0.0f;
     }
   }
 #pragma unroll
-  for (int i = 0; i < D / 32; ++i) store_as(p.out, at + lane + 32 * i, p.dtype, l == 0.0f ? 0.0f : acc[i] / l);
+  for (int i = 0; i < E; ++i) store_as(p.out, at + lane * E + i, p.dtype, l == 0.0f ? 0.0f : acc[i] / l);
 }
 
 }  // namespace ojx

@@ -7,7 +7,7 @@
 //   warp 13      loader: page lookups, and TMA copies of K and V.  16-bit rows go straight
 //                into the MMA's swizzled layout (boxes of 8 to 64 rows of one page); runs of
 //                8-bit rows land in a ring of half tiles, with their steps.
-//   warps 0-3    8-bit rows: widen them to f16 in the MMA's layout.  16-bit rows: zero what
+//   warps 0-3    8-bit rows (with warps 16-19): widen them to f16 in the MMA's layout.  16-bit rows: zero what
 //                must not reach a product in a sequence's last tiles; or, where the page size
 //                is no multiple of eight rows, load all rows themselves with cp.async.
 //   warps 4-11   softmax of unit 0 (4-7) and 1 (8-11), one row per thread (TMEM lane).
@@ -30,13 +30,15 @@ namespace ojx {
 
 constexpr int TC_BN = 128;
 constexpr int TC_PRODUCERS = 128;
-constexpr int TC_THREADS = 512;
-// Registers a thread after the split: 128 at launch (65,536 / 512), then 4 x 32 x (112 + 72)
-// + 8 x 32 x 160 = 64,512, within the launch's 65,536.
+// Threads and registers a thread: 16-bit caches 512 with 128 at launch (65,536), then
+// 4 x 32 x (112 + 72) + 8 x 32 x 160 = 64,512; 8-bit caches 640 with 96 at launch (61,440), then
+// 8 x 32 x 64 + 4 x 32 x 64 + 8 x 32 x 144 = 61,440.
 
 template <int FMT, int D, int QT>
 struct TcLayout {
   static constexpr bool QUANT = FMT >= TA_INT8;
+  static constexpr int THREADS = QUANT ? 640 : 512;
+  static constexpr int REGS_IN = QUANT ? 64 : 112, REGS_MMA = QUANT ? 64 : 72, REGS_SOFTMAX = QUANT ? 144 : 160;
   static constexpr int DB = D / 64;
   static constexpr int LEAD = QT == 1 ? 2 : 1;          // K tiles before the first V tile
   static constexpr int TILE = TC_BN * D * 2;            // a K or V tile as the MMA reads it
@@ -193,7 +195,7 @@ __device__ __forceinline__ void tc_commit(uint32_t bar, bool lead) {
 }
 
 template <int FMT, int D, int QT>
-__global__ void __launch_bounds__(TC_THREADS, 1) tree_attention_tc_kernel(const __grid_constant__ CUtensorMap tmK,
+__global__ void __launch_bounds__(TcLayout<FMT, D, QT>::THREADS, 1) tree_attention_tc_kernel(const __grid_constant__ CUtensorMap tmK,
                                                                           const __grid_constant__ CUtensorMap tmV,
                                                                           const TaParams p, uint64_t budget) {
   using L = TcLayout<FMT, D, QT>;
@@ -236,17 +238,17 @@ __global__ void __launch_bounds__(TC_THREADS, 1) tree_attention_tc_kernel(const 
     mbar_init(q_full, 8);
     mbar_init(done_bar, 1);
     for (int s = 0; s < KST; ++s) {
-      mbar_init(k_full(s), tma ? 1 : 4);
+      mbar_init(k_full(s), tma ? 1 : QUANT ? 8 : 4);
       mbar_init(k_empty(s), 1);
     }
     for (int s = 0; s < VST; ++s) {
-      mbar_init(v_full(s), 4);
+      mbar_init(v_full(s), QUANT ? 8 : 4);
       mbar_init(v_empty(s), 1);
       mbar_init(v_land(s), 1);
     }
     for (int s = 0; s < L::RAWS; ++s) {
       mbar_init(raw_full(s), 33);
-      mbar_init(raw_empty(s), 4);
+      mbar_init(raw_empty(s), 8);
     }
     for (int t = 0; t < 2; ++t) {
       mbar_init(s_full(t), 1);
@@ -270,15 +272,15 @@ __global__ void __launch_bounds__(TC_THREADS, 1) tree_attention_tc_kernel(const 
   tc_fence_after();
   const uint32_t tmem = *s_tmem;
 
-  if (warp < 4) {
+  if (warp < 4 || warp >= 16) {
     // ── widening, cleaning, or loading by cp.async ─────────────────────────────────
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 112;");
-    const int tid = threadIdx.x;
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(L::REGS_IN));
+    const int tid = warp < 4 ? threadIdx.x : threadIdx.x - 384;
     TaWalk walk;
     walk.begin(p, *s_share, TC_BN);
     TcCursor in;
     if constexpr (QUANT) {
-      constexpr int CPR = D / 16, PER = TC_BN * CPR / 128;  // 16-byte pieces per row; per thread
+      constexpr int CPR = D / 16, PER = TC_BN * CPR / 256;  // 16-byte pieces per row; per thread
       // Eight neighbouring threads take four pieces of each of two rows, from other halves of
       // the row: then neither their reads nor their two stores each meet a bank twice.
       const int col = D == 128 ? ((tid & 7) + ((tid >> 3) & 1) * 4) & 7 : tid % CPR;
@@ -297,8 +299,8 @@ __global__ void __launch_bounds__(TC_THREADS, 1) tree_attention_tc_kernel(const 
         const uint4* raw = reinterpret_cast<const uint4*>(smem + L::OFF_RAW + slot * L::RAW) + row0 * CPR + col;
         uint4 w[PER];
 #pragma unroll
-        for (int i = 0; i < PER; ++i) w[i] = raw[i * 128];
-        if (!v) {  // the row's steps, and the values' offset of the reference
+        for (int i = 0; i < PER; ++i) w[i] = raw[i * 256];
+        if (!v && warp < 4) {  // the row's steps, and the values' offset of the reference
           const float2 st = *reinterpret_cast<const float2*>(smem + L::OFF_RAWSTEP + (n & 3) * 1024 + tid * 8);
           float ks = st.x, vs = st.y;
           if (tail && !(fabsf(ks) < INFINITY && fabsf(vs) < INFINITY)) {
@@ -322,7 +324,7 @@ __global__ void __launch_bounds__(TC_THREADS, 1) tree_attention_tc_kernel(const 
         if (tail) {
 #pragma unroll
           for (int i = 0; i < PER; ++i)
-            if (row0 + i * (128 / CPR) >= left) w[i] = make_uint4(0, 0, 0, 0);
+            if (row0 + i * (256 / CPR) >= left) w[i] = make_uint4(0, 0, 0, 0);
         }
         __syncwarp();
         if (lane == 0) mbar_arrive(raw_empty(slot));
@@ -333,7 +335,7 @@ __global__ void __launch_bounds__(TC_THREADS, 1) tree_attention_tc_kernel(const 
         bool any = false;
 #pragma unroll
         for (int i = 0; i < PER; ++i) {
-          const int r = row0 + i * (128 / CPR);
+          const int r = row0 + i * (256 / CPR);
           const uint32_t x[4] = {w[i].x, w[i].y, w[i].z, w[i].w};
           uint32_t y[8];
 #pragma unroll
@@ -414,7 +416,7 @@ __global__ void __launch_bounds__(TC_THREADS, 1) tree_attention_tc_kernel(const 
       constexpr int LAG = KST + VST - 1;             // groups in flight before the oldest is handed over
       const int col = tid % CPR;
       // groups committed and not yet handed over, oldest first: (is V, its number, in the tail)
-      uint32_t q_item[LAG + 1];
+      uint32_t q_item[LAG + 1] = {};
       int pending = 0;
       auto where = [&](bool v, uint32_t n, int r) -> uint32_t {
         if (!v) return sK0 + (n % KST) * L::TILE + (col >> 3) * 16384 + r * 128 + (((col & 7) ^ (r & 7)) << 4);
@@ -483,7 +485,7 @@ __global__ void __launch_bounds__(TC_THREADS, 1) tree_attention_tc_kernel(const 
     }
   } else if (warp >= 12) {
     // ── MMA issuer (warps 13-15 only give up registers) ────────────────────────
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(L::REGS_MMA));
     if (warp == 12) {
       // The whole warp runs the loop, with addresses from lane 0, and one lane issues: so the
       // descriptors stay in uniform registers.  (Issued from a branch of one lane, an MMA of
@@ -686,7 +688,7 @@ __global__ void __launch_bounds__(TC_THREADS, 1) tree_attention_tc_kernel(const 
     __syncwarp();
   } else {
     // ── softmax ──────────────────────────────────────────────────────────
-    asm volatile("setmaxnreg.inc.sync.aligned.u32 160;");
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(L::REGS_SOFTMAX));
     const int t = (warp - 4) >> 2;
     const int quarter = warp & 3;
     const int lrow = quarter * 32 + lane;
@@ -1016,6 +1018,7 @@ __global__ void __launch_bounds__(TC_THREADS, 1) tree_attention_tc_kernel(const 
     }
   }
 
+  grid_dep_launch_dependents();  // the join kernel may start; it waits for this grid's end
   tc_fence_before();
   __syncthreads();
   if (warp == 12) {
