@@ -12,8 +12,9 @@
 // (top: 127 for int8, 448 for e4m3); a row with a NaN or an infinity reads back as NaN.
 //
 // Every byte is used once, so these kernels are bound by HBM (a few rows: by latency).
-// A lane holds CH elements of both halves of a pair, so the rotation needs no exchange
-// between lanes, and 32 / lanes-per-row rows share a warp.
+// A lane holds eight elements (where rows are no whole 16-byte vectors: one, several times)
+// of both halves of a pair, so the rotation needs no exchange between lanes, and
+// 32 / lanes-per-row rows share a warp.
 #pragma once
 #include <type_traits>
 #include <cuda_bf16.h>
@@ -52,43 +53,27 @@ __device__ __forceinline__ __nv_bfloat16 from_f32<__nv_bfloat16>(float v) { retu
 template <>
 __device__ __forceinline__ __half from_f32<__half>(float v) { return __float2half_rn(v); }
 
-// CH consecutive elements as fp32.  CH = 8 reads 16-byte vectors (p 16-byte aligned).
-template <typename T, int CH>
-__device__ __forceinline__ void load_chunk(const T* p, float (&v)[CH]) {
-  if constexpr (CH == 8) {
-    constexpr int NV = 8 * sizeof(T) / 16;
-    uint4 raw[NV];
-#pragma unroll
-    for (int i = 0; i < NV; ++i) raw[i] = reinterpret_cast<const uint4*>(p)[i];
-    const T* e = reinterpret_cast<const T*>(raw);
-#pragma unroll
-    for (int i = 0; i < 8; ++i) v[i] = to_f32<T>(e[i]);
-  } else {
-#pragma unroll
-    for (int i = 0; i < CH; ++i) v[i] = to_f32<T>(p[i]);
-  }
+// One element, and eight (16-byte vectors, p 16-byte aligned), of memory whose type is only
+// known at run time (weights).
+__device__ __forceinline__ float load_as(const void* p, int64_t at, int dtype) {
+  if (dtype == OJX_F32) return static_cast<const float*>(p)[at];
+  if (dtype == OJX_BF16) return to_f32(static_cast<const __nv_bfloat16*>(p)[at]);
+  return to_f32(static_cast<const __half*>(p)[at]);
 }
-template <typename T, int CH>
-__device__ __forceinline__ void store_chunk(T* p, const float (&v)[CH]) {
-  if constexpr (CH == 8) {
-    constexpr int NV = 8 * sizeof(T) / 16;
-    uint4 raw[NV];
-    T* e = reinterpret_cast<T*>(raw);
+template <typename T>
+__device__ __forceinline__ void load_eight(const T* p, float (&v)[8]) {
+  constexpr int NV = 8 * sizeof(T) / 16;
+  uint4 raw[NV];
 #pragma unroll
-    for (int i = 0; i < 8; ++i) e[i] = from_f32<T>(v[i]);
+  for (int i = 0; i < NV; ++i) raw[i] = reinterpret_cast<const uint4*>(p)[i];
+  const T* e = reinterpret_cast<const T*>(raw);
 #pragma unroll
-    for (int i = 0; i < NV; ++i) reinterpret_cast<uint4*>(p)[i] = raw[i];
-  } else {
-#pragma unroll
-    for (int i = 0; i < CH; ++i) p[i] = from_f32<T>(v[i]);
-  }
+  for (int i = 0; i < 8; ++i) v[i] = to_f32<T>(e[i]);
 }
-// The same from memory whose type is only known at run time (weights).
-template <int CH>
-__device__ __forceinline__ void load_chunk_as(const void* p, int64_t at, int dtype, float (&v)[CH]) {
-  if (dtype == OJX_F32) load_chunk<float, CH>(static_cast<const float*>(p) + at, v);
-  else if (dtype == OJX_BF16) load_chunk<__nv_bfloat16, CH>(static_cast<const __nv_bfloat16*>(p) + at, v);
-  else load_chunk<__half, CH>(static_cast<const __half*>(p) + at, v);
+__device__ __forceinline__ void load_eight_as(const void* p, int64_t at, int dtype, float (&v)[8]) {
+  if (dtype == OJX_F32) load_eight(static_cast<const float*>(p) + at, v);
+  else if (dtype == OJX_BF16) load_eight(static_cast<const __nv_bfloat16*>(p) + at, v);
+  else load_eight(static_cast<const __half*>(p) + at, v);
 }
 
 __device__ __forceinline__ uint8_t quantise_one(float x, float step, int format) {
@@ -160,41 +145,19 @@ __device__ __forceinline__ bool pair_at(const QkParams& p, int pi, int& a, int& 
   return false;
 }
 
-// Cosines and sines of one pair chunk: cs[e], sn[e] belong to pair e of the chunk pair.
-// (INTER, CH = 8: pairs 0-3 lie in the first chunk, 4-7 in the second.)
-template <int CH, bool INTER>
-__device__ __forceinline__ void load_turn(const QkParams& p, int64_t pos, int a, float (&cs)[CH], float (&sn)[CH]) {
-  const float* row = p.table + pos * p.rotary;
-  const int first = INTER ? a / 2 : a;
-#pragma unroll
-  for (int e = 0; e < CH; ++e) {
-    cs[e] = row[first + e];
-    sn[e] = row[p.half + first + e];
-  }
+// Cosine and sine of the pair whose first element is `a`.
+template <bool INTER>
+__device__ __forceinline__ void load_turn(const QkParams& p, int64_t pos, int a, float& cs, float& sn) {
+  const float* row = p.table + pos * p.rotary + (INTER ? a / 2 : a);
+  cs = row[0];
+  sn = row[p.half];
 }
 
-// Turn a chunk pair by the angle (sign = 1) or back (sign = -1).
-template <int CH, bool INTER>
-__device__ __forceinline__ void turn_pair(float (&xa)[CH], float (&xb)[CH], const float (&cs)[CH],
-                                          const float (&sn)[CH], float sign) {
-  if constexpr (INTER && CH > 1) {
-#pragma unroll
-    for (int e = 0; e < CH / 2; ++e) {
-      float u = xa[2 * e], v = xa[2 * e + 1], s = sign * sn[e];
-      xa[2 * e] = u * cs[e] - v * s;
-      xa[2 * e + 1] = u * s + v * cs[e];
-      u = xb[2 * e], v = xb[2 * e + 1], s = sign * sn[CH / 2 + e];
-      xb[2 * e] = u * cs[CH / 2 + e] - v * s;
-      xb[2 * e + 1] = u * s + v * cs[CH / 2 + e];
-    }
-  } else {
-#pragma unroll
-    for (int e = 0; e < CH; ++e) {
-      const float u = xa[e], v = xb[e], s = sign * sn[e];
-      xa[e] = u * cs[e] - v * s;
-      xb[e] = u * s + v * cs[e];
-    }
-  }
+// Turn a pair by the angle (sign = 1) or back (sign = -1).
+__device__ __forceinline__ void turn_pair(float& xa, float& xb, float cs, float sn, float sign) {
+  const float u = xa, v = xb, s = sign * sn;
+  xa = u * cs - v * s;
+  xb = u * s + v * cs;
 }
 
 __device__ __forceinline__ float group_sum(float v, int lanes) {
@@ -213,26 +176,16 @@ __device__ __forceinline__ int64_t slot_row(const ojx_kv_cache& c, int64_t slot,
   return (page * c.kv_heads + head) * c.page_size + slot % c.page_size;
 }
 
-template <int CH>
-__device__ __forceinline__ void store_cached(void* base, int64_t at, int format, float step, const float (&v)[CH]) {
-  if (format == OJX_KV_BF16) {
-    store_chunk<__nv_bfloat16, CH>(static_cast<__nv_bfloat16*>(base) + at, v);
-  } else if (format == OJX_KV_F16) {
-    store_chunk<__half, CH>(static_cast<__half*>(base) + at, v);
-  } else {
-    uint8_t q[CH];
-#pragma unroll
-    for (int e = 0; e < CH; ++e) q[e] = quantise_one(v[e], step, format);
-    uint8_t* dst = static_cast<uint8_t*>(base) + at;
-#pragma unroll
-    for (int e = 0; e < CH; ++e) dst[e] = q[e];
-  }
+__device__ __forceinline__ void store_cached(void* base, int64_t at, int format, float step, float v) {
+  if (format == OJX_KV_BF16) static_cast<__nv_bfloat16*>(base)[at] = from_f32<__nv_bfloat16>(v);
+  else if (format == OJX_KV_F16) static_cast<__half*>(base)[at] = from_f32<__half>(v);
+  else static_cast<uint8_t*>(base)[at] = quantise_one(v, step, format);
 }
 
 // Forward rows: query and key heads are normed and rotated (p.norm) and stored densely
 // or, keys with k_to_cache and all value heads, into the cache.  A warp takes one token
 // and p.iters row groups of it, so the token's cosines are loaded once for its heads.
-template <typename T, int CH, int NP, bool INTER>
+template <typename T, int NP, bool INTER>
 __global__ void __launch_bounds__(256) qk_rows_kernel(const QkParams p) {
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int sub = lane / p.lanes, j = lane % p.lanes, per_warp = 32 / p.lanes;
@@ -242,7 +195,7 @@ __global__ void __launch_bounds__(256) qk_rows_kernel(const QkParams p) {
   const int heads = p.hq + p.hk + p.hv;
   int head = static_cast<int>(item % p.blocks_per_token) * per_warp * p.iters + sub;
 
-  float cs[NP][CH], sn[NP][CH];
+  float cs[NP], sn[NP];
   if (p.norm) {
     const int64_t pos = load_index(p.positions, token, p.pos64);
     const bool known = pos >= 0 && pos < p.table_rows;
@@ -251,13 +204,10 @@ __global__ void __launch_bounds__(256) qk_rows_kernel(const QkParams p) {
     for (int n = 0; n < NP; ++n) {
       int a = 0, b = 0;
       const int pi = j + n * p.lanes;
-      const bool turns = pi < p.npairs && pair_at<CH, INTER>(p, pi, a, b);
-#pragma unroll
-      for (int e = 0; e < CH; ++e) {
-        cs[n][e] = known ? 1.0f : NAN;  // a token without a position reads as NaN
-        sn[n][e] = 0.0f;
-      }
-      if (turns && known) load_turn<CH, INTER>(p, pos, a, cs[n], sn[n]);
+      const bool turns = pi < p.npairs && pair_at<1, INTER>(p, pi, a, b);
+      cs[n] = known ? 1.0f : NAN;  // a token without a position reads as NaN
+      sn[n] = 0.0f;
+      if (turns && known) load_turn<INTER>(p, pos, a, cs[n], sn[n]);
     }
   }
   const int64_t slot = p.slots ? load_index(p.slots, token, p.slot64) : -1;
@@ -269,21 +219,19 @@ __global__ void __launch_bounds__(256) qk_rows_kernel(const QkParams p) {
     const T* x = is_q   ? static_cast<const T*>(p.q) + token * p.q_st + h * p.q_sh
                  : is_k ? static_cast<const T*>(p.k) + token * p.k_st + h * p.k_sh
                         : static_cast<const T*>(p.v) + token * p.v_st + h * p.v_sh;
-    float xa[NP][CH], xb[NP][CH];
+    float xa[NP], xb[NP];
     float ss = 0.0f;
 #pragma unroll
     for (int n = 0; n < NP; ++n) {
       const int pi = j + n * p.lanes;
-#pragma unroll
-      for (int e = 0; e < CH; ++e) xa[n][e] = xb[n][e] = 0.0f;
+      xa[n] = xb[n] = 0.0f;
       if (valid && pi < p.npairs) {
         int a, b;
-        pair_at<CH, INTER>(p, pi, a, b);
-        load_chunk<T, CH>(x + a, xa[n]);
-        load_chunk<T, CH>(x + b, xb[n]);
+        pair_at<1, INTER>(p, pi, a, b);
+        xa[n] = to_f32<T>(x[a]);
+        xb[n] = to_f32<T>(x[b]);
       }
-#pragma unroll
-      for (int e = 0; e < CH; ++e) ss += xa[n][e] * xa[n][e] + xb[n][e] * xb[n][e];
+      ss += xa[n] * xa[n] + xb[n] * xb[n];
     }
     if (p.norm) {
       ss = group_sum(ss, p.lanes);
@@ -295,18 +243,15 @@ __global__ void __launch_bounds__(256) qk_rows_kernel(const QkParams p) {
           const int pi = j + n * p.lanes;
           if (pi < p.npairs) {
             int a, b;
-            pair_at<CH, INTER>(p, pi, a, b);
-            float wa[CH], wb[CH];
+            pair_at<1, INTER>(p, pi, a, b);
+            float wa = 1.0f, wb = 1.0f;
             if (w) {
-              load_chunk_as<CH>(w, a, p.dtype_w, wa);
-              load_chunk_as<CH>(w, b, p.dtype_w, wb);
+              wa = load_as(w, a, p.dtype_w);
+              wb = load_as(w, b, p.dtype_w);
             }
-#pragma unroll
-            for (int e = 0; e < CH; ++e) {
-              xa[n][e] = xa[n][e] * r * (w ? wa[e] : 1.0f);
-              xb[n][e] = xb[n][e] * r * (w ? wb[e] : 1.0f);
-            }
-            turn_pair<CH, INTER>(xa[n], xb[n], cs[n], sn[n], 1.0f);
+            xa[n] = xa[n] * r * wa;
+            xb[n] = xb[n] * r * wb;
+            turn_pair(xa[n], xb[n], cs[n], sn[n], 1.0f);
           }
         }
       }
@@ -318,8 +263,7 @@ __global__ void __launch_bounds__(256) qk_rows_kernel(const QkParams p) {
       float amax = 0.0f;
 #pragma unroll
       for (int n = 0; n < NP; ++n)
-#pragma unroll
-        for (int e = 0; e < CH; ++e) amax = max_nan(amax, max_nan(fabsf(xa[n][e]), fabsf(xb[n][e])));
+        amax = max_nan(amax, max_nan(fabsf(xa[n]), fabsf(xb[n])));
       for (int o = p.lanes >> 1; o > 0; o >>= 1) amax = max_nan(amax, __shfl_xor_sync(0xffffffffu, amax, o));
       step = quantise_step(amax, p.cache.format);
       if (cached) row = slot_row(p.cache, slot, h);
@@ -333,9 +277,9 @@ __global__ void __launch_bounds__(256) qk_rows_kernel(const QkParams p) {
           const int pi = j + n * p.lanes;
           if (pi < p.npairs) {
             int a, b;
-            pair_at<CH, INTER>(p, pi, a, b);
-            store_cached<CH>(base, row * p.D + a, p.cache.format, step, xa[n]);
-            store_cached<CH>(base, row * p.D + b, p.cache.format, step, xb[n]);
+            pair_at<1, INTER>(p, pi, a, b);
+            store_cached(base, row * p.D + a, p.cache.format, step, xa[n]);
+            store_cached(base, row * p.D + b, p.cache.format, step, xb[n]);
           }
         }
       }
@@ -347,9 +291,9 @@ __global__ void __launch_bounds__(256) qk_rows_kernel(const QkParams p) {
         const int pi = j + n * p.lanes;
         if (pi < p.npairs) {
           int a, b;
-          pair_at<CH, INTER>(p, pi, a, b);
-          store_chunk<T, CH>(out + a, xa[n]);
-          store_chunk<T, CH>(out + b, xb[n]);
+          pair_at<1, INTER>(p, pi, a, b);
+          out[a] = from_f32<T>(xa[n]);
+          out[b] = from_f32<T>(xb[n]);
         }
       }
     }
@@ -359,7 +303,7 @@ __global__ void __launch_bounds__(256) qk_rows_kernel(const QkParams p) {
 // Gradient rows.  Blocks [0, q_blocks) take query heads, the rest key heads; a warp walks
 // tokens and all heads of its side, keeping its share of dw in registers; the block's
 // sum goes to its own row of `partial`, so the result does not depend on timing.
-template <typename T, int CH, int NP, bool INTER>
+template <typename T, int NP, bool INTER>
 __global__ void __launch_bounds__(256) qk_grad_kernel(const QkParams p) {
   extern __shared__ float sw[];  // [warps][D]
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5;
@@ -376,22 +320,19 @@ __global__ void __launch_bounds__(256) qk_grad_kernel(const QkParams p) {
   const void* w = is_q ? p.qw : p.kw;
 
   int at[NP][2];
-  float wa[NP][CH], wb[NP][CH], da[NP][CH], db[NP][CH];
+  float wa[NP], wb[NP], da[NP], db[NP];
   bool on[NP], turns[NP];
 #pragma unroll
   for (int n = 0; n < NP; ++n) {
     const int pi = j + n * p.lanes;
     on[n] = pi < p.npairs;
     at[n][0] = at[n][1] = 0;
-    turns[n] = on[n] && pair_at<CH, INTER>(p, pi, at[n][0], at[n][1]);
-#pragma unroll
-    for (int e = 0; e < CH; ++e) {
-      wa[n][e] = wb[n][e] = 1.0f;
-      da[n][e] = db[n][e] = 0.0f;
-    }
+    turns[n] = on[n] && pair_at<1, INTER>(p, pi, at[n][0], at[n][1]);
+    wa[n] = wb[n] = 1.0f;
+    da[n] = db[n] = 0.0f;
     if (w && on[n]) {
-      load_chunk_as<CH>(w, at[n][0], p.dtype_w, wa[n]);
-      load_chunk_as<CH>(w, at[n][1], p.dtype_w, wb[n]);
+      wa[n] = load_as(w, at[n][0], p.dtype_w);
+      wb[n] = load_as(w, at[n][1], p.dtype_w);
     }
   }
   const int row_groups = (heads + per_warp - 1) / per_warp;
@@ -400,39 +341,32 @@ __global__ void __launch_bounds__(256) qk_grad_kernel(const QkParams p) {
     const int64_t pos = load_index(p.positions, token, p.pos64);
     const bool known = pos >= 0 && pos < p.table_rows;
     if (!known && lane == 0) index_error();
-    float cs[NP][CH], sn[NP][CH];
+    float cs[NP], sn[NP];
 #pragma unroll
     for (int n = 0; n < NP; ++n) {
-#pragma unroll
-      for (int e = 0; e < CH; ++e) {
-        cs[n][e] = known ? 1.0f : NAN;
-        sn[n][e] = 0.0f;
-      }
-      if (turns[n] && known) load_turn<CH, INTER>(p, pos, at[n][0], cs[n], sn[n]);
+      cs[n] = known ? 1.0f : NAN;
+      sn[n] = 0.0f;
+      if (turns[n] && known) load_turn<INTER>(p, pos, at[n][0], cs[n], sn[n]);
     }
     for (int rg = 0; rg < row_groups; ++rg) {
       const int h = rg * per_warp + sub;
       const bool valid = h < heads;
       const T* x = xs + token * x_st + h * x_sh;
       const T* g = gs + token * g_st + h * g_sh;
-      float xa[NP][CH], xb[NP][CH], ga[NP][CH], gb[NP][CH];
+      float xa[NP], xb[NP], ga[NP], gb[NP];
       float ss = 0.0f, hx = 0.0f;
 #pragma unroll
       for (int n = 0; n < NP; ++n) {
-#pragma unroll
-        for (int e = 0; e < CH; ++e) xa[n][e] = xb[n][e] = ga[n][e] = gb[n][e] = 0.0f;
+        xa[n] = xb[n] = ga[n] = gb[n] = 0.0f;
         if (valid && on[n]) {
-          load_chunk<T, CH>(x + at[n][0], xa[n]);
-          load_chunk<T, CH>(x + at[n][1], xb[n]);
-          load_chunk<T, CH>(g + at[n][0], ga[n]);
-          load_chunk<T, CH>(g + at[n][1], gb[n]);
-          turn_pair<CH, INTER>(ga[n], gb[n], cs[n], sn[n], -1.0f);
+          xa[n] = to_f32<T>(x[at[n][0]]);
+          xb[n] = to_f32<T>(x[at[n][1]]);
+          ga[n] = to_f32<T>(g[at[n][0]]);
+          gb[n] = to_f32<T>(g[at[n][1]]);
+          turn_pair(ga[n], gb[n], cs[n], sn[n], -1.0f);
         }
-#pragma unroll
-        for (int e = 0; e < CH; ++e) {
-          ss += xa[n][e] * xa[n][e] + xb[n][e] * xb[n][e];
-          hx += ga[n][e] * wa[n][e] * xa[n][e] + gb[n][e] * wb[n][e] * xb[n][e];
-        }
+        ss += xa[n] * xa[n] + xb[n] * xb[n];
+        hx += ga[n] * wa[n] * xa[n] + gb[n] * wb[n] * xb[n];
       }
       for (int o = p.lanes >> 1; o > 0; o >>= 1) {
         ss += __shfl_xor_sync(0xffffffffu, ss, o);
@@ -445,34 +379,28 @@ __global__ void __launch_bounds__(256) qk_grad_kernel(const QkParams p) {
 #pragma unroll
         for (int n = 0; n < NP; ++n) {
           if (!on[n]) continue;
-          float oa[CH], ob[CH];
-#pragma unroll
-          for (int e = 0; e < CH; ++e) {
-            oa[e] = r * (ga[n][e] * wa[n][e] - xa[n][e] * back);
-            ob[e] = r * (gb[n][e] * wb[n][e] - xb[n][e] * back);
-            da[n][e] += ga[n][e] * (xa[n][e] * r);
-            db[n][e] += gb[n][e] * (xb[n][e] * r);
-          }
-          store_chunk<T, CH>(dx + at[n][0], oa);
-          store_chunk<T, CH>(dx + at[n][1], ob);
+          const float oa = r * (ga[n] * wa[n] - xa[n] * back);
+          const float ob = r * (gb[n] * wb[n] - xb[n] * back);
+          da[n] += ga[n] * (xa[n] * r);
+          db[n] += gb[n] * (xb[n] * r);
+          dx[at[n][0]] = from_f32<T>(oa);
+          dx[at[n][1]] = from_f32<T>(ob);
         }
       }
     }
   }
   // rows of the warp, then warps of the block, in a fixed order
 #pragma unroll
-  for (int n = 0; n < NP; ++n)
-#pragma unroll
-    for (int e = 0; e < CH; ++e) {
-      for (int o = p.lanes; o < 32; o <<= 1) {
-        da[n][e] += __shfl_xor_sync(0xffffffffu, da[n][e], o);
-        db[n][e] += __shfl_xor_sync(0xffffffffu, db[n][e], o);
-      }
-      if (sub == 0 && on[n]) {
-        sw[warp * p.D + at[n][0] + e] = da[n][e];
-        sw[warp * p.D + at[n][1] + e] = db[n][e];
-      }
+  for (int n = 0; n < NP; ++n) {
+    for (int o = p.lanes; o < 32; o <<= 1) {
+      da[n] += __shfl_xor_sync(0xffffffffu, da[n], o);
+      db[n] += __shfl_xor_sync(0xffffffffu, db[n], o);
     }
+    if (sub == 0 && on[n]) {
+      sw[warp * p.D + at[n][0]] = da[n];
+      sw[warp * p.D + at[n][1]] = db[n];
+    }
+  }
   __syncthreads();
   for (int d = threadIdx.x; d < p.D; d += blockDim.x) {
     float s = 0.0f;
@@ -573,7 +501,7 @@ __device__ __forceinline__ void load_weight(const void* w, int at, int dtype, bo
   float v[8];
 #pragma unroll
   for (int e = 0; e < 8; ++e) v[e] = 1.0f;
-  if (w && on) load_chunk_as<8>(w, at, dtype, v);
+  if (w && on) load_eight_as(w, at, dtype, v);
 #pragma unroll
   for (int i = 0; i < 4; ++i) x[i] = f2_pair(v[2 * i], v[2 * i + 1]);
 }
@@ -975,9 +903,7 @@ struct StreamAt {  // the group that is issued, or used, next
 __device__ __forceinline__ void stage_weights(const QkParams& p, float* sw) {
   for (int i = threadIdx.x; i < 2 * p.D; i += blockDim.x) {
     const void* w = i < p.D ? p.qw : p.kw;
-    float v[1] = {1.0f};
-    if (w) load_chunk_as<1>(w, i < p.D ? i : i - p.D, p.dtype_w, v);
-    sw[i] = v[0];
+    sw[i] = w ? load_as(w, i < p.D ? i : i - p.D, p.dtype_w) : 1.0f;
   }
 }
 __device__ __forceinline__ void staged_weight(const float* w, bool on, uint64_t (&x)[4]) {

@@ -67,37 +67,6 @@ struct TcLayout {
 __device__ __forceinline__ void tc_sts128(uint32_t a, uint32_t x, uint32_t y, uint32_t z, uint32_t w) {
   asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(a), "r"(x), "r"(y), "r"(z), "r"(w) : "memory");
 }
-__device__ __forceinline__ float4 tc_lds4f(uint32_t a) {
-  float4 v;
-  asm volatile("ld.shared.v4.f32 {%0,%1,%2,%3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(a) : "memory");
-  return v;
-}
-// Two float32 operations an instruction.
-__device__ __forceinline__ uint64_t tc_pair(float a, float b) {
-  uint64_t r;
-  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
-  return r;
-}
-__device__ __forceinline__ float2 tc_split(uint64_t v) {
-  float2 r;
-  asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(v));
-  return r;
-}
-__device__ __forceinline__ uint64_t tc_fma2(uint64_t a, uint64_t b, uint64_t c) {
-  uint64_t r;
-  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
-  return r;
-}
-__device__ __forceinline__ uint64_t tc_mul2(uint64_t a, uint64_t b) {
-  uint64_t r;
-  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
-  return r;
-}
-__device__ __forceinline__ uint64_t tc_add2(uint64_t a, uint64_t b) {
-  uint64_t r;
-  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
-  return r;
-}
 // Zeroes the non-finite 16-bit elements of a word; true if there were any.
 template <bool BF>
 __device__ __forceinline__ bool tc_clean(uint32_t& w) {
@@ -807,7 +776,7 @@ __global__ void __launch_bounds__(TcLayout<FMT, D, QT>::THREADS, 1) tree_attenti
           above = hi_e > -1000 ? static_cast<float>(hi_e + 1) : -60.0f;
         }
         const uint32_t tS = trow + t * TC_BN;
-        const uint64_t rs2 = tc_pair(row_scale, row_scale);
+        const uint64_t rs2 = f2_pair(row_scale, row_scale);
         float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll 1
         for (int c0 = 0; c0 < TC_BN; c0 += 64) {
@@ -822,8 +791,8 @@ __global__ void __launch_bounds__(TcLayout<FMT, D, QT>::THREADS, 1) tree_attenti
               float2 b = make_float2(__uint_as_float(r[c + 2]), __uint_as_float(r[c + 3]));
               if (QUANT) {
                 const ulonglong2 ks = steps[(c0 + c) / 4];
-                a = tc_split(tc_mul2(tc_pair(a.x, a.y), ks.x));
-                b = tc_split(tc_mul2(tc_pair(b.x, b.y), ks.y));
+                a = f2_split(f2_mul(f2_pair(a.x, a.y), ks.x));
+                b = f2_split(f2_mul(f2_pair(b.x, b.y), ks.y));
               }
               mx[(c >> 2) & 3] = fmaxf(fmaxf(mx[(c >> 2) & 3], fmaxf(a.x, a.y)), fmaxf(b.x, b.y));
             }
@@ -844,7 +813,7 @@ __global__ void __launch_bounds__(TcLayout<FMT, D, QT>::THREADS, 1) tree_attenti
         const float m_new = raise ? top : m_run;
         const float m_use = m_new == -INFINITY ? 0.0f : m_new;
         const float alpha = raise ? ta_exp2(m_run - m_use) : 1.0f;
-        const uint64_t neg2 = tc_pair(-m_use, -m_use);
+        const uint64_t neg2 = f2_pair(-m_use, -m_use);
         uint64_t sum2[2] = {0, 0};
         // (S_t in tensor memory means that the unit's last product is complete, O_t with it)
 #pragma unroll 1
@@ -866,13 +835,13 @@ __global__ void __launch_bounds__(TcLayout<FMT, D, QT>::THREADS, 1) tree_attenti
               }
 #pragma unroll
               for (int h = 0; h < 2; ++h) {
-                uint64_t x = tc_pair(__uint_as_float(r[c + e + 2 * h]), __uint_as_float(r[c + e + 2 * h + 1]));
-                if (QUANT) x = tc_mul2(x, h ? ks.y : ks.x);
-                const float2 a = tc_split(tc_fma2(x, rs2, neg2));
-                uint64_t w2 = tc_pair(ta_exp2(a.x), ta_exp2(a.y));
-                sum2[h] = tc_add2(sum2[h], w2);
-                if (QUANT) w2 = tc_mul2(w2, h ? vs.y : vs.x);
-                const float2 w = tc_split(w2);
+                uint64_t x = f2_pair(__uint_as_float(r[c + e + 2 * h]), __uint_as_float(r[c + e + 2 * h + 1]));
+                if (QUANT) x = f2_mul(x, h ? ks.y : ks.x);
+                const float2 a = f2_split(f2_fma(x, rs2, neg2));
+                uint64_t w2 = f2_pair(ta_exp2(a.x), ta_exp2(a.y));
+                sum2[h] = f2_add(sum2[h], w2);
+                if (QUANT) w2 = f2_mul(w2, h ? vs.y : vs.x);
+                const float2 w = f2_split(w2);
                 const uint32_t pk = ta_pack(w.x, w.y, BF);
                 hi_w[e / 2 + h] = pk;
                 if (BF) lo_w[e / 2 + h] = ta_pack(w.x - __uint_as_float(pk << 16), w.y - __uint_as_float(pk & 0xffff0000u), true);
@@ -884,7 +853,7 @@ __global__ void __launch_bounds__(TcLayout<FMT, D, QT>::THREADS, 1) tree_attenti
         }
         float sum[4];
         {
-          const float2 a = tc_split(sum2[0]), b = tc_split(sum2[1]);
+          const float2 a = f2_split(sum2[0]), b = f2_split(sum2[1]);
           sum[0] = a.x, sum[1] = a.y, sum[2] = b.x, sum[3] = b.y;
         }
         l_run = l_run * alpha + ((sum[0] + sum[1]) + (sum[2] + sum[3]));
