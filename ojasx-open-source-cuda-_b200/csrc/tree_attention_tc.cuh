@@ -770,7 +770,7 @@ __global__ void __launch_bounds__(TcLayout<FMT, D, QT>::THREADS, 1) tree_attenti
         float above = 0.0f;
         bool narrow = true;
         if (QUANT) {
-          const int4 big = *reinterpret_cast<const int4*>(steps + 96), small = *reinterpret_cast<const int4*>(steps + 98);
+          const int4 big = *reinterpret_cast<const int4*>(steps + 96), small = *reinterpret_cast<const int4*>(steps + 97);
           const int hi_e = max(max(big.x, big.y), max(big.z, big.w)), lo_e = min(min(small.x, small.y), min(small.z, small.w));
           narrow = hi_e - lo_e <= 8;
           above = hi_e > -1000 ? static_cast<float>(hi_e + 1) : -60.0f;

@@ -409,6 +409,26 @@ def test_attention_scales_of_any_size(S, fmt):
     within(got[0], want, attention_tolerance(got, want, size))
 
 
+@pytest.mark.parametrize("fmt", ["float16", "int8", "float8"])
+@pytest.mark.parametrize("t,hq,hk,dim", [(6, 4, 1, 128), (12, 4, 1, 64), (24, 4, 1, 128), (40, 8, 2, 64), (40, 4, 1, 128)])
+def test_attention_value_steps_far_apart(S, fmt, t, hq, hk, dim):
+    """Every thirteenth value row is 2^20 times the others, and its key takes almost all of
+    its weight away (a score about 40 below the others'): the output comes from the small
+    rows, whose weights must keep their bits."""
+    n = 300 + t
+    cache = S.KVCache.from_pages(*pages_for(fmt, 32, hk, 16, dim))
+    k, v = rnd(1, n, hk, dim, dtype=torch.float16), rnd(2, n, hk, dim, dtype=torch.float16, scale=2.0 ** -8)
+    q = rnd(3, 1, t, hq, dim, dtype=torch.float16).abs()
+    k[::13] = -50.0 / dim ** 0.5
+    v[::13] *= 2.0 ** 20
+    v[::13] = v[::13].clamp(-60000, 60000)
+    cache.append(k.cuda(), v.cuda(), torch.arange(n).cuda())
+    got = S.tree_attention(q.cuda(), cache, torch.arange(32).int()[None].cuda(), torch.tensor([n - t], dtype=torch.int32).cuda())
+    vis = torch.ones(t, n).tril(n - t).bool()
+    want, size = ref.attend(q[0], ref.stored(k, fmt)[0], ref.stored(v, fmt)[0], vis, dim ** -0.5)
+    within(got[0], want, attention_tolerance(got, want, size))
+
+
 def test_attention_strided_queries_and_shared_mask(S):
     cache = S.KVCache.from_pages(*pages_for("int8", 8, 2, 16, 128))
     x = rnd(1, 128, 2, 128, dtype=torch.bfloat16)
