@@ -92,11 +92,13 @@ static int launch_rows(QkParams& p, int dtype, bool vec, bool inter, cudaStream_
   split = std::min(split, groups);
   p.iters = (groups + split - 1) / split;
   p.blocks_per_token = (groups + p.iters - 1) / p.iters;
-  // Streaming wants every warp to have a ring's worth of groups several times over: from 4
-  // tokens a warp it is the faster form (prefetching in registers: the other).
+  // Streaming wants every warp to have a ring's worth of groups several times over; fewer
+  // tokens leave that to prefetching in registers.  Streamed / prefetched, 40 heads of 128,
+  // bf16: 400 tokens 4.8 / 4.4 us (with int8 caching 8.7 / 9.5), 800 tokens 6.3 / 8.7 (10.2 /
+  // 13.2), 2400 tokens 11.9 / 17.6 (18.7 / 25.5).
   const int sms = current_props().sm_count;
   const bool table_ok = !p.norm || (aligned16(p.table) && p.rotary % 4 == 0);
-  if (vec && table_ok && p.tokens >= 16ll * sms && side_by_side(p.q_sh, p.D, p.hq) && side_by_side(p.k_sh, p.D, p.hk) &&
+  if (vec && table_ok && p.tokens >= 4ll * sms && side_by_side(p.q_sh, p.D, p.hq) && side_by_side(p.k_sh, p.D, p.hk) &&
       side_by_side(p.v_sh, p.D, p.hv)) {
     const int heads_each = (dtype == OJX_F32 ? 1 : 2) * per_warp;
     p.gq = (p.hq + heads_each - 1) / heads_each;
@@ -250,6 +252,13 @@ static int launch_tree_tc(TaParams& p, cudaStream_t s) {
 
 template <int FMT>
 static int launch_tree_fmt(TaParams& p, cudaStream_t s) {
+  // Times for eight sequences of 16000 keys, 8 key heads of 128, in us:
+  //   up to 16 rows the kernel of warp MMAs, which is done when HBM is (16 rows f16 74, e4m3 72);
+  //   beyond them it would pass over the keys again, and tcgen05's takes over, whose time
+  //   hardly depends on the rows (16 rows f16 75, e4m3 137; 64 rows 81, 141);
+  //   up to 8 rows without the second half of a fragment (e4m3, 8 rows 60; 16 rows 72);
+  //   beyond 128 rows two tiles share a pass (132 rows f16: two 110, one after the other 146),
+  //   below it they would halve a tile (96 rows f16: one 84, two 104).
   const int rows = p.tokens * p.group;
   if (rows > 16) {
     const bool two = rows > 128;
@@ -344,7 +353,8 @@ int ojx_qk_norm_rope_backward(const ojx_qk_desc* d, const ojx_rows* gq, const oj
   if (!p.partial) return workspace_error();
   int smem = 8 * p.D * 4;
   const int sms = current_props().sm_count, per_warp = 32 / p.lanes;
-  const bool stream_rows = vec && p.tokens >= 16ll * sms && aligned16(p.table) && p.rotary % 4 == 0 &&
+  // (streamed / prefetched as above: 800 tokens 10.2 / 9.5 us, 1200 11.9 / 12.0, 2400 16.7 / 19.1)
+  const bool stream_rows = vec && p.tokens >= 8ll * sms && aligned16(p.table) && p.rotary % 4 == 0 &&
                            side_by_side(p.q_sh, p.D, p.hq) && side_by_side(p.k_sh, p.D, p.hk) && side_by_side(p.gq_sh, p.D, p.hq) &&
                            side_by_side(p.gk_sh, p.D, p.hk);
   const int heads_each = per_warp * (es == 4 ? 1 : 2);
