@@ -252,7 +252,7 @@ static int launch_tree_tc(TaParams& p, cudaStream_t s) {
 
 template <int FMT>
 static int launch_tree_fmt(TaParams& p, cudaStream_t s) {
-  // Times for eight sequences of 16000 keys, 8 key heads of 128, in us:
+  // Times for eight sequences of up to 16000 keys, 8 key heads of 128, in us:
   //   up to 16 rows the kernel of warp MMAs, which is done when HBM is (16 rows f16 74, e4m3 72);
   //   beyond them it would pass over the keys again, and tcgen05's takes over, whose time
   //   hardly depends on the rows (16 rows f16 75, e4m3 137; 64 rows 81, 141);
