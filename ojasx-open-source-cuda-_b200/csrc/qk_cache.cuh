@@ -185,6 +185,8 @@ __device__ __forceinline__ void store_cached(void* base, int64_t at, int format,
 // Forward rows: query and key heads are normed and rotated (p.norm) and stored densely
 // or, keys with k_to_cache and all value heads, into the cache.  A warp takes one token
 // and p.iters row groups of it, so the token's cosines are loaded once for its heads.
+// For rows that are no whole 16-byte vectors: element loads, whose instructions bound it
+// (4096 tokens of 40 heads of 100, bf16: 68 us, 0.97 TB/s).
 template <typename T, int NP, bool INTER>
 __global__ void __launch_bounds__(256) qk_rows_kernel(const QkParams p) {
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
@@ -302,7 +304,8 @@ __global__ void __launch_bounds__(256) qk_rows_kernel(const QkParams p) {
 
 // Gradient rows.  Blocks [0, q_blocks) take query heads, the rest key heads; a warp walks
 // tokens and all heads of its side, keeping its share of dw in registers; the block's
-// sum goes to its own row of `partial`, so the result does not depend on timing.
+// sum goes to its own row of `partial`, so the result does not depend on timing.  (The
+// same rows: 140 us.)
 template <typename T, int NP, bool INTER>
 __global__ void __launch_bounds__(256) qk_grad_kernel(const QkParams p) {
   extern __shared__ float sw[];  // [warps][D]
@@ -672,7 +675,8 @@ __device__ __forceinline__ void cache_row(const QkParams& p, int64_t slot, bool 
 // Forward rows in 16-byte chunks.  A group is 32 / lanes heads of one side (queries, keys,
 // values) of a token; a warp runs p.iters groups of one token with the next two groups'
 // loads in flight: at 16 warps an SM that covers HBM's latency.  One group at a time took
-// 116 us for 16384 tokens of 40 bf16 heads of 128.
+// 116 us for 16384 tokens of 40 bf16 heads of 128.  A few tokens (8: 3.3 us) are one
+// dependent round of loads.
 template <typename T, bool INTER, bool NORM>
 __global__ void __launch_bounds__(256, 2) qk_rows_fast_kernel(const QkParams p) {
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
@@ -876,7 +880,10 @@ __global__ void __launch_bounds__(256, 2) qk_grad_fast_kernel(const QkParams p) 
 // memory) into the warp's own ring, and with a token's first group the position's row of
 // the table.  A group is two rows a lane (float32: one): what is done once a group, the
 // wait, the next copy and the addresses, then weighs half as much, and instructions are
-// what bounds these kernels once the loads are ahead.
+// what bounds these kernels once the loads are ahead.  16384 tokens of 40 heads of 128, bf16:
+// forward 56 us (6.0 TB/s), gradient 96 us (5.2 TB/s); 8192 tokens of 48 heads, 16 of them to
+// int8 pages, 51 us; append of 50021 tokens of 4 heads, f32 to int8, 76 us (3.4 TB/s: the
+// quotients).
 // (Two float32 rows, with the ring of three that then fits, appended 50021 tokens in 92 us,
 // one with a ring of four in 77.)
 template <typename T>
@@ -1148,7 +1155,7 @@ __device__ __forceinline__ void store_as(void* p, int64_t at, int dtype, float v
 }
 
 // dw of one side: its blocks' partial sums, in 32 interleaved runs of blocks joined in
-// order.  grid (ceil(D / 32), 2), 32 x 32 threads.
+// order.  grid (ceil(D / 32), 2), 32 x 32 threads.  Bound by latency: 3.2 us for 296 blocks.
 __global__ void __launch_bounds__(1024) qk_grad_weight_kernel(const float* partial, int q_blocks, int blocks, int D, void* dqw, void* dkw,
                                                               int dtype) {
   __shared__ float s[32][33];
@@ -1171,7 +1178,7 @@ __global__ void __launch_bounds__(1024) qk_grad_weight_kernel(const float* parti
 
 // Rows of the cache at `slots` as dense [n][heads][D] keys and values; a skipped slot
 // gives zeros.  A thread takes eight elements of a row's key and value, and of the rows
-// two, so four loads are in flight.
+// two, so four loads are in flight.  50021 tokens of 4 heads, int8 to f32: 46 us (5.6 TB/s).
 template <typename T>
 __global__ void __launch_bounds__(256) kv_read_kernel(const ojx_kv_cache c, const void* slots, int slot64, int64_t n,
                                                       T* k_out, T* v_out) {
@@ -1241,7 +1248,8 @@ __global__ void __launch_bounds__(256) kv_read_kernel(const ojx_kv_cache c, cons
 // Moves the rows of the accepted nodes path[b][0..count[b]] of the drafts at context +
 // node to context + 0, 1, ...  One block per (sequence, head); a thread owns a 16-byte
 // column of the rows and moves them in path order.  A node's index is at least its
-// place in the path, so a row is read before a later row is written over it.
+// place in the path, so a row is read before a later row is written over it.  64 sequences,
+// 5 accepted of 48: 8.2 us, the latency of a chain of moves.
 __global__ void __launch_bounds__(128) kv_keep_path_kernel(const ojx_kv_cache c, const int32_t* page_table, int width,
                                                            const int32_t* contexts, const int32_t* path,
                                                            const int32_t* count, int tokens) {

@@ -128,6 +128,10 @@ static int launch_rows(QkParams& p, int dtype, bool vec, bool inter, cudaStream_
     if (vec && !p.norm) qk_rows_fast_kernel<T, false, false><<<gr, 256, 0, s>>>(p);
     else if (vec && !inter) qk_rows_fast_kernel<T, false, true><<<gr, 256, 0, s>>>(p);
     else if (vec) qk_rows_fast_kernel<T, true, true><<<gr, 256, 0, s>>>(p);
+    // (rows of up to 128 elements hold two pairs a lane, not eight: 4096 tokens of 40 heads of
+    // 100, bf16, 68 us against 162; their gradient 140 against 307)
+    else if (p.npairs <= 64 && !inter) qk_rows_kernel<T, 2, false><<<gr, 256, 0, s>>>(p);
+    else if (p.npairs <= 64) qk_rows_kernel<T, 2, true><<<gr, 256, 0, s>>>(p);
     else if (!inter) qk_rows_kernel<T, 8, false><<<gr, 256, 0, s>>>(p);
     else qk_rows_kernel<T, 8, true><<<gr, 256, 0, s>>>(p);
     return launched("qk_rows launch");
@@ -378,6 +382,8 @@ int ojx_qk_norm_rope_backward(const ojx_qk_desc* d, const ojx_rows* gq, const oj
     }
     if (vec && !inter) qk_grad_fast_kernel<T, false><<<blocks, 256, smem, s>>>(p);
     else if (vec) qk_grad_fast_kernel<T, true><<<blocks, 256, smem, s>>>(p);
+    else if (p.npairs <= 64 && !inter) qk_grad_kernel<T, 2, false><<<blocks, 256, smem, s>>>(p);
+    else if (p.npairs <= 64) qk_grad_kernel<T, 2, true><<<blocks, 256, smem, s>>>(p);
     else if (!inter) qk_grad_kernel<T, 8, false><<<blocks, 256, smem, s>>>(p);
     else qk_grad_kernel<T, 8, true><<<blocks, 256, smem, s>>>(p);
     return launched("qk_grad launch");

