@@ -207,6 +207,22 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor, at::Tensor> qk_backward(const at:
   return {dq, dk, dqw, dkw};
 }
 
+// The gradient as a step of a graph (create_graph): its own derivative is refused, not
+// silently left out.
+struct QkGradOnce : torch::autograd::Function<QkGradOnce> {
+  static torch::autograd::variable_list forward(torch::autograd::AutogradContext*, const at::Tensor& gq, const at::Tensor& gk,
+                                                const at::Tensor& q, const at::Tensor& k, const MaybeTensor& qw, const MaybeTensor& kw,
+                                                const at::Tensor& table, const at::Tensor& positions, double eps, bool interleaved,
+                                                bool weights) {
+    auto [dq, dk, dqw, dkw] = qk_backward(gq, gk, q, k, qw, kw, table, positions, eps, interleaved, weights);
+    auto some = [&](const at::Tensor& t) { return t.defined() ? t : at::empty({0}, q.options()); };
+    return {dq, dk, some(dqw), some(dkw)};
+  }
+  static torch::autograd::variable_list backward(torch::autograd::AutogradContext*, torch::autograd::variable_list) {
+    throw std::runtime_error("qk_norm_rope: differentiable once");
+  }
+};
+
 struct QkFunction : torch::autograd::Function<QkFunction> {
   static torch::autograd::variable_list forward(torch::autograd::AutogradContext* ctx, const at::Tensor& q, const at::Tensor& k,
                                                 const MaybeTensor& qw, const MaybeTensor& kw, const at::Tensor& table,
@@ -223,6 +239,13 @@ struct QkFunction : torch::autograd::Function<QkFunction> {
     auto maybe = [](const at::Tensor& t) { return t.defined() ? MaybeTensor(t) : MaybeTensor(); };
     const at::Tensor gq = grads[0].defined() ? grads[0] : at::zeros_like(s[0], at::MemoryFormat::Contiguous);
     const at::Tensor gk = grads[1].defined() ? grads[1] : at::zeros_like(s[1], at::MemoryFormat::Contiguous);
+    if (at::GradMode::is_enabled()) {
+      auto out = QkGradOnce::apply(gq, gk, s[0], s[1], maybe(s[2]), maybe(s[3]), s[4], s[5], ctx->saved_data["eps"].toDouble(),
+                                   ctx->saved_data["interleaved"].toBool(), ctx->saved_data["weights"].toBool());
+      const bool w = ctx->saved_data["weights"].toBool();
+      return {out[0], out[1], w && s[2].defined() ? out[2] : at::Tensor(), w && s[3].defined() ? out[3] : at::Tensor(),
+              at::Tensor(), at::Tensor(), at::Tensor(), at::Tensor()};
+    }
     auto [dq, dk, dqw, dkw] = qk_backward(gq, gk, s[0], s[1], maybe(s[2]), maybe(s[3]), s[4], s[5], ctx->saved_data["eps"].toDouble(),
                                           ctx->saved_data["interleaved"].toBool(), ctx->saved_data["weights"].toBool());
     return {dq, dk, dqw, dkw, at::Tensor(), at::Tensor(), at::Tensor(), at::Tensor()};

@@ -143,6 +143,7 @@ class QKNormRopeFunction(torch.autograd.Function):
         return _qk_forward(q, k, q_weight, k_weight, table, positions, eps, interleaved)
 
     @staticmethod
+    @torch.autograd.function.once_differentiable
     def backward(ctx, grad_q, grad_k):
         from torchcl.serving import _qk_backward
         q, k, q_weight, k_weight, table, positions = ctx.saved_tensors

@@ -201,7 +201,8 @@ def qk_norm_rope(q, k, q_weight, k_weight, table, positions, eps: float = 1e-6, 
     a position outside the table gives NaN and ValueError at the next synchronize).
     Pairs are (i, i + rotary_dim/2), or (2i, 2i + 1) when `interleaved`.  Sums run in
     fp32; outputs are rounded once to the inputs' dtype.  Returns dense (q, k).
-    Differentiable in q, k and the weights (QKNormRopeFunction)."""
+    Differentiable once in q, k and the weights (QKNormRopeFunction); a derivative of its
+    gradient raises RuntimeError."""
     if _cuda(q):
         return L.torch_binding().qk_norm_rope(q, k, q_weight, k_weight, table, positions, eps, interleaved)
     if torch.is_grad_enabled() and any(getattr(t, "requires_grad", False) for t in (q, k, q_weight, k_weight)):

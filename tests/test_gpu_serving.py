@@ -83,6 +83,25 @@ def test_qk_backward(S, tokens, hq, hk, dim, rotary, inter, dtype):
         within(dw, dwant, u * dwant.abs() + (64 + rows) * F32 * dsize)
 
 
+@pytest.mark.parametrize("weighted", [True, False])
+def test_qk_gradient_in_a_graph(S, weighted):
+    """create_graph changes no gradient, and a second derivative is refused."""
+    q, k = rnd(1, 7, 4, 64).cuda().requires_grad_(), rnd(2, 7, 2, 64).cuda().requires_grad_()
+    w = rnd(3, 64).cuda().requires_grad_() if weighted else None
+    table, pos = S.rope_table(16, 64).cuda(), torch.arange(7, dtype=torch.int32).cuda()
+    inputs = [t for t in (q, k, w) if t is not None]
+
+    def loss():
+        a, b = S.qk_norm_rope(q, k, w, None, table, pos)
+        return (a * a * a).sum() + b.sum()
+
+    plain = torch.autograd.grad(loss(), inputs)
+    kept = torch.autograd.grad(loss(), inputs, create_graph=True)
+    assert all(torch.equal(a, b) for a, b in zip(plain, kept))
+    with pytest.raises(RuntimeError, match="differentiable once"):
+        torch.autograd.grad(kept[0].sum(), q)
+
+
 def test_qk_gradient_against_differences(S):
     """<grad, v> against (L(x + hv) - L(x - hv)) / 2h, L = sum(g y) of the float32 kernel.
     Error: h^2/6 L''' <= h^2 * |g| (third derivatives of a normalised row are O(1) for rows
