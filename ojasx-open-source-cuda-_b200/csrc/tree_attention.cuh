@@ -8,10 +8,10 @@
 //
 // A quantised key is an 8-bit vector times a step, so the products run on the stored
 // values, which are exact in f16, and the step multiplies the score: s_j = step_kj * (q.k8_j).
-// For the values the step joins the weight: sum_j (p_j step_vj) v8_j.  The weights of a row
-// are kept below one by measuring them against the largest s_j + log2(step_vj) instead of
-// the largest s_j, so they use f16's range whatever the steps are.  A bf16 query row is
-// brought into f16's range by a power of two, which the score's factor takes back.
+// For the values the step joins the weight: sum_j (p_j step_vj) v8_j.  A row measures its
+// weights against the largest s_j + log2(step_vj) instead of the largest s_j, so they use
+// f16's range whatever the steps are (see TA_BIAS).  A bf16 query row is brought into f16's
+// range by a power of two, which the score's factor takes back.
 //
 // Up to 16 rows a key head, this file: each key and value is read once, so HBM bounds 16-bit
 // caches (64 sequences of up to 8191 keys, 8 key heads of 128, 4 rows: 223 us, 6.5 TB/s) and
@@ -45,6 +45,29 @@ struct TaParams {
 };
 
 constexpr int TA_F16 = 0, TA_BF16 = 1, TA_INT8 = 2, TA_FP8 = 3;
+
+// Weights enter the second product in f16 (over bf16 values: as two bf16 numbers): 11 bits,
+// which is what the output's own rounding to f16 keeps; the sum of the weights stays in
+// fp32.  A row's largest weight (times its value's step) lies near 2^7 when its reference is
+// set and below 2^15 until the reference moves, so weights keep their 11 bits down to 2^-21
+// of the largest and contribute down to 2^-31 of it: a long context whose keys share what
+// one large score leaves is not lost.  (With the largest at one, and steps 2^8 apart taken
+// as the largest of them, 65536 keys of 2^-16 of the largest weight each added nothing.)
+constexpr float TA_BIAS = 7.0f;
+// Value steps whose powers of two differ by no more than this are taken as the largest of
+// their block, which costs that many of the bits above.
+constexpr int TA_NEAR = 2;
+// log2 of the value steps that weights are measured in.  Above, no product passes f16's range
+// up to the largest float there is (2^121 a step); the weights' own sum keeps 2^-11 of the
+// largest weight at 2^121, 2^-32 at 2^100.  Below, a sum of 2^17 weights stays in fp32's range;
+// smaller steps lose the weights' bits one by one.
+constexpr int TA_STEP_LOW = -90, TA_STEP_HIGH = 122;
+__device__ __forceinline__ int ta_step_exponent(float step) {
+  return min(max(static_cast<int>((__float_as_uint(step) >> 23) & 255) - 127, TA_STEP_LOW), TA_STEP_HIGH);
+}
+__device__ __forceinline__ float ta_step_log2(float step) {
+  return fminf(fmaxf(__log2f(step), static_cast<float>(TA_STEP_LOW)), static_cast<float>(TA_STEP_HIGH));
+}
 
 __device__ __forceinline__ float ta_exp2(float x) {
   float y;
@@ -538,19 +561,19 @@ __global__ void __launch_bounds__(TaLayout<FMT, D, FEW>::NW * 32, 1) tree_attent
       float above = 0.0f;
       bool narrow = true;
       if constexpr (QUANT) {
-        // value steps of one block that differ by less than 2^8: the largest stands for all
+        // value steps of one block that lie close together: the largest stands for all
         const float own = k0 + lane < hi ? ld_shared_f32(sk + 2 * L::TILE + lane * 8 + 4) : 0.0f;
-        const int e = min(max(static_cast<int>((__float_as_uint(own) >> 23) & 255) - 127, -60), 60);
+        const int e = ta_step_exponent(own);
         const int big = __reduce_max_sync(0xffffffffu, own > 0.0f ? e : -1000);
         const int small = __reduce_min_sync(0xffffffffu, own > 0.0f ? e : 1000);
-        narrow = big - small <= 8;
-        above = big > -1000 ? static_cast<float>(big + 1) : -60.0f;
+        narrow = big - small <= TA_NEAR;
+        above = static_cast<float>(big > -1000 ? big + 1 : TA_STEP_LOW);
 #pragma unroll
         for (int j = 0; j < NT; ++j) {
           const float4 st = ta_lds4f(sk + 2 * L::TILE + (8 * j + 2 * t) * 8);
           ks2[j][0] = st.x, vs2[j][0] = st.y, ks2[j][1] = st.z, vs2[j][1] = st.w;
 #pragma unroll
-          for (int c = 0; c < 2; ++c) lv[j][c] = narrow ? above : fminf(fmaxf(__log2f(vs2[j][c]), -60.0f), 60.0f);
+          for (int c = 0; c < 2; ++c) lv[j][c] = narrow ? above : ta_step_log2(vs2[j][c]);
         }
       }
 
@@ -579,7 +602,8 @@ __global__ void __launch_bounds__(TaLayout<FMT, D, FEW>::NW * 32, 1) tree_attent
       for (int half = 0; half < H; ++half) {
         top[half] = fmaxf(top[half], __shfl_xor_sync(0xffffffffu, top[half], 1));
         top[half] = fmaxf(top[half], __shfl_xor_sync(0xffffffffu, top[half], 2));
-        // the reference moves only when a weight would pass 2^8, so o is seldom rescaled
+        if (!BF) top[half] -= TA_BIAS;
+        // the reference moves only when a weight would pass 2^15 (bf16: 2^8), so o is seldom rescaled
         const bool raise = top[half] > ref[half] + 8.0f;
         const float next = raise ? top[half] : ref[half];
         use[half] = next == -INFINITY ? 0.0f : next;

@@ -285,9 +285,9 @@ __global__ void __launch_bounds__(TcLayout<FMT, D, QT>::THREADS, 1) tree_attenti
           float* d = reinterpret_cast<float*>(smem + L::OFF_STEPS + (n % L::STEPS) * L::STEP_BYTES) + tid;
           d[0] = ks == 0.0f ? 1.17549435e-38f : ks;  // (a row of zeros: its products are zero, and a hidden score stays -inf)
           d[128] = vs;
-          d[256] = fminf(fmaxf(__log2f(vs), -60.0f), 60.0f);
+          d[256] = ta_step_log2(vs);
           // the largest and the smallest power of two among the rows' steps
-          const int e = min(max(static_cast<int>((__float_as_uint(vs) >> 23) & 255) - 127, -60), 60);
+          const int e = ta_step_exponent(vs);
           const int big = __reduce_max_sync(0xffffffffu, vs > 0.0f ? e : -1000);
           const int small = __reduce_min_sync(0xffffffffu, vs > 0.0f ? e : 1000);
           if (lane == 0) {
@@ -771,15 +771,15 @@ __global__ void __launch_bounds__(TcLayout<FMT, D, QT>::THREADS, 1) tree_attenti
         // Two passes over the scores in tensor memory, 64 columns an iteration: the loops stay
         // small, for what bounds a fully unrolled row is the fetching of its instructions.
         const ulonglong2* steps = reinterpret_cast<const ulonglong2*>(smem + L::OFF_STEPS + ((tile_no + j) % (L::STEPS ? L::STEPS : 1)) * L::STEP_BYTES);
-        // Value steps of one tile seldom differ by more than 2^8: then the largest stands for
-        // all (weights keep 2^-22 of the largest, f16's range), and no offset is read a key.
-        float above = 0.0f;
+        // Value steps of one tile seldom lie far apart: then the largest stands for all, and no
+        // offset is read a key.
+        float above = BF ? 0.0f : -TA_BIAS;
         bool narrow = true;
         if (QUANT) {
           const int4 big = *reinterpret_cast<const int4*>(steps + 96), small = *reinterpret_cast<const int4*>(steps + 97);
           const int hi_e = max(max(big.x, big.y), max(big.z, big.w)), lo_e = min(min(small.x, small.y), min(small.z, small.w));
-          narrow = hi_e - lo_e <= 8;
-          above = hi_e > -1000 ? static_cast<float>(hi_e + 1) : -60.0f;
+          narrow = hi_e - lo_e <= TA_NEAR;
+          above += static_cast<float>(hi_e > -1000 ? hi_e + 1 : TA_STEP_LOW);
         }
         const uint32_t tS = trow + t * TC_BN;
         const uint64_t rs2 = f2_pair(row_scale, row_scale);
@@ -815,6 +815,7 @@ __global__ void __launch_bounds__(TcLayout<FMT, D, QT>::THREADS, 1) tree_attenti
         }
         float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
         if (narrow) top = fmaf(top, row_scale, above);  // (row_scale is positive: the largest stays the largest)
+        else top -= TA_BIAS;
         const bool raise = valid && top > m_run + 8.0f;
         const float m_new = raise ? top : m_run;
         const float m_use = m_new == -INFINITY ? 0.0f : m_new;
