@@ -48,7 +48,10 @@ constexpr int TA_F16 = 0, TA_BF16 = 1, TA_INT8 = 2, TA_FP8 = 3;
 
 // Weights enter the second product in f16 (over bf16 values: as two bf16 numbers): 11 bits,
 // which is what the output's own rounding to f16 keeps; the sum of the weights stays in
-// fp32.  A row's largest weight (times its value's step) lies near 2^7 when its reference is
+// fp32.  (With a second product for their next bits, f16 queries over e4m3 were off by 2.1e-4
+// of the output's norm instead of 2.9e-4, bf16 queries over int8 by 1.7e-3 either way; eight
+// trees of 48 nodes took 269 us instead of 231, a decoding batch of 64 took 202 instead of
+// 184.)  A row's largest weight (times its value's step) lies near 2^7 when its reference is
 // set and below 2^15 until the reference moves, so weights keep their 11 bits down to 2^-21
 // of the largest and contribute down to 2^-31 of it: a long context whose keys share what
 // one large score leaves is not lost.  (With the largest at one, and steps 2^8 apart taken
