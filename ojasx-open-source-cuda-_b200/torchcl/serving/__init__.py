@@ -25,6 +25,7 @@ import torch
 from torchcl import _lib as L
 from torchcl.api import _get_buf, _get_dtype, _get_shape, _wrap_output, is_opencl_tensor, to_opencl
 from torchcl.ops.engine import ojx_dtype
+from torchcl.runtime import context as _ctx
 from torchcl.runtime.context import get_queue
 from torchcl.runtime.memory import CLBuffer, get_buffer_pool, note_use
 
@@ -245,8 +246,8 @@ class KVCache:
     which pages make up a sequence is the caller's page table.  head_dim is a multiple of
     16 up to 512 (64 or 128 for tree_attention).
 
-    The constructor takes zeroed pages from torchcl's pool; from_pages wraps tensors that
-    exist.  Calls that share a cache are ordered by their streams, as for any buffer; a
+    The constructor takes zeroed pages from torchcl's pool (it returns when they are clear);
+    from_pages wraps tensors that exist.  Calls that share a cache are ordered by their streams, as for any buffer; a
     slot given twice in one call holds one of the two."""
 
     def __init__(self, num_pages: int, page_size: int, kv_heads: int, head_dim: int, format: str = "int8"):
@@ -264,6 +265,8 @@ class KVCache:
         for buf in self._pages:
             if buf is not None:
                 pool.zero_fill(buf)
+        if not _ctx._capture_active:  # calls on any stream may follow: the pages are clear by then
+            L.check(L.lib().ojx_stream_synchronize(get_queue()), "KVCache")
         self._owned = True
         self._set(num_pages, page_size, kv_heads, head_dim, format)
 
