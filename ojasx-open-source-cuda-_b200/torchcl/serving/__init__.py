@@ -19,6 +19,7 @@ from __future__ import annotations
 
 import ctypes
 import math
+import threading
 
 import torch
 
@@ -229,12 +230,40 @@ def qkv_to_cache(q, k, v, q_weight, k_weight, table, positions, cache: "KVCache"
     if math.prod(sa.shape) != d.tokens:
         raise ValueError(f"slots: {sa.shape} for {d.tokens} tokens")
     q_out, qp = _empty(_get_shape(q), dtype, on_torch)
-    L.check(L.lib().ojx_qkv_to_cache(_ref(d), _ref(v_rows), qp, _ref(cache._use()), sa.ptr,
+    L.check(L.lib().ojx_qkv_to_cache(_ref(d), _ref(v_rows), qp, _ref(cache._use(False)), sa.ptr,
                                      int(sa.dtype == torch.int64), _stream(on_torch)), "qkv_to_cache")
     return q_out
 
 
 # ── the cache ────────────────────────────────────────────────────────────────
+
+_dropped: list = []  # (device, pages) of caches that are gone, which calls may still use
+_dropped_lock = threading.RLock()  # reentrant: a finalizer runs wherever a collection starts
+
+
+def _free_pages(pages) -> None:
+    for buf in pages:
+        if isinstance(buf, CLBuffer):
+            get_buffer_pool().free(buf)
+
+
+def _capturing() -> bool:
+    return _ctx._capture_active or torch.cuda.is_current_stream_capturing()
+
+
+def _give_back() -> None:
+    """Return the pages of dropped caches to their allocators, once the device is done with
+    them.  A capture allows no wait: then they stay until the next cache is made or dropped."""
+    if not _dropped or _capturing():
+        return
+    with _dropped_lock:
+        batch = list(_dropped)
+        _dropped.clear()
+    for device in {d for d, _ in batch}:
+        torch.cuda.synchronize(device)
+    for _, pages in batch:
+        _free_pages(pages)
+
 
 class KVCache:
     """Keys and values in pages [num_pages, kv_heads, page_size, head_dim].
@@ -247,8 +276,11 @@ class KVCache:
     16 up to 512 (64 or 128 for tree_attention).
 
     The constructor takes zeroed pages from torchcl's pool (it returns when they are clear);
-    from_pages wraps tensors that exist.  Calls that share a cache are ordered by their streams, as for any buffer; a
-    slot given twice in one call holds one of the two."""
+    from_pages wraps tensors that exist.  Dropping a cache whose pages were used on the other
+    side's streams (torchcl's pages in calls on torch tensors, or torch's in calls on handles)
+    waits for the device before the pages go back; during a graph capture they go back later.
+    A graph of such calls needs the cache kept.  Calls that share a cache are ordered by their
+    streams, as for any buffer; a slot given twice in one call holds one of the two."""
 
     def __init__(self, num_pages: int, page_size: int, kv_heads: int, head_dim: int, format: str = "int8"):
         if format not in _FORMAT_DTYPES:
@@ -257,6 +289,7 @@ class KVCache:
             raise ValueError("a cache has at least one page, row and head")
         if head_dim < 16 or head_dim > 512 or head_dim % 16:
             raise ValueError(f"head_dim {head_dim} is not a multiple of 16 up to 512")
+        _give_back()
         pool = get_buffer_pool()
         rows = num_pages * page_size * kv_heads
         quantised = format in ("int8", "float8")
@@ -271,12 +304,15 @@ class KVCache:
         self._set(num_pages, page_size, kv_heads, head_dim, format)
 
     def __del__(self):
-        if getattr(self, "_owned", False):
-            for buf in self._pages:
-                try:
-                    get_buffer_pool().free(buf)
-                except Exception:
-                    pass
+        try:
+            if getattr(self, "_shared", False):
+                with _dropped_lock:
+                    _dropped.append((self._device, self._pages))
+                _give_back()
+            elif getattr(self, "_owned", False):
+                _free_pages(self._pages)
+        except Exception:
+            pass
 
     @classmethod
     def from_pages(cls, k_pages, v_pages, k_scale=None, v_scale=None) -> "KVCache":
@@ -312,13 +348,17 @@ class KVCache:
     def _set(self, num_pages, page_size, kv_heads, head_dim, format):
         self.num_pages, self.page_size, self.kv_heads = num_pages, page_size, kv_heads
         self.head_dim, self.format = head_dim, format
+        self._device = _ctx.get_device() if self._owned else self._pages[0].device.index
         addr = [None if b is None else b.buffer if isinstance(b, CLBuffer) else b.data_ptr() for b in self._pages]
         self._pooled = any(isinstance(b, CLBuffer) for b in self._pages)
         self._desc = L.KVCacheDesc(*addr, num_pages, page_size, kv_heads, head_dim, L.KV_FORMATS[format])
 
         self._where = ctypes.addressof(self._desc)
+        self._shared = False  # used by calls that its pages' allocator knows nothing of
 
-    def _use(self) -> "L.KVCacheDesc":
+    def _use(self, on_torch: bool) -> "L.KVCacheDesc":
+        if self._pooled == on_torch:
+            self._shared = True
         if self._pooled:
             for buf in self._pages:
                 if buf is not None:
@@ -326,7 +366,7 @@ class KVCache:
         return self._desc
 
     def _address(self) -> int:
-        self._use()
+        self._use(True)
         return self._where
 
     def append(self, k, v, slots) -> None:
@@ -344,7 +384,7 @@ class KVCache:
         sa = _Arg(slots, on_torch, "slots", _INTS, integer=True)
         if math.prod(sa.shape) != n:
             raise ValueError(f"slots: {sa.shape} for {n} tokens")
-        L.check(L.lib().ojx_kv_append(_ref(self._use()), _ref(k_rows), _ref(v_rows), ojx_dtype(ka.dtype), n, sa.ptr,
+        L.check(L.lib().ojx_kv_append(_ref(self._use(False)), _ref(k_rows), _ref(v_rows), ojx_dtype(ka.dtype), n, sa.ptr,
                                       int(sa.dtype == torch.int64), _stream(on_torch)), "KVCache.append")
 
     def read(self, slots, dtype: torch.dtype = torch.bfloat16):
@@ -359,7 +399,7 @@ class KVCache:
         shape = (*sa.shape, self.kv_heads, self.head_dim)
         k, kp = _empty(shape, dtype, on_torch)
         v, vp = _empty(shape, dtype, on_torch)
-        L.check(L.lib().ojx_kv_read(_ref(self._use()), kp, vp, code, n, sa.ptr, int(sa.dtype == torch.int64),
+        L.check(L.lib().ojx_kv_read(_ref(self._use(False)), kp, vp, code, n, sa.ptr, int(sa.dtype == torch.int64),
                                     _stream(on_torch)), "KVCache.read")
         return k, v
 
@@ -377,7 +417,7 @@ class KVCache:
         batch, tokens = pa.shape
         if ta.shape[0] != batch or ca.shape != (batch,) or na.shape != (batch,):
             raise ValueError(f"page_table {ta.shape}, context_lens {ca.shape}, count {na.shape} for {batch} sequences")
-        L.check(L.lib().ojx_kv_keep_path(_ref(self._use()), ta.ptr, ta.shape[1], ca.ptr, pa.ptr, na.ptr, batch, tokens,
+        L.check(L.lib().ojx_kv_keep_path(_ref(self._use(on_torch)), ta.ptr, ta.shape[1], ca.ptr, pa.ptr, na.ptr, batch, tokens,
                                          _stream(on_torch)), "KVCache.keep_path")
 
 
@@ -442,7 +482,7 @@ def tree_attention(q, cache: KVCache, page_table, context_lens, mask=None, draft
             raise ValueError(f"mask: shape {ma.shape} is neither {rows} nor {(batch, *rows)}")
     out, op = _empty(qa.shape, qa.dtype, on_torch)
     d = L.TreeAttentionDesc()
-    d.cache = cache._use()
+    d.cache = cache._use(False)
     d.q, d.out = qa.ptr, op
     d.q_stride_b, d.q_stride_t, d.q_stride_h = qa.strides[:3]
     d.dtype, d.batch, d.tokens, d.q_heads = ojx_dtype(qa.dtype), batch, tokens, heads

@@ -1,5 +1,5 @@
 """The serving operators beside other work: caches made on torchcl's stream and used on
-torch's."""
+torch's, and caches dropped while calls run."""
 import pytest
 import torch
 
@@ -42,3 +42,70 @@ def test_a_new_cache_is_cleared_before_its_first_use(S, side):
     k, v = cache.read(slots)
     assert torch.equal(k, x) and torch.equal(v, -x)
     assert not cache.read(slots - 2)[0][1:].any()
+
+
+def test_pages_freed_while_torch_still_uses_them(S):
+    """A cache deleted while a call on torch's stream waits to run: its pages are not those of
+    the next cache, whose clearing would reach the call."""
+    x = rnd(2, 64, 2, 64, dtype=torch.float16).cuda()
+    slots = torch.arange(64).cuda()
+    cache = S.KVCache(64, 16, 2, 64, "float16")
+    cache.append(x, x, slots)
+    torch.cuda.synchronize()
+    side = torch.cuda.Stream()
+    with torch.cuda.stream(side):
+        torch.cuda._sleep(LONG)
+        k, v = cache.read(slots, dtype=torch.float16)
+    del cache
+    others = [S.KVCache(64, 16, 2, 64, "float16") for _ in range(3)]
+    torch.cuda.synchronize()
+    assert torch.equal(k, x) and torch.equal(v, x)
+    assert not others[0].read(slots)[0].any()
+
+
+def test_freed_pages_come_back(S):
+    """Caches made, used on torch's stream and dropped in a loop do not add up."""
+    from torchcl.runtime.memory import get_buffer_pool
+    x = rnd(3, 4, 4, 128, dtype=torch.float16).cuda()
+    used = []
+    for _ in range(12):
+        cache = S.KVCache(1 << 12, 64, 4, 128, "float16")
+        cache.append(x, x, torch.arange(4).cuda())
+        torch.cuda.synchronize()
+        del cache
+        used.append(get_buffer_pool().get_stats()["total_allocated_bytes"])
+    assert used[-1] == used[2]
+
+
+def test_torch_pages_freed_while_torchcl_still_uses_them(S):
+    import torchcl
+    n = 1 << 14
+    x = rnd(4, n, 2, 64, dtype=torch.float16)
+    cache = S.KVCache.from_pages(*pages_for("float16", n // 16, 2, 16, 64))
+    cache.append(x.cuda(), x.cuda(), torch.arange(n).cuda())
+    torch.cuda.synchronize()
+    slots = torchcl.to_opencl(torch.arange(n).int())
+    cache.read(slots, dtype=torch.float16)
+    torch.full((8,), 7.0, dtype=torch.float16, device="cuda")  # (loads the kernel)
+    torch.cuda.synchronize()
+    busy_torchcl()
+    k, _ = cache.read(slots, dtype=torch.float16)
+    del cache
+    waste = [torch.full((n // 16, 2, 16, 64), 7.0, dtype=torch.float16, device="cuda") for _ in range(4)]
+    torch.cuda.synchronize()
+    assert torch.equal(torchcl.to_cpu(k), x)
+    del waste
+
+
+def test_pages_dropped_in_a_capture_go_back_after_it(S, monkeypatch):
+    x = rnd(6, 1, 1, 64, dtype=torch.float16).cuda()
+    cache = S.KVCache(4, 16, 1, 64, "float16")
+    cache.append(x, x, torch.tensor([3], device="cuda"))
+    pages = cache._pages[:2]
+    with monkeypatch.context() as m:
+        m.setattr(S, "_capturing", lambda: True)
+        del cache
+        S.KVCache(4, 16, 1, 64, "float16")
+        assert not any(buf._freed for buf in pages)
+    S.KVCache(4, 16, 1, 64, "float16")
+    assert all(buf._freed for buf in pages)
