@@ -293,13 +293,18 @@ class KVCache:
         pool = get_buffer_pool()
         rows = num_pages * page_size * kv_heads
         quantised = format in ("int8", "float8")
-        self._pages = [pool.allocate(rows * head_dim * (1 if quantised else 2)) for _ in "kv"]
-        self._pages += [pool.allocate(rows * 4) for _ in "kv"] if quantised else [None, None]
-        for buf in self._pages:
-            if buf is not None:
-                pool.zero_fill(buf)
-        if not _ctx._capture_active:  # calls on any stream may follow: the pages are clear by then
-            L.check(L.lib().ojx_stream_synchronize(get_queue()), "KVCache")
+        data = rows * head_dim * (1 if quantised else 2)
+        self._pages = []
+        try:
+            for nbytes in (data, data, *((rows * 4, rows * 4) if quantised else ())):
+                self._pages.append(pool.allocate(nbytes))
+                pool.zero_fill(self._pages[-1])
+            if not _ctx._capture_active:  # calls on any stream may follow: the pages are clear by then
+                L.check(L.lib().ojx_stream_synchronize(get_queue()), "KVCache")
+        except Exception:
+            _free_pages(self._pages)
+            raise
+        self._pages += [None] * (4 - len(self._pages))
         self._owned = True
         self._set(num_pages, page_size, kv_heads, head_dim, format)
 

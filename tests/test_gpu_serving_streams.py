@@ -109,3 +109,19 @@ def test_pages_dropped_in_a_capture_go_back_after_it(S, monkeypatch):
         assert not any(buf._freed for buf in pages)
     S.KVCache(4, 16, 1, 64, "float16")
     assert all(buf._freed for buf in pages)
+
+
+def test_a_cache_that_does_not_fit_keeps_nothing(S):
+    from torchcl import _lib as L
+    from torchcl.runtime.memory import get_buffer_pool
+    pool = get_buffer_pool()
+    pool.empty_cache()
+    before = pool.get_stats()["active_bytes"]
+    pool.free(pool.allocate(12032 * 64 * 64 * 2))  # the keys' block is in the pool, the values' is not
+    L.check(L.lib().ojx_pool_debug_fail_next(2))
+    try:
+        with pytest.raises(MemoryError):
+            S.KVCache(12032, 64, 1, 64, "float16")
+    finally:
+        L.check(L.lib().ojx_pool_debug_fail_next(0))
+    assert pool.get_stats()["active_bytes"] == before
