@@ -90,6 +90,10 @@ def _stream(on_torch: bool):
     return torch.cuda.current_stream().cuda_stream if on_torch else get_queue()
 
 
+def _device(on_torch: bool) -> int:
+    return torch.cuda.current_device() if on_torch else _ctx.get_device()
+
+
 def _empty(shape, dtype, on_torch: bool):
     """(tensor or handle, address) of a new dense output."""
     if on_torch:
@@ -219,7 +223,7 @@ def qkv_to_cache(q, k, v, q_weight, k_weight, table, positions, cache: "KVCache"
     k (unrounded) and v go straight into `cache` at `slots` ([tokens], int32 or int64;
     a negative slot skips the token's keys and values)."""
     if _cuda(q):
-        return L.torch_binding().qkv_to_cache(q, k, v, q_weight, k_weight, table, positions, cache._address(), slots, eps,
+        return L.torch_binding().qkv_to_cache(q, k, v, q_weight, k_weight, table, positions, cache._address(q), slots, eps,
                                               interleaved)
     on_torch = _on_torch(q)
     d, dtype, _, keep = _qk_desc(on_torch, q, k, q_weight, k_weight, table, positions, eps, interleaved)
@@ -230,7 +234,7 @@ def qkv_to_cache(q, k, v, q_weight, k_weight, table, positions, cache: "KVCache"
     if math.prod(sa.shape) != d.tokens:
         raise ValueError(f"slots: {sa.shape} for {d.tokens} tokens")
     q_out, qp = _empty(_get_shape(q), dtype, on_torch)
-    L.check(L.lib().ojx_qkv_to_cache(_ref(d), _ref(v_rows), qp, _ref(cache._use(False)), sa.ptr,
+    L.check(L.lib().ojx_qkv_to_cache(_ref(d), _ref(v_rows), qp, _ref(cache._use(_device(on_torch), on_torch)), sa.ptr,
                                      int(sa.dtype == torch.int64), _stream(on_torch)), "qkv_to_cache")
     return q_out
 
@@ -263,6 +267,12 @@ def _give_back() -> None:
         torch.cuda.synchronize(device)
     for _, pages in batch:
         _free_pages(pages)
+
+
+def _one_device(*tensors) -> None:
+    where = {str(t.device) for t in tensors if t is not None}
+    if len(where) > 1:
+        raise ValueError(f"pages and steps on more than one device: {', '.join(sorted(where))}")
 
 
 class KVCache:
@@ -339,6 +349,7 @@ class KVCache:
             if t is not None and not (t.is_cuda and t.is_contiguous() and t.dtype == torch.float32
                                       and t.shape == k_pages.shape[:3]):
                 raise ValueError(f"{n}: expected dense float32 {tuple(k_pages.shape[:3])}")
+        _one_device(k_pages, v_pages, k_scale, v_scale)
         self = cls.__new__(cls)
         self._owned = False
         self._pages = [k_pages, v_pages, k_scale, v_scale]
@@ -361,7 +372,9 @@ class KVCache:
         self._where = ctypes.addressof(self._desc)
         self._shared = False  # used by calls that its pages' allocator knows nothing of
 
-    def _use(self, on_torch: bool) -> "L.KVCacheDesc":
+    def _use(self, device: int, on_torch: bool) -> "L.KVCacheDesc":
+        if device != self._device:
+            raise ValueError(f"the cache is on cuda:{self._device}, the call on cuda:{device}")
         if self._pooled == on_torch:
             self._shared = True
         if self._pooled:
@@ -370,15 +383,16 @@ class KVCache:
                     note_use(buf)  # a graph being captured must keep it
         return self._desc
 
-    def _address(self) -> int:
-        self._use(True)
+    def _address(self, t) -> int:
+        """For a call of the binding whose first tensor is t."""
+        self._use(t.get_device(), True)
         return self._where
 
     def append(self, k, v, slots) -> None:
         """Write keys and values [tokens, kv_heads, head_dim] (float32, bfloat16 or
         float16) to `slots` ([tokens], int32 or int64; a negative slot is skipped)."""
         if _cuda(k):
-            return L.torch_binding().kv_append(self._address(), k, v, slots)
+            return L.torch_binding().kv_append(self._address(k), k, v, slots)
         on_torch = _on_torch(k)
         ka, k_rows, n = _rows(k, on_torch, "k")
         if ka.shape[-2:] != (self.kv_heads, self.head_dim):
@@ -389,14 +403,14 @@ class KVCache:
         sa = _Arg(slots, on_torch, "slots", _INTS, integer=True)
         if math.prod(sa.shape) != n:
             raise ValueError(f"slots: {sa.shape} for {n} tokens")
-        L.check(L.lib().ojx_kv_append(_ref(self._use(False)), _ref(k_rows), _ref(v_rows), ojx_dtype(ka.dtype), n, sa.ptr,
+        L.check(L.lib().ojx_kv_append(_ref(self._use(_device(on_torch), on_torch)), _ref(k_rows), _ref(v_rows), ojx_dtype(ka.dtype), n, sa.ptr,
                                       int(sa.dtype == torch.int64), _stream(on_torch)), "KVCache.append")
 
     def read(self, slots, dtype: torch.dtype = torch.bfloat16):
         """(k, v), dense [tokens, kv_heads, head_dim] of `dtype`, as the cache holds them
         at `slots`; a negative slot gives zeros."""
         if _cuda(slots):
-            return L.torch_binding().kv_read(self._address(), slots, dtype)
+            return L.torch_binding().kv_read(self._address(slots), slots, dtype)
         on_torch = _on_torch(slots)
         code = ojx_dtype(dtype)
         sa = _Arg(slots, on_torch, "slots", _INTS, integer=True)
@@ -404,7 +418,7 @@ class KVCache:
         shape = (*sa.shape, self.kv_heads, self.head_dim)
         k, kp = _empty(shape, dtype, on_torch)
         v, vp = _empty(shape, dtype, on_torch)
-        L.check(L.lib().ojx_kv_read(_ref(self._use(False)), kp, vp, code, n, sa.ptr, int(sa.dtype == torch.int64),
+        L.check(L.lib().ojx_kv_read(_ref(self._use(_device(on_torch), on_torch)), kp, vp, code, n, sa.ptr, int(sa.dtype == torch.int64),
                                     _stream(on_torch)), "KVCache.read")
         return k, v
 
@@ -422,7 +436,7 @@ class KVCache:
         batch, tokens = pa.shape
         if ta.shape[0] != batch or ca.shape != (batch,) or na.shape != (batch,):
             raise ValueError(f"page_table {ta.shape}, context_lens {ca.shape}, count {na.shape} for {batch} sequences")
-        L.check(L.lib().ojx_kv_keep_path(_ref(self._use(on_torch)), ta.ptr, ta.shape[1], ca.ptr, pa.ptr, na.ptr, batch, tokens,
+        L.check(L.lib().ojx_kv_keep_path(_ref(self._use(_device(on_torch), on_torch)), ta.ptr, ta.shape[1], ca.ptr, pa.ptr, na.ptr, batch, tokens,
                                          _stream(on_torch)), "KVCache.keep_path")
 
 
@@ -463,7 +477,7 @@ def tree_attention(q, cache: KVCache, page_table, context_lens, mask=None, draft
     nothing, give zeros; nothing a query does not see reaches it, whatever it holds.
     Returns dense [batch, tokens, q_heads, head_dim]."""
     if _cuda(q):
-        return L.torch_binding().tree_attention(q, cache._address(), page_table, context_lens, mask, draft_lens, scale)
+        return L.torch_binding().tree_attention(q, cache._address(q), page_table, context_lens, mask, draft_lens, scale)
     on_torch = _on_torch(q)
     qa = _Arg(q, on_torch, "q", (torch.bfloat16, torch.float16))
     if len(qa.shape) != 4 or qa.shape[3] != cache.head_dim:
@@ -487,7 +501,7 @@ def tree_attention(q, cache: KVCache, page_table, context_lens, mask=None, draft
             raise ValueError(f"mask: shape {ma.shape} is neither {rows} nor {(batch, *rows)}")
     out, op = _empty(qa.shape, qa.dtype, on_torch)
     d = L.TreeAttentionDesc()
-    d.cache = cache._use(False)
+    d.cache = cache._use(_device(on_torch), on_torch)
     d.q, d.out = qa.ptr, op
     d.q_stride_b, d.q_stride_t, d.q_stride_h = qa.strides[:3]
     d.dtype, d.batch, d.tokens, d.q_heads = ojx_dtype(qa.dtype), batch, tokens, heads

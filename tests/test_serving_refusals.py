@@ -1,0 +1,29 @@
+"""What the serving operators refuse before any device work: caches of another device."""
+from types import SimpleNamespace
+
+import pytest
+import torch
+
+from torchcl import _lib as L
+from torchcl import serving
+
+
+def bare_cache(device, pooled=False):
+    """A KVCache without pages, as if made on `device`."""
+    cache = serving.KVCache.__new__(serving.KVCache)
+    cache._owned, cache._pooled, cache._shared, cache._pages, cache._device = False, pooled, False, [], device
+    cache._desc, cache._where = L.KVCacheDesc(), 64
+    return cache
+
+
+def test_a_cache_of_another_device_is_refused():
+    on = lambda device: SimpleNamespace(get_device=lambda: device)  # noqa: E731
+    cache = bare_cache(1)
+    assert cache._address(on(1)) == 64 and cache._use(1, False) is cache._desc
+    for call in (lambda: cache._address(on(0)), lambda: cache._use(0, False), lambda: cache._use(0, True)):
+        with pytest.raises(ValueError, match="cuda:1.*cuda:0"):
+            call()
+    where = lambda *ids: [SimpleNamespace(device=torch.device("cuda", i)) for i in ids]  # noqa: E731
+    serving._one_device(*where(0, 0), None, None)
+    with pytest.raises(ValueError, match="more than one device: cuda:0, cuda:1"):
+        serving._one_device(*where(0, 0, 1, 0))
