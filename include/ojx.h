@@ -323,7 +323,8 @@ int ojx_attention(void* out, const void* q, const void* k, const void* v, int32_
  * attention of new or drafted tokens over it, verification of drafts.  No counterpart
  * in the reference.  All calls are asynchronous on s.  Index arrays live on the device;
  * one found out of its range there is skipped and reported by the next
- * ojx_poll_device_error as OJX_ERR_INVALID.  ────────────────────────────────────── */
+ * ojx_poll_device_error as OJX_ERR_INVALID.  Pointers are aligned to their elements, or as
+ * stated.  ────────────────────────────────────────────────────────────────────── */
 
 /* element formats of a cache: 16-bit floats (the dtype's own code), or 8 bits with one
  * fp32 step per row (one head of one token): int8 holds round(x / step), e4m3 the
@@ -382,7 +383,8 @@ int ojx_qkv_to_cache(const ojx_qk_desc* d, const ojx_rows* v, void* q_out, const
 /* Keys and values [n][kv_heads][head_dim] into the cache at `slots`. */
 int ojx_kv_append(const ojx_kv_cache* cache, const ojx_rows* k, const ojx_rows* v, int32_t dtype,
                   int64_t n, const void* slots, int32_t slots_int64, ojx_stream s);
-/* The rows at `slots` as dense [n][kv_heads][head_dim] of `dtype` (zeros where skipped). */
+/* The rows at `slots` as dense [n][kv_heads][head_dim] of `dtype` (zeros where skipped);
+ * the outputs are 16-byte aligned. */
 int ojx_kv_read(const ojx_kv_cache* cache, void* k_out, void* v_out, int32_t dtype, int64_t n,
                 const void* slots, int32_t slots_int64, ojx_stream s);
 /* Keeps the accepted drafts: for every sequence b the rows of nodes path[b][0..count[b]]
@@ -399,7 +401,7 @@ int ojx_kv_keep_path(const ojx_kv_cache* cache, const int32_t* page_table, int32
 typedef struct ojx_tree_attention_desc {
   ojx_kv_cache cache;
   const void* q; /* [batch][tokens][q_heads][head_dim], strides below, rows contiguous */
-  void* out;     /* dense */
+  void* out;     /* dense, 16-byte aligned */
   int64_t q_stride_b, q_stride_t, q_stride_h;
   int32_t dtype, batch, tokens, q_heads;
   const int32_t* page_table; /* [batch][table_width] */

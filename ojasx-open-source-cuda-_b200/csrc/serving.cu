@@ -478,6 +478,7 @@ int ojx_tree_attention(const ojx_tree_attention_desc* d, ojx_stream stream) {
   if (d->batch == 0 || d->tokens == 0 || d->q_heads == 0) return OJX_OK;
   if (!d->q || !d->out || !d->context_lens || (d->table_width > 0 && !d->page_table))
     return set_error(OJX_ERR_INVALID, "ojx_tree_attention: NULL pointer");
+  if (!aligned16(d->out)) return set_error(OJX_ERR_INVALID, "ojx_tree_attention: out must be 16-byte aligned");
   if (static_cast<int64_t>(d->tokens) * d->q_heads > INT32_MAX / 2 ||
       static_cast<int64_t>(d->table_width) * c.page_size > INT32_MAX / 2 ||
       c.num_pages * c.page_size > INT32_MAX / c.kv_heads)

@@ -1,4 +1,6 @@
-"""What the serving operators refuse before any device work: caches of another device."""
+"""What the serving operators refuse before any device work: caches of another device,
+addresses that a kernel could not write."""
+import ctypes
 from types import SimpleNamespace
 
 import pytest
@@ -27,3 +29,17 @@ def test_a_cache_of_another_device_is_refused():
     serving._one_device(*where(0, 0), None, None)
     with pytest.raises(ValueError, match="more than one device: cuda:0, cuda:1"):
         serving._one_device(*where(0, 0, 1, 0))
+
+
+@pytest.mark.parametrize("tokens", [1, 40])  # few rows a key head store elements, more of them vectors
+def test_attention_refuses_an_output_that_vectors_cannot_reach(tokens):
+    some = ctypes.create_string_buffer(64)
+    at = (ctypes.addressof(some) + 15) // 16 * 16
+    d = L.TreeAttentionDesc()
+    d.cache = L.KVCacheDesc(at, at, at, at, 4, 16, 2, 64, L.KV_FORMATS["int8"])
+    d.batch, d.tokens, d.q_heads, d.dtype, d.scale, d.table_width = 1, tokens, 4, L.BF16, 1.0, 1
+    d.q = d.page_table = d.context_lens = at
+    for off in (2, 4, 8):
+        d.out = at + off
+        assert L.lib().ojx_tree_attention(ctypes.byref(d), None) == L.OJX_ERR_INVALID
+        assert "aligned" in L.last_error()
