@@ -322,8 +322,8 @@ int ojx_attention(void* out, const void* q, const void* k, const void* v, int32_
 /* ── serving: norms and rotations of queries and keys, a quantised paged cache,
  * attention of new or drafted tokens over it, verification of drafts.  No counterpart
  * in the reference.  All calls are asynchronous on s.  Index arrays live on the device;
- * one found out of its range there is skipped and reported by the next
- * ojx_poll_device_error as OJX_ERR_INVALID.  Pointers are aligned to their elements, or as
+ * one found out of its range there is skipped and reported as OJX_ERR_INVALID by the first
+ * ojx_poll_device_error after the kernel, or the graph that replays it, has run.  Pointers are aligned to their elements, or as
  * stated.  ────────────────────────────────────────────────────────────────────── */
 
 /* element formats of a cache: 16-bit floats (the dtype's own code), or 8 bits with one

@@ -90,8 +90,8 @@ int launch_attn_softmax(const float* S, int64_t ld, int64_t rows, int M, int nk,
 int launch_sum_columns(void* out, int dt_out, const void* in, int dt_in, int64_t rows, int64_t cols,
                        int64_t ld, cudaStream_t s);
 int read_and_clear_device_error(unsigned int* word);
-// The same word of the serving kernels' translation unit; read only once one of them
-// has been launched since the last look (0 otherwise).
+// The same word of the serving kernels' translation unit (0 before the first of them was
+// launched or captured on the current device).
 int read_and_clear_serving_error(unsigned int* word);
 // The first failed device-side bounds check (site, coordinate, coordinate, extent)
 // of the OJX_DEBUG_BOUNDS build; debug_bounds_build() says whether this is that build.

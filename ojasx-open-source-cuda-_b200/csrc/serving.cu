@@ -2,6 +2,7 @@
 // checks, launch shapes and workspaces.  A translation unit of its own, with its own
 // device error word, so that it compiles beside the GEMM kernels.
 #include <algorithm>
+#include <mutex>
 #include <type_traits>
 #include "tmap.h"
 #include "qk_cache.cuh"
@@ -11,21 +12,36 @@
 
 namespace ojx {
 
-static std::atomic<int> g_serving_launched{0};
+// Devices on which a serving kernel has ever been launched or recorded by a capture: their
+// error word is read at every poll from then on, for a kernel may still be running, or be
+// replayed by a graph, long after the last call.
+constexpr int MAX_DEVICES = 128;
+static std::atomic<bool> g_serving_used[MAX_DEVICES];
+static int device_slot() {
+  int dev = 0;
+  cudaGetDevice(&dev);
+  return dev >= 0 && dev < MAX_DEVICES ? dev : 0;
+}
+
+// Fetched and cleared in one step, so that no bit that is set meanwhile is lost.
+__device__ unsigned int g_taken_error = 0;
+__global__ void take_serving_error_kernel() { g_taken_error = atomicExch(&g_dev_error, 0u); }
 
 int read_and_clear_serving_error(unsigned int* word) {
   *word = 0;
-  if (!g_serving_launched.exchange(0)) return OJX_OK;
-  unsigned int zero = 0;
+  if (!g_serving_used[device_slot()].load(std::memory_order_relaxed)) return OJX_OK;
   int st = cuda_status(cudaMemcpyFromSymbol(word, g_dev_error, sizeof(unsigned int)), "read serving error word");
-  if (st) return st;
-  if (!*word) return OJX_OK;
-  return cuda_status(cudaMemcpyToSymbol(g_dev_error, &zero, sizeof(unsigned int)), "clear serving error word");
+  if (st || !*word) return st;
+  static std::mutex mu;  // (two polls share g_taken_error)
+  std::lock_guard<std::mutex> g(mu);
+  take_serving_error_kernel<<<1, 1>>>();
+  if ((st = cuda_status(cudaGetLastError(), "take serving error word"))) return st;
+  return cuda_status(cudaMemcpyFromSymbol(word, g_taken_error, sizeof(unsigned int)), "take serving error word");
 }
 
 static int launched(const char* what) {
   g_launches.fetch_add(1);
-  g_serving_launched.store(1);
+  g_serving_used[device_slot()].store(true, std::memory_order_relaxed);
   return cuda_status(cudaGetLastError(), what);
 }
 

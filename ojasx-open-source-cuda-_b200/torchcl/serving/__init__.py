@@ -12,7 +12,8 @@ handles (launched on torchcl's current stream) or torch CUDA tensors (launched o
 current stream of the current device; strided views are read in place when their last
 dimension is dense).  Integer arguments beside handles may also be CPU tensors; they are
 uploaded.  Calls are asynchronous.  An index that lies outside its range on the device is
-skipped and reported as ValueError by the next torchcl.synchronize() or to_cpu().
+skipped and reported as ValueError by the first torchcl.synchronize() or to_cpu() after the
+call has run (both wait for torchcl's streams only: synchronise torch's before, for its calls).
 The reference has no counterpart of these functions.
 """
 from __future__ import annotations

@@ -1,5 +1,5 @@
 """The serving operators beside other work: caches made on torchcl's stream and used on
-torch's, and caches dropped while calls run."""
+torch's, caches dropped while calls run, errors of calls that still run or are replayed."""
 import pytest
 import torch
 
@@ -13,6 +13,10 @@ LONG = 200_000_000  # clocks of a wait on a stream: about a tenth of a second
 def S():
     from torchcl import serving
     return serving
+
+
+def i32(*v):
+    return torch.tensor(v, dtype=torch.int32)
 
 
 def busy_torchcl():
@@ -125,3 +129,46 @@ def test_a_cache_that_does_not_fit_keeps_nothing(S):
     finally:
         L.check(L.lib().ojx_pool_debug_fail_next(0))
     assert pool.get_stats()["active_bytes"] == before
+
+
+# ── errors found on the device ───────────────────────────────────────────────
+
+def test_errors_of_calls_that_still_run_are_reported_later(S):
+    import torchcl
+    x = rnd(1, 1, 1, 64).cuda()
+    cache = S.KVCache.from_pages(*pages_for("int8", 2, 1, 16, 64))
+    torchcl.synchronize()
+    side = torch.cuda.Stream()
+    bad = torch.tensor([10 ** 6], device="cuda")
+    torch.cuda.synchronize()
+    with torch.cuda.stream(side):
+        torch.cuda._sleep(LONG)
+        cache.append(x, x, bad)
+    torchcl.synchronize()  # torchcl's stream is idle: nothing to report yet
+    side.synchronize()
+    with pytest.raises(ValueError, match="out of range"):
+        torchcl.synchronize()
+    torchcl.synchronize()  # once
+
+
+def test_errors_of_replayed_calls_are_reported(S):
+    import torchcl
+    from torchcl.api import _get_buf
+    from torchcl.jit.graph_runner import capture_graph
+    from torchcl.runtime.memory import get_buffer_pool
+    h = torchcl.to_opencl
+    cache = S.KVCache(2, 16, 1, 64, "int8")
+    x, slots = h(rnd(1, 2, 1, 64)), h(i32(3, 4))
+    cache.append(x, x, slots)
+    with capture_graph() as g:
+        cache.append(x, x, slots)
+    g.replay()
+    torchcl.synchronize()
+    get_buffer_pool().host_to_device(i32(3, 99), _get_buf(slots))
+    for _ in range(2):
+        g.replay()
+        with pytest.raises(ValueError, match="out of range"):
+            torchcl.synchronize()
+    get_buffer_pool().host_to_device(i32(3, 5), _get_buf(slots))
+    g.replay()
+    torchcl.synchronize()
