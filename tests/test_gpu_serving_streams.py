@@ -140,6 +140,7 @@ def test_errors_of_calls_that_still_run_are_reported_later(S):
     torchcl.synchronize()
     side = torch.cuda.Stream()
     bad = torch.tensor([10 ** 6], device="cuda")
+    cache.append(x, x, bad - 10 ** 6)  # (loads the kernel)
     torch.cuda.synchronize()
     with torch.cuda.stream(side):
         torch.cuda._sleep(LONG)
