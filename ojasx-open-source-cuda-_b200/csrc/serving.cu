@@ -218,14 +218,17 @@ static int plan_tree(TaParams& p, int tile_rows, int unit, int D, cudaStream_t s
 template <int D>
 static int join_tree(const TaParams& p, int tile_rows, int unit, int ctas, cudaStream_t s) {
   const int64_t all = static_cast<int64_t>(p.batch) * p.cache.kv_heads * p.tokens * p.group;
-  // (launched while the attention kernel ends: what it reads of the call's inputs overlaps)
+  // (launched while the attention kernel ends: what it reads of the call's inputs overlaps.
+  // Not so in a capture: ojx_graph_capture_end orders the recorded nodes by plain edges.)
+  cudaStreamCaptureStatus capture = cudaStreamCaptureStatusNone;
+  if (s) cudaStreamIsCapturing(s, &capture);
   cudaLaunchConfig_t cfg{};
   cfg.gridDim = dim3(static_cast<unsigned>((all + 3) / 4));
   cfg.blockDim = dim3(128);
   cfg.stream = s;
   cudaLaunchAttribute attr{};
   attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr.val.programmaticStreamSerializationAllowed = 1;
+  attr.val.programmaticStreamSerializationAllowed = capture == cudaStreamCaptureStatusNone ? 1 : 0;
   cfg.attrs = &attr;
   cfg.numAttrs = 1;
   const int st = cuda_status(cudaLaunchKernelEx(&cfg, tree_attention_parts_kernel<D>, p, tile_rows, unit, ctas), "tree_attention parts launch");

@@ -1,5 +1,6 @@
 """The serving operators beside other work: caches made on torchcl's stream and used on
-torch's, caches dropped while calls run, errors of calls that still run or are replayed."""
+torch's, caches dropped while calls run, errors of calls that still run or are replayed,
+captured decoding steps."""
 import pytest
 import torch
 
@@ -173,3 +174,39 @@ def test_errors_of_replayed_calls_are_reported(S):
     get_buffer_pool().host_to_device(i32(3, 5), _get_buf(slots))
     g.replay()
     torchcl.synchronize()
+
+
+# ── capture and replay ───────────────────────────────────────────────────────
+
+@pytest.mark.parametrize("tokens", [1, 5, 24])
+def test_a_captured_decoding_step_with_attention(S, tokens):
+    import torchcl
+    from torchcl.api import _get_buf
+    from torchcl.jit.graph_runner import capture_graph
+    from torchcl.runtime.memory import get_buffer_pool
+    h = torchcl.to_opencl
+    cache = S.KVCache(16, 16, 2, 64, "float8")
+    x = rnd(1, tokens, 8, 64, dtype=torch.bfloat16)
+    q, k, v = h(x[:, :4].contiguous()), h(x[:, 4:6].contiguous()), h(x[:, 6:].contiguous())
+    qq = h(x[:, :4].contiguous()[None])
+    table, pos = h(S.rope_table(256, 64)), h(torch.arange(tokens, dtype=torch.int32) + 40)
+    prompt = h(rnd(2, 100, 2, 64, dtype=torch.bfloat16))
+    cache.append(prompt, prompt, h(torch.arange(100, dtype=torch.int32)))
+    slots, ptab, ctx = h(torch.arange(tokens, dtype=torch.int32) + 40), h(torch.arange(16, dtype=torch.int32)[None].contiguous()), h(i32(40))
+
+    def step():
+        S.qkv_to_cache(q, k, v, None, None, table, pos, cache, slots)
+        return S.tree_attention(qq, cache, ptab, ctx)
+
+    want = torchcl.to_cpu(step())
+    with capture_graph() as g:
+        out = step()
+    g.replay()
+    torchcl.synchronize()
+    assert torch.equal(torchcl.to_cpu(out), want)
+    get_buffer_pool().host_to_device(i32(7), _get_buf(ctx))  # new inputs in place
+    again = torchcl.to_cpu(step())
+    assert not torch.equal(again, want)
+    g.replay()
+    torchcl.synchronize()
+    assert torch.equal(torchcl.to_cpu(out), again)
