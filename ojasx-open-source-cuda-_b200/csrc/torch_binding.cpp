@@ -8,6 +8,7 @@
 #include <ATen/ATen.h>
 #include <c10/cuda/CUDAStream.h>
 #include <torch/extension.h>
+#include <new>
 #include <sstream>
 #include "../../include/ojx.h"
 
@@ -40,16 +41,21 @@ void bind_entries(const py::dict& d) {
   take(d, "ojx_last_error", g.last_error);
 }
 
+// (Both exceptions are plain C++: a gradient runs on an autograd thread that does not hold the
+// interpreter's lock, and torch or pybind11 turns them into Python's where it does.)
 [[noreturn]] void refuse(const std::string& why) { throw py::value_error(why); }
+
+struct OutOfMemory : std::bad_alloc {  // MemoryError; RuntimeError from a gradient
+  explicit OutOfMemory(std::string why) : why_(std::move(why)) {}
+  const char* what() const noexcept override { return why_.c_str(); }
+  std::string why_;
+};
 
 void check(int status, const char* what) {
   if (status == OJX_OK) return;
   const std::string msg = std::string(what) + ": " + g.last_error();
   if (status == OJX_ERR_INVALID) throw py::value_error(msg);
-  if (status == OJX_ERR_OOM) {
-    PyErr_SetString(PyExc_MemoryError, msg.c_str());
-    throw py::error_already_set();
-  }
+  if (status == OJX_ERR_OOM) throw OutOfMemory(msg);
   throw std::runtime_error(msg);
 }
 
