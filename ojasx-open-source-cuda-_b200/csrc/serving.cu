@@ -45,6 +45,14 @@ static int launched(const char* what) {
   return cuda_status(cudaGetLastError(), what);
 }
 
+// Two kernels that hand over through their stream's workspace are launched one right after
+// the other: a call of another thread on the same stream must neither come between them nor
+// replace (grow) the workspace before the second one has it.
+static std::mutex& pair_mutex() {
+  static std::mutex mu;
+  return mu;
+}
+
 static bool known_dtype(int dt) { return dt == OJX_F32 || dt == OJX_BF16 || dt == OJX_F16; }
 static bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
 
@@ -238,6 +246,7 @@ static int join_tree(const TaParams& p, int tile_rows, int unit, int ctas, cudaS
 template <int FMT, int D, bool FEW>
 static int launch_tree(TaParams& p, cudaStream_t s) {
   using L = TaLayout<FMT, D, FEW>;
+  std::lock_guard<std::mutex> pair(pair_mutex());
   int ctas = 0, st = plan_tree(p, 16, L::UNIT, D, s, &ctas);
   if (st) return st;
   auto kern = tree_attention_kernel<FMT, D, FEW>;
@@ -253,6 +262,7 @@ static int launch_tree_tc(TaParams& p, cudaStream_t s) {
   auto kern = tree_attention_tc_kernel<FMT, D, QT>;
   int st = ensure_smem_attr(reinterpret_cast<const void*>(kern), L::SMEM);
   if (st) return st;
+  std::lock_guard<std::mutex> pair(pair_mutex());
   int ctas = 0;
   if ((st = plan_tree(p, QT * TC_BN, TC_BN, D, s, &ctas))) return st;
   // A TMA box holds rows of one page, so the page size decides its rows; the swizzle's
@@ -372,6 +382,7 @@ int ojx_qk_norm_rope_backward(const ojx_qk_desc* d, const ojx_rows* gq, const oj
   };
   p.q_blocks = static_cast<int>(blocks_of(d->q_heads));
   const int blocks = p.q_blocks + static_cast<int>(blocks_of(d->kv_heads));
+  std::lock_guard<std::mutex> pair(pair_mutex());
   p.partial = static_cast<float*>(stream_workspace(s, static_cast<size_t>(blocks) * p.D * 4, 9, false));
   if (!p.partial) return workspace_error();
   int smem = 8 * p.D * 4;

@@ -1,6 +1,8 @@
 """The serving operators beside other work: caches made on torchcl's stream and used on
 torch's, caches dropped while calls run, errors of calls that still run or are replayed,
-captured decoding steps."""
+captured decoding steps, calls from two threads."""
+import threading
+
 import pytest
 import torch
 
@@ -210,3 +212,47 @@ def test_a_captured_decoding_step_with_attention(S, tokens):
     g.replay()
     torchcl.synchronize()
     assert torch.equal(torchcl.to_cpu(out), again)
+
+
+# ── two threads, one stream ──────────────────────────────────────────────────
+
+def test_two_threads_on_one_stream(S):
+    """torchcl's default stream is every thread's: calls of two kernels that share a workspace,
+    of two sizes, keep to themselves."""
+    import torchcl
+    from torchcl.serving import _qk_backward
+    h = torchcl.to_opencl
+    cache = S.KVCache(64, 16, 2, 64, "float16")
+    x = h(rnd(1, 1024, 2, 64, dtype=torch.float16))
+    cache.append(x, x, h(torch.arange(1024, dtype=torch.int32)))
+
+    def attend(batch, tokens, seed):
+        q = h(rnd(seed, batch, tokens, 8, 64, dtype=torch.float16))
+        table, ctx = h(torch.arange(64, dtype=torch.int32).repeat(batch, 1)), h(torch.full((batch,), 900, dtype=torch.int32))
+        return lambda: [S.tree_attention(q, cache, table, ctx)]
+
+    def gradient(tokens, seed):
+        a = [h(rnd(seed + i, tokens, n, 64)) for i, n in enumerate((4, 2, 4, 2))]
+        w, table, pos = h(torch.ones(64)), h(S.rope_table(64, 64)), h(torch.arange(tokens, dtype=torch.int32) % 64)
+        return lambda: _qk_backward(*a, w, w, table, pos, 1e-6, False)
+
+    works = [[attend(1, 1, 2), gradient(40, 9)], [attend(5, 40, 5), gradient(3000, 19)]]
+    want = [[[torchcl.to_cpu(t) for t in f()] for f in fs] for fs in works]
+    wrong = []
+
+    def run(fs, expected):
+        try:
+            kept = [[f() for f in fs] for _ in range(100)]
+            for outs in kept:
+                for o, e in zip(outs, expected):
+                    if not all(torch.equal(torchcl.to_cpu(a), b) for a, b in zip(o, e)):
+                        wrong.append("another thread's parts")
+        except Exception as e:  # (a thread's exception would be lost)
+            wrong.append(repr(e))
+
+    threads = [threading.Thread(target=run, args=a) for a in zip(works, want)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not wrong, wrong[:3]
