@@ -127,6 +127,21 @@ void same_rows(const RowsOf& o, const char* name, int64_t tokens, int64_t heads,
 
 using MaybeTensor = std::optional<at::Tensor>;
 
+// Derivatives that `what` does not have: an input that wants one is refused, so that it is not
+// left out without a word.
+void no_tangent(const char* what, std::initializer_list<const at::Tensor*> inputs) {
+  for (const at::Tensor* t : inputs)
+    if (t && t->defined() && t->_fw_grad(0).defined()) throw std::runtime_error(std::string(what) + " has no forward-mode derivative");
+}
+void no_gradient(const char* what, std::initializer_list<const at::Tensor*> inputs) {
+  no_tangent(what, inputs);
+  if (!at::GradMode::is_enabled()) return;
+  for (const at::Tensor* t : inputs)
+    if (t && t->defined() && t->requires_grad())
+      throw std::runtime_error(std::string(what) + " has no gradient: detach its inputs, or call it under torch.no_grad()");
+}
+const at::Tensor* some(const MaybeTensor& t) { return t ? &*t : nullptr; }
+
 struct QkCall {
   ojx_qk_desc d{};
   RowsOf q, k;
@@ -221,8 +236,8 @@ struct QkGradOnce : torch::autograd::Function<QkGradOnce> {
                                                 const at::Tensor& table, const at::Tensor& positions, double eps, bool interleaved,
                                                 bool weights) {
     auto [dq, dk, dqw, dkw] = qk_backward(gq, gk, q, k, qw, kw, table, positions, eps, interleaved, weights);
-    auto some = [&](const at::Tensor& t) { return t.defined() ? t : at::empty({0}, q.options()); };
-    return {dq, dk, some(dqw), some(dkw)};
+    auto kept = [&](const at::Tensor& t) { return t.defined() ? t : at::empty({0}, q.options()); };
+    return {dq, dk, kept(dqw), kept(dkw)};
   }
   static torch::autograd::variable_list backward(torch::autograd::AutogradContext*, torch::autograd::variable_list) {
     throw std::runtime_error("qk_norm_rope: differentiable once");
@@ -260,6 +275,8 @@ struct QkFunction : torch::autograd::Function<QkFunction> {
 
 std::tuple<at::Tensor, at::Tensor> qk_norm_rope(const at::Tensor& q, const at::Tensor& k, const MaybeTensor& qw, const MaybeTensor& kw,
                                                 const at::Tensor& table, const at::Tensor& positions, double eps, bool interleaved) {
+  no_tangent("qk_norm_rope", {&q, &k, some(qw), some(kw)});
+  no_gradient("qk_norm_rope's table", {&table});
   if (at::GradMode::is_enabled() && (q.requires_grad() || k.requires_grad() || (qw && qw->requires_grad()) || (kw && kw->requires_grad()))) {
     auto out = QkFunction::apply(q, k, qw, kw, table, positions, eps, interleaved);
     return {out[0], out[1]};
@@ -270,6 +287,7 @@ std::tuple<at::Tensor, at::Tensor> qk_norm_rope(const at::Tensor& q, const at::T
 at::Tensor qkv_to_cache(const at::Tensor& q, const at::Tensor& k, const at::Tensor& v, const MaybeTensor& qw, const MaybeTensor& kw,
                         const at::Tensor& table, const at::Tensor& positions, uintptr_t cache, const at::Tensor& slots, double eps,
                         bool interleaved) {
+  no_gradient("qkv_to_cache", {&q, &k, &v, some(qw), some(kw), &table});
   const QkCall c = qk_call(q, k, qw, kw, table, positions, eps, interleaved);
   const RowsOf vr = rows_of(v, "v", q.device());
   same_rows(vr, "v", c.k.tokens, c.k.heads, c.k.dim);
@@ -282,6 +300,7 @@ at::Tensor qkv_to_cache(const at::Tensor& q, const at::Tensor& k, const at::Tens
 }
 
 void kv_append(uintptr_t cache, const at::Tensor& k, const at::Tensor& v, const at::Tensor& slots) {
+  no_gradient("KVCache.append", {&k, &v});
   const ojx_kv_cache* c = cache_at(cache);
   const at::Device dev = call_device(k);
   const RowsOf kr = rows_of(k, "k", dev), vr = rows_of(v, "v", dev);
@@ -312,6 +331,7 @@ std::tuple<at::Tensor, at::Tensor> kv_read(uintptr_t cache, const at::Tensor& sl
 
 at::Tensor tree_attention(const at::Tensor& q_in, uintptr_t cache, const at::Tensor& page_table, const at::Tensor& context_lens,
                           const MaybeTensor& mask, const MaybeTensor& draft_lens, std::optional<double> scale) {
+  no_gradient("tree_attention", {&q_in});
   const ojx_kv_cache* c = cache_at(cache);
   const at::Device dev = call_device(q_in);
   if (q_in.scalar_type() != at::kBFloat16 && q_in.scalar_type() != at::kHalf) refuse("q: expected bfloat16 or float16");
@@ -360,6 +380,7 @@ at::Tensor tree_attention(const at::Tensor& q_in, uintptr_t cache, const at::Ten
 
 std::tuple<at::Tensor, at::Tensor, at::Tensor> verify_drafts(const at::Tensor& target, const at::Tensor& tokens, const at::Tensor& parents,
                                                              const at::Tensor& uniforms, const MaybeTensor& draft) {
+  no_gradient("verify_drafts", {&target, &uniforms, some(draft)});
   const at::Device dev = call_device(target);
   if (target.dim() != 3) refuse("target_probs: shape " + shape_of(target.sizes()) + " is not [batch, nodes, vocab]");
   const at::Tensor p = dense_last(target);

@@ -7,6 +7,8 @@
     tree_attention   attention of the newest tokens (one, a chunk, or a tree of drafts) over a cache
     verify_drafts    acceptance of drafted tokens against the target's probabilities
 
+qk_norm_rope has a gradient (not for its table); the others have none, and refuse inputs that
+require one with RuntimeError, except under torch.no_grad().
 Every function takes device tensors of either kind, and returns the same kind: torchcl
 handles (launched on torchcl's current stream) or torch CUDA tensors (launched on torch's
 current stream of the current device; strided views are read in place when their last
@@ -89,6 +91,11 @@ class _Arg:
 
 def _stream(on_torch: bool):
     return torch.cuda.current_stream().cuda_stream if on_torch else get_queue()
+
+
+def _no_gradient(what: str, *inputs) -> None:
+    if torch.is_grad_enabled() and any(getattr(t, "requires_grad", False) for t in inputs):
+        raise RuntimeError(f"{what} has no gradient: detach its inputs, or call it under torch.no_grad()")
 
 
 def _device(on_torch: bool) -> int:
@@ -212,6 +219,7 @@ def qk_norm_rope(q, k, q_weight, k_weight, table, positions, eps: float = 1e-6, 
     gradient raises RuntimeError."""
     if _cuda(q):
         return L.torch_binding().qk_norm_rope(q, k, q_weight, k_weight, table, positions, eps, interleaved)
+    _no_gradient("qk_norm_rope's table", table)
     if torch.is_grad_enabled() and any(getattr(t, "requires_grad", False) for t in (q, k, q_weight, k_weight)):
         from torchcl.autograd import QKNormRopeFunction
         return QKNormRopeFunction.apply(q, k, q_weight, k_weight, table, positions, eps, interleaved)
@@ -226,6 +234,7 @@ def qkv_to_cache(q, k, v, q_weight, k_weight, table, positions, cache: "KVCache"
     if _cuda(q):
         return L.torch_binding().qkv_to_cache(q, k, v, q_weight, k_weight, table, positions, cache._address(q), slots, eps,
                                               interleaved)
+    _no_gradient("qkv_to_cache", q, k, v, q_weight, k_weight, table)
     on_torch = _on_torch(q)
     d, dtype, _, keep = _qk_desc(on_torch, q, k, q_weight, k_weight, table, positions, eps, interleaved)
     va, v_rows, _ = _rows(v, on_torch, "v", (d.tokens, d.kv_heads, d.head_dim))
@@ -394,6 +403,7 @@ class KVCache:
         float16) to `slots` ([tokens], int32 or int64; a negative slot is skipped)."""
         if _cuda(k):
             return L.torch_binding().kv_append(self._address(k), k, v, slots)
+        _no_gradient("KVCache.append", k, v)
         on_torch = _on_torch(k)
         ka, k_rows, n = _rows(k, on_torch, "k")
         if ka.shape[-2:] != (self.kv_heads, self.head_dim):
@@ -479,6 +489,7 @@ def tree_attention(q, cache: KVCache, page_table, context_lens, mask=None, draft
     Returns dense [batch, tokens, q_heads, head_dim]."""
     if _cuda(q):
         return L.torch_binding().tree_attention(q, cache._address(q), page_table, context_lens, mask, draft_lens, scale)
+    _no_gradient("tree_attention", q)
     on_torch = _on_torch(q)
     qa = _Arg(q, on_torch, "q", (torch.bfloat16, torch.float16))
     if len(qa.shape) != 4 or qa.shape[3] != cache.head_dim:
@@ -534,6 +545,7 @@ def verify_drafts(target_probs, tokens, parents, uniforms, draft_probs=None):
     Sums are exact in units of 2^-38, so results do not depend on the launch shape."""
     if _cuda(target_probs):
         return L.torch_binding().verify_drafts(target_probs, tokens, parents, uniforms, draft_probs)
+    _no_gradient("verify_drafts", target_probs, uniforms, draft_probs)
     on_torch = _on_torch(target_probs)
     pa = _Arg(target_probs, on_torch, "target_probs")
     if len(pa.shape) != 3:

@@ -1,13 +1,22 @@
-"""What the serving operators refuse and how they fail: failures inside a gradient."""
+"""What the serving operators refuse and how they fail: failures inside a gradient, derivatives
+that do not exist."""
 import subprocess
 import sys
 import textwrap
 
 import pytest
+import torch
 
 from conftest import PKG
+from test_gpu_serving import pages_for, rnd
 
 pytestmark = pytest.mark.gpu
+
+
+@pytest.fixture(scope="module")
+def S():
+    from torchcl import serving
+    return serving
 
 
 def test_out_of_memory_inside_a_gradient():
@@ -45,3 +54,43 @@ def test_out_of_memory_inside_a_gradient():
     """
     r = subprocess.run([sys.executable, "-c", textwrap.dedent(code.format(pkg=str(PKG)))], capture_output=True, text=True, timeout=250)
     assert r.returncode == 0 and "both raised" in r.stdout, (r.returncode, r.stdout[-500:], r.stderr[-2000:])
+
+
+def operands(S):
+    q, k = rnd(1, 3, 4, 64, dtype=torch.bfloat16).cuda(), rnd(2, 3, 2, 64, dtype=torch.bfloat16).cuda()
+    cache = S.KVCache.from_pages(*pages_for("int8", 4, 2, 16, 64))
+    return q, k, S.rope_table(16, 64).cuda(), torch.arange(3, device="cuda"), cache
+
+
+def test_derivatives_that_do_not_exist_are_refused(S):
+    """tree_attention, the cache and verification have none; an input that wants one says so
+    instead of losing it.  Without gradients recorded the same tensors are fine."""
+    q, k, table, pos, cache = operands(S)
+    w = torch.ones(64, dtype=torch.bfloat16, device="cuda")
+    pages, ctx = torch.arange(4).int().cuda()[None], torch.tensor([3], dtype=torch.int32, device="cuda")
+    p, tok = torch.full((1, 2, 5), 0.2, device="cuda"), torch.zeros(1, 2, dtype=torch.int32, device="cuda")
+    u = torch.full((1, 2), 0.5, device="cuda")
+    g = lambda t: t.detach().clone().requires_grad_()  # noqa: E731
+    calls = [lambda: S.qkv_to_cache(g(q), k, k, w, w, table, pos, cache, pos), lambda: S.qkv_to_cache(q, g(k), k, w, w, table, pos, cache, pos),
+             lambda: S.qkv_to_cache(q, k, g(k), w, w, table, pos, cache, pos), lambda: S.qkv_to_cache(q, k, k, g(w), w, table, pos, cache, pos),
+             lambda: S.qkv_to_cache(q, k, k, w, g(w), table, pos, cache, pos), lambda: cache.append(g(k), k, pos),
+             lambda: cache.append(k, g(k), pos), lambda: S.tree_attention(g(q)[None], cache, pages, ctx),
+             lambda: S.verify_drafts(g(p), tok, tok, u), lambda: S.verify_drafts(p, tok, tok, u, draft_probs=g(p))]
+    for call in calls:
+        with pytest.raises(RuntimeError, match="no gradient"):
+            call()
+        with torch.no_grad():
+            call()
+    with pytest.raises(RuntimeError, match="no gradient"):
+        S.qk_norm_rope(q, k, w, w, g(table), pos)
+
+
+def test_forward_mode_is_refused(S):
+    import torch.autograd.forward_ad as fwd
+    q, k, table, pos, cache = operands(S)
+    with fwd.dual_level():
+        dual = fwd.make_dual(q, torch.ones_like(q))
+        for call in (lambda: S.qk_norm_rope(dual, k, None, None, table, pos), lambda: S.qk_norm_rope(q, fwd.make_dual(k, k), None, None, table, pos),
+                     lambda: S.tree_attention(dual[None], cache, torch.arange(4).int().cuda()[None], torch.tensor([3], dtype=torch.int32, device="cuda"))):
+            with pytest.raises((RuntimeError, NotImplementedError), match="forward|no gradient|jvp"):
+                call()
