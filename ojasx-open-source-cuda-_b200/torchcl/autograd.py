@@ -28,7 +28,7 @@ from typing import Optional
 
 import torch
 
-from torchcl.api import _get_buf, _get_dtype, _get_shape, _wrap_output, is_opencl_tensor, to_opencl
+from torchcl.api import _get_buf, _get_dtype, _get_shape, _wrap_output, is_opencl_tensor, to_opencl, zeros_like
 from torchcl.ops.engine import get_engine
 
 
@@ -139,6 +139,7 @@ class QKNormRopeFunction(torch.autograd.Function):
     def forward(ctx, q, k, q_weight, k_weight, table, positions, eps=1e-6, interleaved=False):
         from torchcl.serving import _qk_forward
         ctx.save_for_backward(q, k, q_weight, k_weight, table, positions)
+        ctx.set_materialize_grads(False)  # (torch would make an unused output's zeros on the host)
         ctx._eps, ctx._interleaved = eps, interleaved
         return _qk_forward(q, k, q_weight, k_weight, table, positions, eps, interleaved)
 
@@ -147,6 +148,8 @@ class QKNormRopeFunction(torch.autograd.Function):
     def backward(ctx, grad_q, grad_k):
         from torchcl.serving import _qk_backward
         q, k, q_weight, k_weight, table, positions = ctx.saved_tensors
+        grad_q = zeros_like(q) if grad_q is None else _dev(grad_q)
+        grad_k = zeros_like(k) if grad_k is None else _dev(grad_k)
         grads = _qk_backward(grad_q, grad_k, q, k, q_weight, k_weight, table, positions, ctx._eps,
                              ctx._interleaved, want_weights=any(ctx.needs_input_grad[2:4]))
         return (*grads, None, None, None, None)

@@ -1,5 +1,5 @@
 """What the serving operators refuse and how they fail: failures inside a gradient, derivatives
-that do not exist."""
+that do not exist; and the gradient on handles."""
 import subprocess
 import sys
 import textwrap
@@ -94,3 +94,37 @@ def test_forward_mode_is_refused(S):
                      lambda: S.tree_attention(dual[None], cache, torch.arange(4).int().cuda()[None], torch.tensor([3], dtype=torch.int32, device="cuda"))):
             with pytest.raises((RuntimeError, NotImplementedError), match="forward|no gradient|jvp"):
                 call()
+
+
+def test_gradients_on_handles(S):
+    """The handles' form of the gradient: the bits of the torch form."""
+    import torchcl
+    from torchcl.serving import _qk_backward
+    h = torchcl.to_opencl
+    q, k, w = rnd(1, 9, 4, 64), rnd(2, 9, 2, 64), 1 + rnd(3, 64, scale=0.2)
+    gq, gk, table, pos = rnd(4, 9, 4, 64), rnd(5, 9, 2, 64), S.rope_table(16, 64), torch.arange(9, dtype=torch.int32)
+    got = _qk_backward(*map(h, (gq, gk, q, k, w, w, table)), pos, 1e-6, False)
+    d = [t.cuda().requires_grad_() for t in (q, k, w, w.clone())]
+    out = S.qk_norm_rope(*d, table.cuda(), pos.cuda())
+    want = torch.autograd.grad(out, d, [gq.cuda(), gk.cuda()])
+    assert all(torch.equal(torchcl.to_cpu(a), b.cpu()) for a, b in zip(got, want))
+
+
+@pytest.mark.parametrize("used", ["both", "q", "k"])
+def test_autograd_through_handles(S, used):
+    """qk_norm_rope of handles that require a gradient, and of handles that do not."""
+    import torchcl
+    h = torchcl.to_opencl
+    q, k, w = rnd(1, 9, 4, 64), rnd(2, 9, 2, 64), 1 + rnd(3, 64, scale=0.2)
+    gq, gk, table, pos = rnd(4, 9, 4, 64), rnd(5, 9, 2, 64), S.rope_table(16, 64), torch.arange(9, dtype=torch.int32)
+    pick = lambda pair: list(pair) if used == "both" else [pair[used == "k"]]  # noqa: E731
+    d = [t.cuda().requires_grad_() for t in (q, k, w, w.clone())]
+    want = torch.autograd.grad(pick(S.qk_norm_rope(*d, table.cuda(), pos.cuda())), d, [t.cuda() for t in pick((gq, gk))])
+    ours = [h(t).requires_grad_() for t in (q, k, w, w.clone())]
+    out = S.qk_norm_rope(*ours, h(table), h(pos))
+    got = torch.autograd.grad(pick(out), ours, [h(t) for t in pick((gq, gk))])
+    assert all(torch.equal(torchcl.to_cpu(a), b.cpu()) for a, b in zip(got, want))
+    cache = S.KVCache(2, 16, 2, 64, "float16")
+    for call in (lambda: cache.append(ours[1], ours[1], h(pos)), lambda: S.qk_norm_rope(h(q), h(k), None, None, h(table).requires_grad_(), h(pos))):
+        with pytest.raises(RuntimeError, match="no gradient"):
+            call()
