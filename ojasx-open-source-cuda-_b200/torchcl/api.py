@@ -167,6 +167,7 @@ def _create_lazy_unary(op_name: str, a):
         raise ValueError(f"Unknown unary op for fusion: {op_name}")
     ae = _elem(a)
     shape, dtype = _get_shape(ae), _get_dtype(ae)
+    ojx_dtype(dtype)  # index arrays are not computed with
     kind = _lazy_type(ae)
     if kind == "gemm" and len(ae._lazy_ops) < L.MAX_UNARY:
         # fold into the GEMM epilogue
@@ -210,6 +211,8 @@ def _create_lazy_binary(op_name: str, a, b):
     if op_name not in L.BINARY:
         raise ValueError(f"Unknown binary op for fusion: {op_name}")
     ae, be = _elem(a), _elem(b)
+    for e in (ae, be):
+        ojx_dtype(_get_dtype(e))
     if _lazy_type(ae) == "gemm":
         r = _fold_into_gemm(op_name, ae, be, lhs=False)
         if r is not None:
@@ -326,7 +329,8 @@ DEFERRED_UPLOAD_MIN_BYTES = 1 << 20
 
 
 def to_opencl(tensor: torch.Tensor):
-    """Copy a CPU tensor (float32 / bfloat16 / float16) to the device.
+    """Copy a CPU tensor (float32 / bfloat16 / float16) to the device, or an index array
+    (int32 / int64) of torchcl.serving, which no other operation takes.
 
     A pageable tensor is copied at once, as the reference does (api.py:210-217).
     A contiguous pinned tensor (torch's pin_memory) of 1 MiB or more is instead read
@@ -577,6 +581,7 @@ def transpose(a):
     shape = _get_shape(a)
     if len(shape) != 2:
         raise ValueError(f"transpose requires 2D tensor, got {shape}")
+    ojx_dtype(_get_dtype(a))
     ae = _elem(a)
     if _lazy_type(ae) == "transpose":
         return _wrap(ae._lazy_inputs[0])

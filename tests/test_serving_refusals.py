@@ -1,5 +1,5 @@
 """What the serving operators refuse before any device work: caches of another device,
-addresses that a kernel could not write."""
+addresses that a kernel could not write, arithmetic on index handles."""
 import ctypes
 from types import SimpleNamespace
 
@@ -43,3 +43,26 @@ def test_attention_refuses_an_output_that_vectors_cannot_reach(tokens):
         d.out = at + off
         assert L.lib().ojx_tree_attention(ctypes.byref(d), None) == L.OJX_ERR_INVALID
         assert "aligned" in L.last_error()
+
+
+@pytest.mark.parametrize("dtype", [torch.int32, torch.int64])
+def test_index_handles_are_not_computed_with(dtype):
+    """At the call, not when its result is read."""
+    import torchcl
+    from torchcl import api
+
+    def handle(t):  # an upload that waits for its first use
+        elem, _ = api._make_handle(tuple(t.shape), t.dtype)
+        elem._torchcl_host = t
+        return api._wrap(elem)
+
+    i, x = handle(torch.ones(2, 2, dtype=dtype)), handle(torch.ones(2, 2))
+    calls = [lambda: torchcl.add(i, i), lambda: torchcl.mul(x, i), lambda: torchcl.sub(i, x), lambda: torchcl.relu(i), lambda: torchcl.transpose(i),
+             lambda: torchcl.matmul(i, i), lambda: i + i, lambda: torchcl.add(torchcl.matmul(x, x), i), lambda: -i]
+    for call in calls:
+        with pytest.raises(ValueError, match="unsupported dtype"):
+            call()
+    torchcl.transpose(x)
+    for other in (torch.float64, torch.uint8, torch.bool, torch.int16):
+        with pytest.raises(ValueError, match="unsupported dtype"):
+            torchcl.to_opencl(torch.ones(2, dtype=other))
