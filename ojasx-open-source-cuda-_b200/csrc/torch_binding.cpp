@@ -1,7 +1,8 @@
 // torch_binding.cpp — the serving operators on torch CUDA tensors: argument checks, output
 // allocation and the call of libojx's C entries on torch's current stream, without
 // Python's share of the work (a small call spends ten times its kernel's duration there).
-// torchcl/serving does the same in Python for torchcl handles; both refuse alike.
+// torchcl/serving does the same in Python for torchcl handles; both refuse the same calls in
+// the same words.
 //
 // The C entries are bound by address from the libojx that torchcl loaded, so this module
 // links against torch only.
@@ -20,6 +21,7 @@ struct Entries {
   decltype(&ojx_qkv_to_cache) qkv_to_cache = nullptr;
   decltype(&ojx_kv_append) kv_append = nullptr;
   decltype(&ojx_kv_read) kv_read = nullptr;
+  decltype(&ojx_kv_keep_path) kv_keep_path = nullptr;
   decltype(&ojx_tree_attention) tree_attention = nullptr;
   decltype(&ojx_verify_drafts) verify_drafts = nullptr;
   decltype(&ojx_last_error) last_error = nullptr;
@@ -36,6 +38,7 @@ void bind_entries(const py::dict& d) {
   take(d, "ojx_qkv_to_cache", g.qkv_to_cache);
   take(d, "ojx_kv_append", g.kv_append);
   take(d, "ojx_kv_read", g.kv_read);
+  take(d, "ojx_kv_keep_path", g.kv_keep_path);
   take(d, "ojx_tree_attention", g.tree_attention);
   take(d, "ojx_verify_drafts", g.verify_drafts);
   take(d, "ojx_last_error", g.last_error);
@@ -329,6 +332,21 @@ std::tuple<at::Tensor, at::Tensor> kv_read(uintptr_t cache, const at::Tensor& sl
   return {k, v};
 }
 
+void kv_keep_path(uintptr_t cache, const at::Tensor& page_table, const at::Tensor& context_lens, const at::Tensor& path, const at::Tensor& count) {
+  const at::Device dev = call_device(path);
+  const at::Tensor p = index_of(path, "path", dev, false), t = index_of(page_table, "page_table", dev, false);
+  const at::Tensor ctx = index_of(context_lens, "context_lens", dev, false), n = index_of(count, "count", dev, false);
+  if (p.dim() != 2 || t.dim() != 2) refuse("path is [batch, tokens] and page_table [batch, pages]");
+  const int64_t batch = p.size(0);
+  if (t.size(0) != batch || ctx.dim() != 1 || ctx.size(0) != batch || n.dim() != 1 || n.size(0) != batch)
+    refuse("page_table " + shape_of(t.sizes()) + ", context_lens " + shape_of(ctx.sizes()) + ", count " + shape_of(n.sizes()) + " for " +
+           std::to_string(batch) + " sequences");
+  const auto at = [](const at::Tensor& x) { return static_cast<const int32_t*>(x.data_ptr()); };
+  check(g.kv_keep_path(cache_at(cache), at(t), static_cast<int32_t>(t.size(1)), at(ctx), at(p), at(n), batch, static_cast<int32_t>(p.size(1)),
+                       stream()),
+        "KVCache.keep_path");
+}
+
 at::Tensor tree_attention(const at::Tensor& q_in, uintptr_t cache, const at::Tensor& page_table, const at::Tensor& context_lens,
                           const MaybeTensor& mask, const MaybeTensor& draft_lens, std::optional<double> scale) {
   no_gradient("tree_attention", {&q_in});
@@ -431,6 +449,7 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("kv_read", [](uintptr_t cache, const at::Tensor& slots, const py::object& dtype) {
     return kv_read(cache, slots, torch::python::detail::py_object_to_dtype(dtype));
   });
+  m.def("kv_keep_path", &kv_keep_path);
   m.def("tree_attention", &tree_attention);
   m.def("verify_drafts", &verify_drafts);
 }

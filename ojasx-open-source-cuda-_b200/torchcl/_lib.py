@@ -271,7 +271,7 @@ def torch_binding():
                 mod = importlib.util.module_from_spec(spec)
                 spec.loader.exec_module(mod)
                 names = ("ojx_qk_norm_rope", "ojx_qk_norm_rope_backward", "ojx_qkv_to_cache", "ojx_kv_append",
-                         "ojx_kv_read", "ojx_tree_attention", "ojx_verify_drafts", "ojx_last_error")
+                         "ojx_kv_read", "ojx_kv_keep_path", "ojx_tree_attention", "ojx_verify_drafts", "ojx_last_error")
                 mod.bind({n: ctypes.cast(getattr(L, n), ctypes.c_void_p).value for n in names})
                 _torch_binding = mod
     return _torch_binding

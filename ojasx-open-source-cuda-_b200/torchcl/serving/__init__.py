@@ -35,26 +35,23 @@ from torchcl.runtime.memory import CLBuffer, get_buffer_pool, note_use
 
 _FORMAT_DTYPES = {"bfloat16": torch.bfloat16, "float16": torch.float16, "int8": torch.int8,
                   "float8": torch.float8_e4m3fn}
-_INTS = (torch.int32, torch.int64)
+_INTS, _INT32, _INT64 = (torch.int32, torch.int64), (torch.int32,), (torch.int64,)
+_FLOATS = (torch.float32, torch.bfloat16, torch.float16)
 _ref = ctypes.byref
 
 
 # ── device arguments ──────────────────────────────────────────────────────────
 
 def _cuda(t) -> bool:
-    """Whether a call is one of torch CUDA tensors: those go through the compiled binding."""
+    """Whether a call is one of torch CUDA tensors: those go through the compiled binding,
+    which checks its arguments in the same order and with the same words.  The functions
+    below serve handles."""
     return isinstance(t, torch.Tensor) and t.is_cuda
 
 
-def _on_torch(t) -> bool:
-    """True for a torch CUDA tensor, False for a torchcl handle, ValueError otherwise."""
-    if isinstance(t, torch.Tensor) and t.is_cuda:
-        if t.device.index != torch.cuda.current_device():
-            raise ValueError(f"tensor on {t.device}, but the current device is cuda:{torch.cuda.current_device()}")
-        return True
-    if is_opencl_tensor(t):
-        return False
-    raise ValueError("expected a device tensor: a torchcl handle or a torch CUDA tensor")
+def _first(t) -> None:
+    if not is_opencl_tensor(t):
+        raise ValueError("expected a device tensor: a torchcl handle or a torch CUDA tensor")
 
 
 def _strides(shape) -> tuple:
@@ -66,31 +63,28 @@ def _strides(shape) -> tuple:
 
 
 class _Arg:
-    """Address, shape, strides and dtype of one device tensor, and what keeps it alive."""
+    """Address, shape, strides and dtype of one handle, and what keeps it alive.  Index arrays
+    may also be CPU tensors: they are uploaded."""
 
     __slots__ = ("ptr", "shape", "strides", "dtype", "keep")
 
-    def __init__(self, t, on_torch: bool, name: str, dtypes=None, integer=False):
-        if integer and not on_torch and isinstance(t, torch.Tensor) and not is_opencl_tensor(t) and not t.is_cuda:
-            t = to_opencl(t)
-        if _on_torch(t) != on_torch:
-            raise ValueError(f"{name}: torch CUDA tensors and torchcl handles cannot be mixed in one call")
-        if on_torch:
-            if not integer and t.dim() and t.shape[-1] > 1 and t.stride(-1) != 1 or integer and not t.is_contiguous():
-                t = t.contiguous()
-            self.ptr, self.shape, self.strides, self.dtype = t.data_ptr(), tuple(t.shape), t.stride(), t.dtype
-            self.keep = t
-        else:
-            buf = _get_buf(t)
-            self.ptr, self.shape, self.dtype = buf.buffer, _get_shape(t), _get_dtype(t)
-            self.strides = _strides(self.shape)
-            self.keep = (t, buf)
+    def __init__(self, t, name: str, dtypes=None):
+        if dtypes in (_INTS, _INT32, _INT64) and isinstance(t, torch.Tensor) and not is_opencl_tensor(t) and not t.is_cuda:
+            if t.dtype in dtypes:
+                t = to_opencl(t)
+        elif not is_opencl_tensor(t):
+            raise ValueError(f"{name}: torch CUDA tensors and torchcl handles (or CPU tensors) cannot be mixed in one call")
+        self.shape, self.dtype = _get_shape(t), _get_dtype(t)
         if dtypes is not None and self.dtype not in dtypes:
-            raise ValueError(f"{name}: dtype {self.dtype}, expected one of {[str(d) for d in dtypes]}")
+            raise ValueError(f"{name}: expected {' or '.join(str(d).removeprefix('torch.') for d in dtypes)}")
+        buf = _get_buf(t)
+        self.ptr, self.strides, self.keep = buf.buffer, _strides(self.shape), (t, buf)
 
 
-def _stream(on_torch: bool):
-    return torch.cuda.current_stream().cuda_stream if on_torch else get_queue()
+def _code(dtype, name: str) -> int:
+    if dtype not in _FLOATS:
+        raise ValueError(f"{name}: unsupported dtype; expected float32, bfloat16 or float16")
+    return ojx_dtype(dtype)
 
 
 def _no_gradient(what: str, *inputs) -> None:
@@ -98,31 +92,25 @@ def _no_gradient(what: str, *inputs) -> None:
         raise RuntimeError(f"{what} has no gradient: detach its inputs, or call it under torch.no_grad()")
 
 
-def _device(on_torch: bool) -> int:
-    return torch.cuda.current_device() if on_torch else _ctx.get_device()
-
-
-def _empty(shape, dtype, on_torch: bool):
-    """(tensor or handle, address) of a new dense output."""
-    if on_torch:
-        out = torch.empty(shape, dtype=dtype, device="cuda")
-        return out, out.data_ptr()
+def _empty(shape, dtype):
+    """(handle, address) of a new dense output."""
     numel = math.prod(shape)
     buf = get_buffer_pool().allocate(numel * torch.empty(0, dtype=dtype).element_size(), dtype, tuple(shape))
     return _wrap_output(buf, tuple(shape), dtype), buf.buffer
 
 
-def _rows(t, on_torch, name, heads_dims=None):
-    """_Arg and L.Rows of [..., heads, head_dim] rows, leading dimensions as one."""
-    if on_torch and isinstance(t, torch.Tensor) and t.is_cuda and t.dim() > 3:
-        t = t.reshape(-1, *t.shape[-2:])
-    a = _Arg(t, on_torch, name)
+def _rows(t, name):
+    """_Arg, L.Rows and (tokens, heads, head_dim) of [..., heads, head_dim] rows, leading
+    dimensions as one."""
+    a = _Arg(t, name)
     if len(a.shape) < 3:
         raise ValueError(f"{name}: expected [tokens, heads, head_dim], got {a.shape}")
-    tokens = math.prod(a.shape[:-2])
-    if heads_dims is not None and (tokens, *a.shape[-2:]) != heads_dims:
-        raise ValueError(f"{name}: shape {a.shape} does not match {heads_dims} rows")
-    return a, L.Rows(a.ptr, a.strides[-3], a.strides[-2]), tokens
+    return a, L.Rows(a.ptr, a.strides[-3], a.strides[-2]), (math.prod(a.shape[:-2]), *a.shape[-2:])
+
+
+def _same_rows(sizes, name, want) -> None:
+    if sizes != want:
+        raise ValueError(f"{name}: shape does not match {list(want)} rows")
 
 
 # ── norms and rotations ────────────────────────────────────────────────────────
@@ -137,47 +125,48 @@ def rope_table(positions: int, rotary_dim: int, theta: float = 10000.0) -> torch
     return torch.cat([angle.cos(), angle.sin()], dim=1).float()
 
 
-def _qk_desc(on_torch, q, k, q_weight, k_weight, table, positions, eps, interleaved):
-    """(L.QkDesc, shape of q, shape of k, dtype, what must stay alive)."""
-    qa, qrows, tokens = _rows(q, on_torch, "q")
-    heads, dim = qa.shape[-2:]
-    ka, krows, _ = _rows(k, on_torch, "k", (tokens, _get_shape(k)[-2] if len(_get_shape(k)) > 2 else -1, dim))
+def _qk_desc(q, k, q_weight, k_weight, table, positions, eps, interleaved):
+    """(L.QkDesc, dtype of the rows, dtype of the weights, what must stay alive)."""
+    _first(q)
+    qa, qrows, (tokens, heads, dim) = _rows(q, "q")
+    ka, krows, k_sizes = _rows(k, "k")
+    _same_rows(k_sizes, "k", (tokens, k_sizes[1], dim))
     if ka.dtype != qa.dtype:
         raise ValueError("q and k must share a dtype")
-    wa = [None if w is None else _Arg(w, on_torch, n) for w, n in ((q_weight, "q_weight"), (k_weight, "k_weight"))]
-    for w, n in zip(wa, ("q_weight", "k_weight")):
-        if w is not None and w.shape != (dim,):
-            raise ValueError(f"{n}: shape {w.shape}, expected ({dim},)")
-    given = [w.dtype for w in wa if w is not None]
-    if len(set(given)) > 1:
-        raise ValueError("q_weight and k_weight must share a dtype")
-    ta = _Arg(table, on_torch, "table", (torch.float32,))
+    weights, weight_type = [None, None], None
+    for i, (w, name) in enumerate(((q_weight, "q_weight"), (k_weight, "k_weight"))):
+        if w is None:
+            continue
+        a = weights[i] = _Arg(w, name)
+        if a.shape != (dim,):
+            raise ValueError(f"{name}: shape {a.shape}, expected ({dim},)")
+        if weight_type not in (None, a.dtype):
+            raise ValueError("q_weight and k_weight must share a dtype")
+        weight_type = a.dtype
+    ta = _Arg(table, "table", (torch.float32,))
     if len(ta.shape) != 2 or ta.shape[1] > dim or ta.shape[1] % 2:
         raise ValueError(f"table: shape {ta.shape} is not [positions, rotary_dim] with an even rotary_dim <= {dim}")
-    if ta.strides[0] != ta.shape[1] and ta.shape[0] > 1:
-        ta = _Arg(table.contiguous(), on_torch, "table", (torch.float32,))
-    pa = _Arg(positions, on_torch, "positions", _INTS, integer=True)
+    pa = _Arg(positions, "positions", _INTS)
     if math.prod(pa.shape) != tokens:
         raise ValueError(f"positions: {pa.shape} for {tokens} tokens")
+    weight_type = weight_type or qa.dtype
     d = L.QkDesc()
-    d.tokens, d.q_heads, d.kv_heads, d.head_dim, d.rotary_dim = tokens, heads, ka.shape[-2], dim, ta.shape[1]
-    d.interleaved, d.dtype = int(bool(interleaved)), ojx_dtype(qa.dtype)
-    d.dtype_weight = ojx_dtype(given[0]) if given else d.dtype
+    d.tokens, d.q_heads, d.kv_heads, d.head_dim, d.rotary_dim = tokens, heads, k_sizes[1], dim, ta.shape[1]
+    d.interleaved, d.dtype, d.dtype_weight = int(bool(interleaved)), _code(qa.dtype, "q"), _code(weight_type, "q_weight")
     d.positions_int64, d.eps = int(pa.dtype == torch.int64), eps
     d.q, d.k = qrows, krows
-    d.q_weight, d.k_weight = (w.ptr if w is not None else None for w in wa)
+    d.q_weight, d.k_weight = (w.ptr if w is not None else None for w in weights)
     d.table, d.table_rows, d.positions = ta.ptr, ta.shape[0], pa.ptr
-    return d, qa.dtype, given[0] if given else qa.dtype, (qa, ka, wa, ta, pa)
+    return d, qa.dtype, weight_type, (qa, ka, weights, ta, pa)
 
 
 def _qk_forward(q, k, q_weight, k_weight, table, positions, eps, interleaved):
     if _cuda(q):
         return L.torch_binding().qk_forward(q, k, q_weight, k_weight, table, positions, eps, interleaved)
-    on_torch = _on_torch(q)
-    d, dtype, _, keep = _qk_desc(on_torch, q, k, q_weight, k_weight, table, positions, eps, interleaved)
-    q_out, qp = _empty(_get_shape(q), dtype, on_torch)
-    k_out, kp = _empty(_get_shape(k), dtype, on_torch)
-    L.check(L.lib().ojx_qk_norm_rope(_ref(d), qp, kp, _stream(on_torch)), "qk_norm_rope")
+    d, dtype, _, keep = _qk_desc(q, k, q_weight, k_weight, table, positions, eps, interleaved)
+    q_out, qp = _empty(_get_shape(q), dtype)
+    k_out, kp = _empty(_get_shape(k), dtype)
+    L.check(L.lib().ojx_qk_norm_rope(_ref(d), qp, kp, get_queue()), "qk_norm_rope")
     return q_out, k_out
 
 
@@ -186,21 +175,22 @@ def _qk_backward(gq, gk, q, k, q_weight, k_weight, table, positions, eps, interl
     if _cuda(q):
         return L.torch_binding().qk_backward(gq, gk, q, k, q_weight, k_weight, table, positions, eps, interleaved,
                                              want_weights)
-    on_torch = _on_torch(q)
-    d, dtype, wdtype, keep = _qk_desc(on_torch, q, k, q_weight, k_weight, table, positions, eps, interleaved)
-    ga, gq_rows, _ = _rows(gq, on_torch, "grad of q", (d.tokens, d.q_heads, d.head_dim))
-    gb, gk_rows, _ = _rows(gk, on_torch, "grad of k", (d.tokens, d.kv_heads, d.head_dim))
+    d, dtype, wdtype, keep = _qk_desc(q, k, q_weight, k_weight, table, positions, eps, interleaved)
+    ga, gq_rows, gq_sizes = _rows(gq, "grad of q")
+    gb, gk_rows, gk_sizes = _rows(gk, "grad of k")
+    _same_rows(gq_sizes, "grad of q", (d.tokens, d.q_heads, d.head_dim))
+    _same_rows(gk_sizes, "grad of k", (d.tokens, d.kv_heads, d.head_dim))
     if ga.dtype != dtype or gb.dtype != dtype:
         raise ValueError("gradients must have the dtype of q and k")
-    dq, dqp = _empty(_get_shape(q), dtype, on_torch)
-    dk, dkp = _empty(_get_shape(k), dtype, on_torch)
+    dq, dqp = _empty(_get_shape(q), dtype)
+    dk, dkp = _empty(_get_shape(k), dtype)
     out, ptrs = [], []
     for w in (q_weight, k_weight):
-        t, p = _empty((d.head_dim,), wdtype, on_torch) if w is not None and want_weights else (None, None)
+        t, p = _empty((d.head_dim,), wdtype) if w is not None and want_weights else (None, None)
         out.append(t)
         ptrs.append(p)
-    L.check(L.lib().ojx_qk_norm_rope_backward(_ref(d), _ref(gq_rows), _ref(gk_rows), dqp, dkp, *ptrs,
-                                              _stream(on_torch)), "qk_norm_rope backward")
+    L.check(L.lib().ojx_qk_norm_rope_backward(_ref(d), _ref(gq_rows), _ref(gk_rows), dqp, dkp, *ptrs, get_queue()),
+            "qk_norm_rope backward")
     return dq, dk, out[0], out[1]
 
 
@@ -235,17 +225,17 @@ def qkv_to_cache(q, k, v, q_weight, k_weight, table, positions, cache: "KVCache"
         return L.torch_binding().qkv_to_cache(q, k, v, q_weight, k_weight, table, positions, cache._address(q), slots, eps,
                                               interleaved)
     _no_gradient("qkv_to_cache", q, k, v, q_weight, k_weight, table)
-    on_torch = _on_torch(q)
-    d, dtype, _, keep = _qk_desc(on_torch, q, k, q_weight, k_weight, table, positions, eps, interleaved)
-    va, v_rows, _ = _rows(v, on_torch, "v", (d.tokens, d.kv_heads, d.head_dim))
+    d, dtype, _, keep = _qk_desc(q, k, q_weight, k_weight, table, positions, eps, interleaved)
+    va, v_rows, v_sizes = _rows(v, "v")
+    _same_rows(v_sizes, "v", (d.tokens, d.kv_heads, d.head_dim))
     if va.dtype != dtype:
         raise ValueError("q, k and v must share a dtype")
-    sa = _Arg(slots, on_torch, "slots", _INTS, integer=True)
+    sa = _Arg(slots, "slots", _INTS)
     if math.prod(sa.shape) != d.tokens:
         raise ValueError(f"slots: {sa.shape} for {d.tokens} tokens")
-    q_out, qp = _empty(_get_shape(q), dtype, on_torch)
-    L.check(L.lib().ojx_qkv_to_cache(_ref(d), _ref(v_rows), qp, _ref(cache._use(_device(on_torch), on_torch)), sa.ptr,
-                                     int(sa.dtype == torch.int64), _stream(on_torch)), "qkv_to_cache")
+    q_out, qp = _empty(_get_shape(q), dtype)
+    L.check(L.lib().ojx_qkv_to_cache(_ref(d), _ref(v_rows), qp, _ref(cache._use(_ctx.get_device(), False)), sa.ptr,
+                                     int(sa.dtype == torch.int64), get_queue()), "qkv_to_cache")
     return q_out
 
 
@@ -404,51 +394,53 @@ class KVCache:
         if _cuda(k):
             return L.torch_binding().kv_append(self._address(k), k, v, slots)
         _no_gradient("KVCache.append", k, v)
-        on_torch = _on_torch(k)
-        ka, k_rows, n = _rows(k, on_torch, "k")
-        if ka.shape[-2:] != (self.kv_heads, self.head_dim):
-            raise ValueError(f"k: rows {ka.shape[-2:]}, the cache holds {(self.kv_heads, self.head_dim)}")
-        va, v_rows, _ = _rows(v, on_torch, "v", (n, self.kv_heads, self.head_dim))
+        _first(k)
+        ka, k_rows, sizes = _rows(k, "k")
+        va, v_rows, v_sizes = _rows(v, "v")
+        if sizes[1:] != (self.kv_heads, self.head_dim):
+            raise ValueError(f"k: rows {sizes[1:]}, the cache holds {(self.kv_heads, self.head_dim)}")
+        _same_rows(v_sizes, "v", sizes)
         if va.dtype != ka.dtype:
             raise ValueError("k and v must share a dtype")
-        sa = _Arg(slots, on_torch, "slots", _INTS, integer=True)
+        n = sizes[0]
+        sa = _Arg(slots, "slots", _INTS)
         if math.prod(sa.shape) != n:
             raise ValueError(f"slots: {sa.shape} for {n} tokens")
-        L.check(L.lib().ojx_kv_append(_ref(self._use(_device(on_torch), on_torch)), _ref(k_rows), _ref(v_rows), ojx_dtype(ka.dtype), n, sa.ptr,
-                                      int(sa.dtype == torch.int64), _stream(on_torch)), "KVCache.append")
+        L.check(L.lib().ojx_kv_append(_ref(self._use(_ctx.get_device(), False)), _ref(k_rows), _ref(v_rows), _code(ka.dtype, "k"), n,
+                                      sa.ptr, int(sa.dtype == torch.int64), get_queue()), "KVCache.append")
 
     def read(self, slots, dtype: torch.dtype = torch.bfloat16):
         """(k, v), dense [tokens, kv_heads, head_dim] of `dtype`, as the cache holds them
         at `slots`; a negative slot gives zeros."""
         if _cuda(slots):
             return L.torch_binding().kv_read(self._address(slots), slots, dtype)
-        on_torch = _on_torch(slots)
-        code = ojx_dtype(dtype)
-        sa = _Arg(slots, on_torch, "slots", _INTS, integer=True)
+        _first(slots)
+        code = _code(dtype, "dtype")
+        sa = _Arg(slots, "slots", _INTS)
         n = math.prod(sa.shape)
         shape = (*sa.shape, self.kv_heads, self.head_dim)
-        k, kp = _empty(shape, dtype, on_torch)
-        v, vp = _empty(shape, dtype, on_torch)
-        L.check(L.lib().ojx_kv_read(_ref(self._use(_device(on_torch), on_torch)), kp, vp, code, n, sa.ptr, int(sa.dtype == torch.int64),
-                                    _stream(on_torch)), "KVCache.read")
+        k, kp = _empty(shape, dtype)
+        v, vp = _empty(shape, dtype)
+        L.check(L.lib().ojx_kv_read(_ref(self._use(_ctx.get_device(), False)), kp, vp, code, n, sa.ptr, int(sa.dtype == torch.int64),
+                                    get_queue()), "KVCache.read")
         return k, v
 
     def keep_path(self, page_table, context_lens, path, count) -> None:
         """After verify_drafts: move the accepted nodes' rows, at context_lens[b] +
         path[b][0..count[b]], to context_lens[b] + 0, 1, ...; the sequence then holds
         context_lens[b] + 1 + count[b] tokens."""
-        on_torch = _on_torch(path)
-        pa = _Arg(path, on_torch, "path", (torch.int32,), integer=True)
-        ta = _Arg(page_table, on_torch, "page_table", (torch.int32,), integer=True)
-        ca = _Arg(context_lens, on_torch, "context_lens", (torch.int32,), integer=True)
-        na = _Arg(count, on_torch, "count", (torch.int32,), integer=True)
+        if _cuda(path):
+            return L.torch_binding().kv_keep_path(self._address(path), page_table, context_lens, path, count)
+        _first(path)
+        pa, ta = _Arg(path, "path", _INT32), _Arg(page_table, "page_table", _INT32)
+        ca, na = _Arg(context_lens, "context_lens", _INT32), _Arg(count, "count", _INT32)
         if len(pa.shape) != 2 or len(ta.shape) != 2:
             raise ValueError("path is [batch, tokens] and page_table [batch, pages]")
         batch, tokens = pa.shape
         if ta.shape[0] != batch or ca.shape != (batch,) or na.shape != (batch,):
             raise ValueError(f"page_table {ta.shape}, context_lens {ca.shape}, count {na.shape} for {batch} sequences")
-        L.check(L.lib().ojx_kv_keep_path(_ref(self._use(_device(on_torch), on_torch)), ta.ptr, ta.shape[1], ca.ptr, pa.ptr, na.ptr, batch, tokens,
-                                         _stream(on_torch)), "KVCache.keep_path")
+        L.check(L.lib().ojx_kv_keep_path(_ref(self._use(_ctx.get_device(), False)), ta.ptr, ta.shape[1], ca.ptr, pa.ptr, na.ptr, batch,
+                                         tokens, get_queue()), "KVCache.keep_path")
 
 
 # ── attention over the cache ─────────────────────────────────────────────────
@@ -490,39 +482,38 @@ def tree_attention(q, cache: KVCache, page_table, context_lens, mask=None, draft
     if _cuda(q):
         return L.torch_binding().tree_attention(q, cache._address(q), page_table, context_lens, mask, draft_lens, scale)
     _no_gradient("tree_attention", q)
-    on_torch = _on_torch(q)
-    qa = _Arg(q, on_torch, "q", (torch.bfloat16, torch.float16))
+    _first(q)
+    qa = _Arg(q, "q", (torch.bfloat16, torch.float16))
     if len(qa.shape) != 4 or qa.shape[3] != cache.head_dim:
         raise ValueError(f"q: shape {qa.shape} is not [batch, tokens, q_heads, {cache.head_dim}]")
     batch, tokens, heads, dim = qa.shape
     if heads % cache.kv_heads:
         raise ValueError(f"{heads} query heads do not share {cache.kv_heads} key heads evenly")
-    ta = _Arg(page_table, on_torch, "page_table", (torch.int32,), integer=True)
-    ca = _Arg(context_lens, on_torch, "context_lens", (torch.int32,), integer=True)
+    ta, ca = _Arg(page_table, "page_table", _INT32), _Arg(context_lens, "context_lens", _INT32)
     if len(ta.shape) != 2 or ta.shape[0] != batch or ca.shape != (batch,):
         raise ValueError(f"page_table {ta.shape} and context_lens {ca.shape} for {batch} sequences")
     da = ma = None
     if draft_lens is not None:
-        da = _Arg(draft_lens, on_torch, "draft_lens", (torch.int32,), integer=True)
+        da = _Arg(draft_lens, "draft_lens", _INT32)
         if da.shape != (batch,):
             raise ValueError(f"draft_lens {da.shape} for {batch} sequences")
     if mask is not None:
-        ma = _Arg(mask, on_torch, "mask", (torch.int64,), integer=True)
+        ma = _Arg(mask, "mask", _INT64)
         rows = (tokens, (tokens + 63) // 64)
         if ma.shape not in (rows, (batch, *rows)):
             raise ValueError(f"mask: shape {ma.shape} is neither {rows} nor {(batch, *rows)}")
-    out, op = _empty(qa.shape, qa.dtype, on_torch)
+    out, op = _empty(qa.shape, qa.dtype)
     d = L.TreeAttentionDesc()
-    d.cache = cache._use(_device(on_torch), on_torch)
+    d.cache = cache._use(_ctx.get_device(), False)
     d.q, d.out = qa.ptr, op
     d.q_stride_b, d.q_stride_t, d.q_stride_h = qa.strides[:3]
-    d.dtype, d.batch, d.tokens, d.q_heads = ojx_dtype(qa.dtype), batch, tokens, heads
+    d.dtype, d.batch, d.tokens, d.q_heads = _code(qa.dtype, "q"), batch, tokens, heads
     d.page_table, d.table_width, d.context_lens = ta.ptr, ta.shape[1], ca.ptr
     d.draft_lens = da.ptr if da is not None else None
     if ma is not None:
         d.mask, d.mask_stride_b = ma.ptr, math.prod(ma.shape[1:]) if len(ma.shape) == 3 else 0
     d.scale = dim ** -0.5 if scale is None else scale
-    L.check(L.lib().ojx_tree_attention(_ref(d), _stream(on_torch)), "tree_attention")
+    L.check(L.lib().ojx_tree_attention(_ref(d), get_queue()), "tree_attention")
     return out
 
 
@@ -546,35 +537,34 @@ def verify_drafts(target_probs, tokens, parents, uniforms, draft_probs=None):
     if _cuda(target_probs):
         return L.torch_binding().verify_drafts(target_probs, tokens, parents, uniforms, draft_probs)
     _no_gradient("verify_drafts", target_probs, uniforms, draft_probs)
-    on_torch = _on_torch(target_probs)
-    pa = _Arg(target_probs, on_torch, "target_probs")
+    _first(target_probs)
+    pa = _Arg(target_probs, "target_probs")
     if len(pa.shape) != 3:
         raise ValueError(f"target_probs: shape {pa.shape} is not [batch, nodes, vocab]")
     batch, nodes, vocab = pa.shape
     qa = None
     if draft_probs is not None:
-        qa = _Arg(draft_probs, on_torch, "draft_probs", (pa.dtype,))
+        qa = _Arg(draft_probs, "draft_probs")
+        if qa.dtype != pa.dtype:
+            raise ValueError("draft_probs: expected the dtype of target_probs")
         if qa.shape != pa.shape:
             raise ValueError(f"draft_probs: shape {qa.shape}, target_probs has {pa.shape}")
-    xa = _Arg(tokens, on_torch, "tokens", (torch.int32,), integer=True)
-    ra = _Arg(parents, on_torch, "parents", (torch.int32,), integer=True)
-    ua = _Arg(uniforms, on_torch, "uniforms", (torch.float32,))
+    xa, ra = _Arg(tokens, "tokens", _INT32), _Arg(parents, "parents", _INT32)
+    ua = _Arg(uniforms, "uniforms", (torch.float32,))
     for a, n in ((xa, "tokens"), (ra, "parents"), (ua, "uniforms")):
         if a.shape != (batch, nodes):
             raise ValueError(f"{n}: shape {a.shape}, expected {(batch, nodes)}")
-    if ua.strides != _strides(ua.shape):
-        ua = _Arg(uniforms.contiguous(), on_torch, "uniforms")
-    path, path_p = _empty((batch, nodes), torch.int32, on_torch)
-    count, count_p = _empty((batch,), torch.int32, on_torch)
-    token, token_p = _empty((batch,), torch.int32, on_torch)
+    path, path_p = _empty((batch, nodes), torch.int32)
+    count, count_p = _empty((batch,), torch.int32)
+    token, token_p = _empty((batch,), torch.int32)
     d = L.VerifyDesc()
     d.target, d.target_stride_b, d.target_stride_t = pa.ptr, pa.strides[0], pa.strides[1]
     if qa is not None:
         d.draft, d.draft_stride_b, d.draft_stride_t = qa.ptr, qa.strides[0], qa.strides[1]
     d.vocab, d.token_ids, d.parents, d.uniforms = vocab, xa.ptr, ra.ptr, ua.ptr
     d.path, d.count, d.next_token = path_p, count_p, token_p
-    d.batch, d.tokens, d.dtype = batch, nodes, ojx_dtype(pa.dtype)
-    L.check(L.lib().ojx_verify_drafts(_ref(d), _stream(on_torch)), "verify_drafts")
+    d.batch, d.tokens, d.dtype = batch, nodes, _code(pa.dtype, "target_probs")
+    L.check(L.lib().ojx_verify_drafts(_ref(d), get_queue()), "verify_drafts")
     return path, count, token
 
 

@@ -1,5 +1,6 @@
 """What the serving operators refuse and how they fail: failures inside a gradient, derivatives
-that do not exist; and the gradient on handles."""
+that do not exist, arguments, in the same words on torch tensors and on handles; and the gradient
+on handles."""
 import subprocess
 import sys
 import textwrap
@@ -29,7 +30,7 @@ def test_out_of_memory_inside_a_gradient():
         from torchcl import _lib as L, serving
         m = L.torch_binding()
         names = ("ojx_qk_norm_rope", "ojx_qk_norm_rope_backward", "ojx_qkv_to_cache", "ojx_kv_append",
-                 "ojx_kv_read", "ojx_tree_attention", "ojx_verify_drafts", "ojx_last_error")
+                 "ojx_kv_read", "ojx_kv_keep_path", "ojx_tree_attention", "ojx_verify_drafts", "ojx_last_error")
         entries = {{n: ctypes.cast(getattr(L.lib(), n), ctypes.c_void_p).value for n in names}}
         fails = ctypes.CFUNCTYPE(ctypes.c_int, *[ctypes.c_void_p] * 8)(lambda *a: L.OJX_ERR_OOM)
         m.bind(dict(entries, ojx_qk_norm_rope_backward=ctypes.cast(fails, ctypes.c_void_p).value))
@@ -128,3 +129,55 @@ def test_autograd_through_handles(S, used):
     for call in (lambda: cache.append(ours[1], ours[1], h(pos)), lambda: S.qk_norm_rope(h(q), h(k), None, None, h(table).requires_grad_(), h(pos))):
         with pytest.raises(RuntimeError, match="no gradient"):
             call()
+
+
+def _bad_calls(S, on, other, cache):
+    """Calls that are refused, by what is wrong; `on` puts a CPU tensor where the call's tensors
+    are, `other` where they are not."""
+    f, i = (lambda *shape, dtype=torch.float16: on(torch.ones(*shape, dtype=dtype))), (lambda *shape, dtype=torch.int32: on(torch.zeros(*shape, dtype=dtype)))
+    q, k, table, pos = f(3, 4, 64), f(3, 2, 64), f(8, 64, dtype=torch.float32), i(3)
+    qk = lambda **kw: S.qk_norm_rope(**{**dict(q=q, k=k, q_weight=None, k_weight=None, table=table, positions=pos), **kw})  # noqa: E731
+    qkv = lambda **kw: S.qkv_to_cache(**{**dict(q=q, k=k, v=k, q_weight=None, k_weight=None, table=table, positions=pos, cache=cache, slots=pos), **kw})  # noqa: E731
+    tree = lambda **kw: S.tree_attention(**{**dict(q=f(2, 3, 4, 64), cache=cache, page_table=i(2, 4), context_lens=i(2)), **kw})  # noqa: E731
+    keep = lambda **kw: cache.keep_path(**{**dict(page_table=i(2, 4), context_lens=i(2), path=i(2, 3), count=i(2)), **kw})  # noqa: E731
+    p = f(2, 3, 9)
+    verify = lambda **kw: S.verify_drafts(**{**dict(target_probs=p, tokens=i(2, 3), parents=i(2, 3), uniforms=f(2, 3, dtype=torch.float32)), **kw})  # noqa: E731
+    f32 = torch.float32
+    return {
+        "q flat": lambda: qk(q=f(3, 64)), "q whole numbers": lambda: qk(q=i(3, 4, 64), k=i(3, 2, 64)), "k tokens": lambda: qk(k=f(4, 2, 64)),
+        "k dim": lambda: qk(k=f(3, 2, 32)), "k dtype": lambda: qk(k=f(3, 2, 64, dtype=f32)), "weight shape": lambda: qk(q_weight=f(32)),
+        "weights differ": lambda: qk(q_weight=f(64), k_weight=f(64, dtype=f32)), "weight whole": lambda: qk(q_weight=i(64)),
+        "table dtype": lambda: qk(table=f(8, 64)), "table odd": lambda: qk(table=f(8, 63, dtype=f32)), "table wide": lambda: qk(table=f(8, 66, dtype=f32)),
+        "table flat": lambda: qk(table=f(64, dtype=f32)), "positions count": lambda: qk(positions=i(4)), "positions dtype": lambda: qk(positions=f(3)),
+        "eps": lambda: qk(eps=-1.0), "mixed": lambda: qk(k=other(torch.ones(3, 2, 64, dtype=torch.float16))), "dim": lambda: qk(q=f(3, 4, 514), k=f(3, 2, 514)),
+        "v shape": lambda: qkv(v=f(3, 4, 64)), "v dtype": lambda: qkv(v=f(3, 2, 64, dtype=f32)), "slots count": lambda: qkv(slots=i(2)),
+        "cache heads": lambda: qkv(k=f(3, 4, 64), v=f(3, 4, 64)), "append heads": lambda: cache.append(q, q, pos), "append v": lambda: cache.append(k, q, pos),
+        "append v dtype": lambda: cache.append(k, f(3, 2, 64, dtype=f32), pos), "append slots": lambda: cache.append(k, k, i(5)),
+        "append whole": lambda: cache.append(i(3, 2, 64), i(3, 2, 64), pos), "append slots dtype": lambda: cache.append(k, k, f(3)),
+        "read dtype": lambda: cache.read(pos, dtype=torch.int32), "read slots": lambda: cache.read(f(3)),
+        "path dtype": lambda: keep(path=i(2, 3, dtype=torch.int64)), "path flat": lambda: keep(path=i(2)), "path batch": lambda: keep(count=i(3)),
+        "path pages": lambda: keep(page_table=i(3, 4)), "q single": lambda: tree(q=f(2, 3, 4, 64, dtype=f32)), "q dim": lambda: tree(q=f(2, 3, 4, 32)),
+        "q heads": lambda: tree(q=f(2, 3, 5, 64)), "table batch": lambda: tree(page_table=i(3, 4)), "table long": lambda: tree(page_table=i(2, 4, dtype=torch.int64)),
+        "contexts": lambda: tree(context_lens=i(3)), "drafts": lambda: tree(draft_lens=i(3)), "mask dtype": lambda: tree(mask=i(3, 1)),
+        "mask shape": lambda: tree(mask=i(3, 2, dtype=torch.int64)), "mask batch": lambda: tree(mask=i(3, 3, 1, dtype=torch.int64)), "scale": lambda: tree(scale=0.0),
+        "target flat": lambda: verify(target_probs=f(2, 9)), "target whole": lambda: verify(target_probs=i(2, 3, 9)), "draft dtype": lambda: verify(draft_probs=f(2, 3, 9, dtype=f32)),
+        "draft shape": lambda: verify(draft_probs=f(2, 3, 8)), "tokens dtype": lambda: verify(tokens=i(2, 3, dtype=torch.int64)), "tokens shape": lambda: verify(tokens=i(2, 4)),
+        "uniforms dtype": lambda: verify(uniforms=f(2, 3)), "uniforms shape": lambda: verify(uniforms=f(3, 2, dtype=f32)), "parents mixed": lambda: verify(uniforms=other(torch.ones(2, 3))),
+    }
+
+
+def test_both_kinds_of_tensors_are_refused_alike(S):
+    import torchcl
+    h, c = torchcl.to_opencl, lambda t: t.cuda()
+    ours, theirs = S.KVCache(4, 16, 2, 64, "float16"), S.KVCache.from_pages(*pages_for("float16", 4, 2, 16, 64))
+    handles, tensors = _bad_calls(S, h, c, ours), _bad_calls(S, c, h, theirs)
+    differ = {}
+    for what in handles:
+        said = []
+        for call in (handles[what], tensors[what]):
+            with pytest.raises(ValueError) as e:
+                call()
+            said.append(str(e.value))
+        if said[0] != said[1]:
+            differ[what] = said
+    assert not differ, differ
