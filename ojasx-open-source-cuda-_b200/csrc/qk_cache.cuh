@@ -973,6 +973,7 @@ __global__ void __launch_bounds__(256, 2) qk_rows_stream_kernel(const QkParams p
   };
 #pragma unroll 1
   for (int i = 0; i < QK_RING; ++i) issue();
+  __syncwarp();  // lane 0's s_known of these groups (later ones: the loop's)
 
   const bool on = j < p.npairs;
   int a = 0, b = 0;
@@ -1093,6 +1094,7 @@ __global__ void __launch_bounds__(256, 2) qk_grad_stream_kernel(const QkParams p
   };
 #pragma unroll 1
   for (int i = 0; i < RING; ++i) issue();
+  __syncwarp();  // lane 0's s_known of these groups (later ones: the loop's)
 
   const bool wide = (reinterpret_cast<uintptr_t>(dxs) & 31) == 0;
   const bool on = j < p.npairs;
