@@ -328,7 +328,7 @@ int ojx_attention(void* out, const void* q, const void* k, const void* v, int32_
 
 /* element formats of a cache: 16-bit floats (the dtype's own code), or 8 bits with one
  * fp32 step per row (one head of one token): int8 holds round(x / step), e4m3 the
- * nearest 8-bit float of x / step, step = max|x| / 127 or / 448 */
+ * nearest 8-bit float of x / step; step = max|x| times 1/127 or 1/448, rounded to fp32 */
 enum { OJX_KV_BF16 = OJX_BF16, OJX_KV_F16 = OJX_F16, OJX_KV_INT8 = 3, OJX_KV_FP8 = 4 };
 
 /* Pages of keys and values: [num_pages][kv_heads][page_size][head_dim] each, and for
@@ -419,7 +419,9 @@ int ojx_tree_attention(const ojx_tree_attention_desc* d, ojx_stream s);
  * draft[b][n] are the probabilities of the token after node n.  Nodes are tried in index
  * order, when their parent is the node reached; with r = target row, W = 1:
  *   accept node i when u_i * (q(x_i) * W) < r(x_i);  else r = max(r - W q, 0), W = sum(r).
- * draft NULL: q is 1 at x_i (a rejected token's r becomes 0, W falls by it).  The next
+ * draft NULL: q is 1 at x_i (a rejected token's r becomes 0, W falls by it).  Tokens are then
+ * distributed as the target's rows, provided that siblings were drawn independently of one
+ * another from their parent's draft row (without draft rows: chosen without u).  The next
  * token is the first v whose cumulated floor(r * 2^38) passes floor(u_0 * total).
  * path [batch][tokens]: nodes accepted, from the root, then -1; count [batch]: accepted
  * drafts; next_token [batch] (-1: the row holds no probability). */

@@ -116,9 +116,10 @@ static int launch_rows(QkParams& p, int dtype, bool vec, bool inter, cudaStream_
   split = std::min(split, groups);
   p.iters = (groups + split - 1) / split;
   p.blocks_per_token = (groups + p.iters - 1) / p.iters;
-  // Streaming wants every warp to have a ring's worth of groups several times over; fewer
-  // tokens leave that to prefetching in registers.  Streamed / prefetched, 40 heads of 128,
-  // bf16: 400 tokens 4.8 / 4.4 us (with int8 caching 8.7 / 9.5), 800 tokens 6.3 / 8.7 (10.2 /
+  // Streaming pays once each warp's ring fills several times; fewer tokens leave the loads to
+  // prefetching in registers.  The rule counts tokens, so that is true of many heads: with few,
+  // a warp has few groups (1537 tokens of 8 float32 heads: two), and only 40 heads of 128 were
+  // timed both ways.  Streamed / prefetched, those heads in bf16: 400 tokens 4.8 / 4.4 us (with int8 caching 8.7 / 9.5), 800 tokens 6.3 / 8.7 (10.2 /
   // 13.2), 2400 tokens 11.9 / 17.6 (18.7 / 25.5).
   const int sms = current_props().sm_count;
   const bool table_ok = !p.norm || (aligned16(p.table) && p.rotary % 4 == 0);

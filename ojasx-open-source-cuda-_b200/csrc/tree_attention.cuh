@@ -17,7 +17,9 @@
 // caches (64 sequences of up to 8191 keys, 8 key heads of 128, 4 rows: 223 us, 6.5 TB/s) and
 // instructions bound 8-bit ones (int8 174 us, e4m3 193 us, 4.2 and 3.9 TB/s): widening, the
 // products with half-empty fragments, and the softmax are about 1060 instructions a warp and
-// block of 32 keys.  Short calls are a chain of latencies (701 keys: 6.8 us).
+// block of 32 keys; half of the issue slots stay empty (fixed latencies).  With up to 8 rows of
+// 128 the 8-bit forms spill (int8 56, e4m3 112 bytes a thread at 168 registers, which twelve
+// warps leave).  Short calls are a chain of latencies (701 keys: 6.8 us).
 #pragma once
 #include "qk_cache.cuh"
 
@@ -50,8 +52,8 @@ constexpr int TA_F16 = 0, TA_BF16 = 1, TA_INT8 = 2, TA_FP8 = 3;
 // which is what the output's own rounding to f16 keeps; the sum of the weights stays in
 // fp32.  (With a second product for their next bits, f16 queries over e4m3 were off by 2.1e-4
 // of the output's norm instead of 2.9e-4, bf16 queries over int8 by 1.7e-3 either way; eight
-// trees of 48 nodes took 269 us instead of 231, a decoding batch of 64 took 202 instead of
-// 184.)  A row's largest weight (times its value's step) lies near 2^7 when its reference is
+// trees of 48 nodes took 267 us instead of 231, a decoding batch of 64 took 204 instead of
+// 183 over int8, 240 instead of 202 over e4m3.)  A row's largest weight (times its value's step) lies near 2^7 when its reference is
 // set and below 2^15 until the reference moves, so weights keep their 11 bits down to 2^-21
 // of the largest and contribute down to 2^-31 of it: a long context whose keys share what
 // one large score leaves is not lost.  (With the largest at one, and steps 2^8 apart taken

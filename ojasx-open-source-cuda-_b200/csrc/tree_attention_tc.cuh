@@ -1,15 +1,16 @@
 // tree_attention_tc.cuh — tree_attention.cuh's operator on tcgen05, for sequences whose
 // rows (tokens x query heads of a key head) fill more of a 128-row MMA tile.
 //
-// A persistent CTA takes an equal share of all 128-key tiles of the call (TaSplit): runs
+// A persistent CTA takes an equal share of all 128-key tiles of the call (TaShare): runs
 // of tiles of consecutive segments (sequence, key head, QT x 128 rows).
 //
 //   warp 13      loader: page lookups, and TMA copies of K and V.  16-bit rows go straight
 //                into the MMA's swizzled layout (boxes of 8 to 64 rows of one page); runs of
-//                8-bit rows land in a ring of half tiles, with their steps.
-//   warps 0-3    8-bit rows (with warps 16-19): widen them to f16 in the MMA's layout.  16-bit rows: zero what
-//                must not reach a product in a sequence's last tiles; or, where the page size
-//                is no multiple of eight rows, load all rows themselves with cp.async.
+//                8-bit rows land in a ring of tiles, with their steps.
+//   warps 0-3    8-bit rows (with warps 16-19): widen them to f16 in the MMA's layout.  16-bit
+//                rows: zero what must not reach a product in a sequence's last tiles; or, where
+//                the page size is no multiple of eight rows, load all rows themselves with
+//                cp.async.
 //   warps 4-11   softmax of unit 0 (4-7) and 1 (8-11), one row per thread (TMEM lane).
 //                QT = 2: a unit is a tile of 128 rows and sees every key tile.  QT = 1: both
 //                units share the rows and take alternate key tiles, joined at the end.
@@ -17,18 +18,21 @@
 //                of its next one, while the other unit is in its softmax.
 //
 // Tensor memory: S_0 [0,128), S_1 [128,256), O_0 [256, 256+D), O_1 [256+D, 256+2D).  A
-// softmax row holds its 128 scores in registers and writes the weights P_t, two 16-bit
+// softmax row walks its 128 scores twice, 64 at a time, and writes the weights P_t, two 16-bit
 // values a column, over S_t, from where the second product reads them (its A operand);
 // shared memory is left to K and V.  bf16 values need bf16 weights, whose eight bits would
 // double the output's rounding: each 32 columns keep the weights' next eight bits in their
 // second half, and a second product adds them.
 // K and V are produced in the order in which the MMAs consume them.
 //
-// Measured (8 trees of 48 nodes over up to 16000 keys, 8 key heads of 128, 192 rows): f16 115 us
-// (3.4 TB/s; the units' chains scores -> softmax -> product, 2300 cycles of softmax a tile),
-// e4m3 212 us (5400 cycles of softmax a tile, for two steps a key; four widening warps instead
-// of eight: 243).  2 trees of 16 nodes over 131000 keys, 4 key heads of 128, bf16: 104 us (4.3
-// TB/s; scores, product and the product of the weights' low bits are 1536 cycles a tile of 2750).
+// Measured (8 trees of 48 nodes over up to 16000 keys, 8 key heads of 128, 192 rows: 37 tiles a
+// CTA): f16 115 us (3.4 TB/s), of a tile 2300 cycles softmax of a unit; e4m3 212 us at 1965 MHz,
+// 11,200 cycles a tile, of which a unit's softmax takes 5400, for two steps a key (four widening
+// warps instead of eight: 243 us).  2 trees of 16 nodes over 131000 keys, 4 key heads of 128,
+// bf16, 46 tiles a CTA: 105 us after a pause, 116 in a loop that the power cap holds at 1640 MHz
+// (3.9 TB/s; 4100 cycles a tile, of which scores, product and the product of the weights' low
+// bits take 1536).  What the rest of a tile waits for has not been counted warp by warp.
+// Registers: the 8-bit forms spill 44 to 84 bytes a thread at their 96, the 16-bit ones 4.
 #pragma once
 #include "tree_attention.cuh"
 

@@ -280,7 +280,7 @@ class KVCache:
 
     format "bfloat16" or "float16" stores rows as they are; "int8" and "float8" (e4m3)
     store eight bits an element and one float32 step per row (a head of a token):
-    step = max|x| / 127 or / 448, read back as stored * step.  A row with a NaN or an
+    step = max|x| * (1/127 or 1/448, in float32), read back as stored * step.  A row with a NaN or an
     infinity reads back as NaN.  Token slot s is row s % page_size of page s // page_size;
     which pages make up a sequence is the caller's page table.  head_dim is a multiple of
     16 up to 512 (64 or 128 for tree_attention).
@@ -478,7 +478,10 @@ def tree_attention(q, cache: KVCache, page_table, context_lens, mask=None, draft
     [tokens, words] or [batch, tokens, words]) or, without a mask, j <= i.  tokens = 1
     without a mask is a decoding step.  Queries i >= draft_lens[b], and queries that see
     nothing, give zeros; nothing a query does not see reaches it, whatever it holds.
-    Returns dense [batch, tokens, q_heads, head_dim]."""
+    Over float16 and 8-bit caches weights count with 11 bits, down to 2^-31 of a row's largest
+    (times its value's step); bfloat16 caches keep 17.  Scratch comes from the library, so
+    torchcl's capture_graph records the call and torch.cuda.graph does not (RuntimeError), as
+    for qk_norm_rope's gradient.  Returns dense [batch, tokens, q_heads, head_dim]."""
     if _cuda(q):
         return L.torch_binding().tree_attention(q, cache._address(q), page_table, context_lens, mask, draft_lens, scale)
     _no_gradient("tree_attention", q)
@@ -530,7 +533,10 @@ def verify_drafts(target_probs, tokens, parents, uniforms, draft_probs=None):
     uniforms float32 [batch, nodes] in [0, 1): u_i decides node i, u_0 the next token.
     Nodes are tried in order, when their parent is the node reached; a rejection leaves
     max(p - q, 0) (or p without the token), renormalised, to the next child and finally to
-    the next token, so accepted tokens and the next one are distributed as the target's.
+    the next token.  Accepted tokens and the next one are distributed as the target's if the
+    children of a node were drawn independently of one another from its row of draft_probs
+    (twice the same token included; children drawn without replacement are not that), or,
+    without draft_probs, were chosen without a look at uniforms.
     Returns int32 path [batch, nodes] (the root and the accepted nodes, then -1), count
     [batch] (accepted drafts) and next_token [batch] (-1: the row holds no probability).
     Sums are exact in units of 2^-38, so results do not depend on the launch shape."""
