@@ -90,8 +90,10 @@ int launch_attn_softmax(const float* S, int64_t ld, int64_t rows, int M, int nk,
 int launch_sum_columns(void* out, int dt_out, const void* in, int dt_in, int64_t rows, int64_t cols,
                        int64_t ld, cudaStream_t s);
 int read_and_clear_device_error(unsigned int* word);
-// The same word of the serving kernels' translation unit (0 before the first of them was
-// launched or captured on the current device).
+int device_error_address(const unsigned int** address);
+// The same word of the serving kernels' translation unit (NULL before the first of them was
+// launched or captured on the current device).  One poll at a time reads and clears.
+int serving_error_address(const unsigned int** address);
 int read_and_clear_serving_error(unsigned int* word);
 // The first failed device-side bounds check (site, coordinate, coordinate, extent)
 // of the OJX_DEBUG_BOUNDS build; debug_bounds_build() says whether this is that build.

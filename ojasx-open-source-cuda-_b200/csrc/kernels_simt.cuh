@@ -358,11 +358,18 @@ int read_bounds_info(long long info[4]) {
 
 bool debug_bounds_build() { return kDebugBounds; }
 
+int device_error_address(const unsigned int** address) {
+  void* p = nullptr;
+  int st = cuda_status(cudaGetSymbolAddress(&p, g_dev_error), "device error word");
+  *address = static_cast<const unsigned int*>(p);
+  return st;
+}
+
 int read_and_clear_device_error(unsigned int* word) {
   unsigned int zero = 0;
   int st = cuda_status(cudaMemcpyFromSymbol(word, g_dev_error, sizeof(unsigned int)),
                        "read device error word");
-  if (st) return st;
+  if (st || !*word) return st;
   return cuda_status(cudaMemcpyToSymbol(g_dev_error, &zero, sizeof(unsigned int)),
                      "clear device error word");
 }

@@ -353,11 +353,26 @@ int ojx_synchronize(void) { return cuda_status(cudaDeviceSynchronize(), "cudaDev
 const char* ojx_last_error(void) { return t_last_error.c_str(); }
 
 int ojx_poll_device_error(void) {
-  unsigned int w = 0;
-  int st = read_and_clear_device_error(&w);
-  if (st) return st;
-  unsigned int serving = 0;
-  if ((st = read_and_clear_serving_error(&serving))) return st;
+  // Both units' words come with one wait (into pinned memory); they are fetched and cleared
+  // only where one is set.  Polls take turns.
+  static std::mutex mu;
+  static unsigned int* words = nullptr;
+  std::lock_guard<std::mutex> turn(mu);
+  int st = OJX_OK;
+  if (!words && (st = cuda_status(cudaHostAlloc(reinterpret_cast<void**>(&words), 2 * sizeof(unsigned int), cudaHostAllocPortable),
+                                  "error words")))
+    return st;
+  const unsigned int* at[2] = {nullptr, nullptr};
+  if ((st = device_error_address(&at[0])) || (st = serving_error_address(&at[1]))) return st;
+  words[0] = words[1] = 0;
+  for (int i = 0; i < 2; ++i)
+    if (at[i] && (st = cuda_status(cudaMemcpyAsync(words + i, at[i], sizeof(unsigned int), cudaMemcpyDeviceToHost, nullptr),
+                                   "read error words")))
+      return st;
+  if ((st = cuda_status(cudaStreamSynchronize(nullptr), "read error words"))) return st;
+  unsigned int w = words[0], serving = words[1];
+  if (w && (st = read_and_clear_device_error(&w))) return st;
+  if (serving && (st = read_and_clear_serving_error(&serving))) return st;
   w |= serving & 1u;  // (bounds records are kept by the GEMM kernels' unit only)
   if (w & 2u) {  // bit 1: a debug-build bounds check failed (sm100.cuh, OJX_DEVERR_BOUNDS)
     long long info[4] = {0, 0, 0, 0};

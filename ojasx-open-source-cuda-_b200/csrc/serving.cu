@@ -27,13 +27,17 @@ static int device_slot() {
 __device__ unsigned int g_taken_error = 0;
 __global__ void take_serving_error_kernel() { g_taken_error = atomicExch(&g_dev_error, 0u); }
 
-int read_and_clear_serving_error(unsigned int* word) {
-  *word = 0;
+int serving_error_address(const unsigned int** address) {
+  *address = nullptr;
   if (!g_serving_used[device_slot()].load(std::memory_order_relaxed)) return OJX_OK;
-  int st = cuda_status(cudaMemcpyFromSymbol(word, g_dev_error, sizeof(unsigned int)), "read serving error word");
-  if (st || !*word) return st;
-  static std::mutex mu;  // (two polls share g_taken_error)
-  std::lock_guard<std::mutex> g(mu);
+  void* p = nullptr;
+  int st = cuda_status(cudaGetSymbolAddress(&p, g_dev_error), "serving error word");
+  *address = static_cast<const unsigned int*>(p);
+  return st;
+}
+
+int read_and_clear_serving_error(unsigned int* word) {
+  int st = OJX_OK;
   take_serving_error_kernel<<<1, 1>>>();
   if ((st = cuda_status(cudaGetLastError(), "take serving error word"))) return st;
   return cuda_status(cudaMemcpyFromSymbol(word, g_taken_error, sizeof(unsigned int)), "take serving error word");
