@@ -60,7 +60,9 @@ constexpr int TA_F16 = 0, TA_BF16 = 1, TA_INT8 = 2, TA_FP8 = 3;
 // as the largest of them, 65536 keys of 2^-16 of the largest weight each added nothing.)
 constexpr float TA_BIAS = 7.0f;
 // Value steps whose powers of two differ by no more than this are taken as the largest of
-// their block, which costs that many of the bits above.
+// their block, which costs that many of the bits above.  (Where all blocks' steps lie further
+// apart, eight e4m3 trees of 48 nodes take 246 us instead of 231, an int8 decoding batch of 64
+// takes 192 instead of 185.)
 constexpr int TA_NEAR = 2;
 // log2 of the value steps that weights are measured in.  Above, no product passes f16's range
 // up to the largest float there is (2^121 a step); the weights' own sum keeps 2^-11 of the

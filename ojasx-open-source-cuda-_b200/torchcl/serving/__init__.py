@@ -333,7 +333,8 @@ class KVCache:
     def from_pages(cls, k_pages, v_pages, k_scale=None, v_scale=None) -> "KVCache":
         """A cache over dense torch CUDA tensors: pages [num_pages, kv_heads, page_size,
         head_dim] of bfloat16, float16, int8 or float8_e4m3fn, and for the last two the
-        steps, float32 [num_pages, kv_heads, page_size]."""
+        steps, float32 [num_pages, kv_heads, page_size], none of them negative; all on one
+        device."""
         formats = {v: k for k, v in _FORMAT_DTYPES.items()}
         for t, n in ((k_pages, "k_pages"), (v_pages, "v_pages")):
             if not (isinstance(t, torch.Tensor) and t.is_cuda and t.is_contiguous() and t.dim() == 4):
